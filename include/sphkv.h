@@ -245,6 +245,7 @@ typedef struct sphkv_decode_params {
                                    exchange, did not arrive within the kernel's bounded
                                    wait; the output is not valid                      */
 #define SPHKV_ST_INTERNAL 16    /* the kernel found its shared memory misaligned      */
+#define SPHKV_ST_BAD_LENGTH 32  /* a sequence's token numbers do not fit (block cache) */
 
 int64_t sphkv_decode_scratch_bytes(int32_t B, int32_t Hkv, int32_t dh, int32_t n_ctas);
 /* What a decode of n_units = B * Hkv units has in a block's shared memory: the teams of warps that
@@ -400,11 +401,75 @@ int sphkv_ragged_logits(const uint8_t* pages, const int32_t* ptable, const int32
 int sphkv_omega_ema(const float* ml, float* omega, int32_t n_units, int32_t kv_groups,
                     int32_t max_blocks, int32_t stride, float beta, void* stream);
 
+/* ---- 8-bit block cache ----------------------------------------------------------------
+ * Keys and values in 8 bits with one fp32 scale for each page (block of page_size tokens), head
+ * and side, for tokens that are not held in spherical pages.  No counterpart in the reference.
+ * A value is code * scale; codes are whole numbers -127 .. 127 or e4m3 floats.  Token t of
+ * sequence b lies in slot t % page_size of page block_table[b][t / page_size]; a page holds all KV
+ * heads of its tokens.  Keys are stored as they come (post-RoPE for sphkv_blocks_decode / _attend).
+ *
+ * Every call is about the last n_b tokens of each sequence, positions ends[b] - n_b .. ends[b] - 1.
+ * Their rows in the dense tensors are cu[b] .. cu[b + 1] - 1 (cu: device i32 [B + 1], ascending from
+ * 0; rows from cu[B] on are left alone), or b * n .. b * n + n - 1 with n = rows / B where cu is NULL.
+ * A sequence whose numbers do not fit (ends outside [0, max_blocks * page_size], cu not ascending
+ * within [0, rows], n_b > ends[b]) is left out and raises SPHKV_ST_BAD_LENGTH in *status; a table
+ * entry outside [0, n_pages) raises SPHKV_ST_BAD_BLOCK and its tokens count as absent. */
+#define SPHKV_BLOCKS_I8 0
+#define SPHKV_BLOCKS_E4M3 1
+
+typedef struct sphkv_blocks {
+  void *k_codes, *v_codes;    /* [n_pages][Hkv][page_size][dh], 16-byte aligned            */
+  float *k_scale, *v_scale;   /* [n_pages][Hkv]                                          */
+  const int32_t* block_table; /* [B][max_blocks]; entries past a sequence's end are not read */
+  const int32_t* ends;        /* [B] tokens held, the ones of this call among them       */
+  int32_t* status;            /* optional device int, OR-ed with SPHKV_ST_* bits         */
+  int32_t n_pages, Hkv, page_size, dh, B, max_blocks; /* page_size 16..128, dh 64 or 128  */
+  int32_t store;              /* SPHKV_BLOCKS_*                                           */
+} sphkv_blocks;
+
+/* Quantises new tokens into their pages.  k, v: dense rows of `dtype`, elements contiguous along
+ * dh, strides in elements.  Per page, head and side: scale' = max |x| / top over the new tokens
+ * (top = 127 or 448, rounded to fp32); a page that held earlier tokens of the sequence keeps
+ * max(scale, scale') and its codes are re-quantised where that is larger.  Codes are the nearest
+ * to x / scale' (the exact quotient, ties to even).  A scale below 2^-126 becomes 0 with codes 0.
+ * Where a new x is not finite, its page, head and side get an infinite or NaN scale and codes 0:
+ * they read back as NaN.  Pages that receive tokens must not be shared by two sequences. */
+int sphkv_blocks_append(const sphkv_blocks* c, const void* k, const void* v, int32_t dtype, int64_t k_row_stride,
+                        int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride, const int32_t* cu,
+                        int64_t rows, void* stream);
+
+/* The values of those tokens as dense contiguous rows [rows][Hkv][dh] of `dtype` (16-byte aligned);
+ * tokens of a bad table entry are written as zeros. */
+int sphkv_blocks_read(const sphkv_blocks* c, void* k_out, void* v_out, int32_t dtype, const int32_t* cu, int64_t rows,
+                      void* stream);
+
+/* Attention of the last token of every sequence over its keys first[b] .. ends[b] - 1 (first: optional
+ * device i32 [B], negative = 0).  q [B][Hq][dh] with strides in elements; out [B][Hq][dh] (optional)
+ * of out_dtype and out_partial f32 [B][Hq][dh + 2] = (max, sum, acc) as sphkv_decode_paged writes it
+ * (optional; sphkv_merge_partials takes both together).  A sequence without keys gets zeros and
+ * (-inf, 0, 0).  Hq / Hkv <= SPHKV_MAX_GQA.  scratch: sphkv_blocks_decode_scratch_bytes() bytes, 256-aligned, free
+ * for other use when the call's kernels are done.  Two launches; the first may become resident while the
+ * kernel before it in the stream still runs, and waits for it before it reads or writes memory. */
+int64_t sphkv_blocks_decode_scratch_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t dh);
+int sphkv_blocks_decode(const sphkv_blocks* c, const void* q, int32_t q_dtype, int64_t q_row_stride,
+                        int64_t q_head_stride, const int32_t* first, void* out, int32_t out_dtype,
+                        float* out_partial, void* scratch, int64_t scratch_bytes, int32_t Hq, float sm_scale,
+                        void* stream);
+
+/* Causal attention of the last n_b tokens of every sequence: the query at position p sees keys
+ * first[b] .. p.  q [rows][Hq][dh] (16-bit types), out [rows][Hq][dh] contiguous; a query without keys gets zeros.
+ * Rows past cu[B] are not written. */
+int64_t sphkv_blocks_attend_scratch_bytes(int32_t B, int64_t rows, int32_t Hq, int32_t Hkv, int32_t dh);
+int sphkv_blocks_attend(const sphkv_blocks* c, const void* q, int32_t q_dtype, int64_t q_row_stride,
+                        int64_t q_head_stride, const int32_t* cu, int64_t rows, const int32_t* first, void* out,
+                        int32_t out_dtype, void* scratch, int64_t scratch_bytes, int32_t Hq, float sm_scale,
+                        void* stream);
+
 /* ---- Library ---------------------------------------------------------------------*/
 int sphkv_abi_version(void);
 const char* sphkv_last_error(void);
 /* sizeof() of sphkv_tiers (0), sphkv_encode_params (1), sphkv_decode_params (2),
- * sphkv_page_lists_params (4) as this library was compiled (-1 for other values); foreign-language
+ * sphkv_page_lists_params (4), sphkv_blocks (5) as this library was compiled (-1 for other values); foreign-language
  * bindings compare it with their own layout. */
 int sphkv_struct_size(int which);
 /* Number of SMs of the current device (grid sizing), or a negative error. */

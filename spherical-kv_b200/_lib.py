@@ -16,7 +16,8 @@ F32, BF16, F16 = 0, 1, 2
 RADIUS_I8, RADIUS_F16 = 0, 1
 MAX_TIER_SLOTS = 4
 MAX_GQA = 8
-ST_BAD_POSITION, ST_BAD_BLOCK, ST_BAD_SLOT, ST_TIMEOUT, ST_INTERNAL = 1, 2, 4, 8, 16
+ST_BAD_POSITION, ST_BAD_BLOCK, ST_BAD_SLOT, ST_TIMEOUT, ST_INTERNAL, ST_BAD_LENGTH = 1, 2, 4, 8, 16, 32
+BLOCKS_I8, BLOCKS_E4M3 = 0, 1
 
 _I4 = C.c_int32 * MAX_TIER_SLOTS
 
@@ -86,6 +87,16 @@ class PageListsParams(C.Structure):
     ]
 
 
+class Blocks(C.Structure):
+    _fields_ = [
+        ("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("block_table", C.c_void_p), ("ends", C.c_void_p), ("status", C.c_void_p),
+        ("n_pages", C.c_int32), ("Hkv", C.c_int32), ("page_size", C.c_int32), ("dh", C.c_int32), ("B", C.c_int32),
+        ("max_blocks", C.c_int32), ("store", C.c_int32),
+    ]
+    packer = struct.Struct("@7P7i4x")
+
+
 # name -> (restype, argtypes); every symbol include/sphkv.h declares
 SIGNATURES = {
     "sphkv_abi_version": (C.c_int, []),
@@ -124,6 +135,17 @@ SIGNATURES = {
                                          C.c_int32] + [C.c_void_p] * 4 + [C.c_int32] * 3 + [C.c_void_p]),
     "sphkv_kmeans_assign": (C.c_int, [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_int32] + [C.c_void_p] * 5),
     "sphkv_pool_append_step": (C.c_int, [C.c_void_p] * 12 + [C.c_int32] * 10 + [C.c_void_p]),
+    # the cache struct of the block functions goes in as its packed bytes
+    "sphkv_blocks_append": (C.c_int, [C.c_char_p, C.c_void_p, C.c_void_p, C.c_int32] + [C.c_int64] * 4 +
+                            [C.c_void_p, C.c_int64, C.c_void_p]),
+    "sphkv_blocks_read": (C.c_int, [C.c_char_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p]),
+    "sphkv_blocks_decode_scratch_bytes": (C.c_int64, [C.c_int32] * 4),
+    "sphkv_blocks_decode": (C.c_int, [C.c_char_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p,
+                                      C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_float, C.c_void_p]),
+    "sphkv_blocks_attend_scratch_bytes": (C.c_int64, [C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_int32]),
+    "sphkv_blocks_attend": (C.c_int, [C.c_char_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_void_p, C.c_int64,
+                                      C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_int32, C.c_float,
+                                      C.c_void_p]),
 }
 
 _lib = None
@@ -151,7 +173,7 @@ def load() -> C.CDLL:
     ver = lib.sphkv_abi_version()
     if ver != 4:
         raise SphKVError(f"libsphkv_b200.so ABI version {ver}, expected 4")
-    for which, st in ((0, Tiers), (1, EncodeParams), (2, DecodeParams), (4, PageListsParams)):
+    for which, st in ((0, Tiers), (1, EncodeParams), (2, DecodeParams), (4, PageListsParams), (5, Blocks)):
         if lib.sphkv_struct_size(which) != C.sizeof(st):
             raise SphKVError(f"struct layout mismatch for {st.__name__}: library "
                              f"{lib.sphkv_struct_size(which)} B, binding {C.sizeof(st)} B")

@@ -1,0 +1,124 @@
+// What the kernels of the 8-bit block cache share: which tokens a piece of work is about, and 8-bit codes to and from floats.
+#pragma once
+#include "tcgen05.cuh"
+
+namespace sphkv {
+
+// A call's dense rows: `rows` of them, cut into sequences by cu, or evenly where cu is NULL.
+struct BlockRows {
+  const int32_t* cu;
+  int32_t rows, even;  // even: rows / B
+  bool lone;           // one row a sequence that need not be among its tokens: a sequence may be empty
+};
+
+// Work on the n_b tokens of every sequence is dealt in pieces (pages that they touch; groups of queries) through a fixed
+// number of slots that the host can tell without reading cu: a sequence has at most (n_b >> shift) + extra pieces, and
+// its slots start at (cu[b] >> shift) + extra * b, which leaves room for (n_b >> shift) + extra of them.
+__host__ __device__ inline int block_slots_even(int n, int shift, int extra) {  // of one sequence
+  return n <= 0 ? 0 : ((n + (1 << shift) - 1) >> shift) + extra - 1;
+}
+inline int64_t block_slots(const BlockRows& r, int B, int shift, int extra) {
+  if (r.cu == nullptr) return (int64_t)B * block_slots_even(r.even, shift, extra);
+  return ((int64_t)r.rows >> shift) + (int64_t)extra * B;
+}
+
+struct BlockPiece {
+  int b, j;     // sequence, and the piece's number in it; b < 0: no such sequence
+  int row0, n;  // the sequence's dense rows
+  int end;      // its tokens; negative: they do not fit, and the status word says so
+};
+__device__ __forceinline__ void bad_status(const sphkv_blocks& c, int bit) {
+  if (c.status) atomicOr(c.status, bit);
+}
+__device__ __forceinline__ BlockPiece checked_piece(const sphkv_blocks& c, const BlockRows& r, int b, int j, int lo, int hi) {
+  BlockPiece p = {b, j, lo, hi - lo, 0};
+  if (b < 0 || lo < 0 || hi < lo || hi > r.rows) {
+    if (b >= 0) bad_status(c, SPHKV_ST_BAD_LENGTH);
+    p.b = -1;
+    p.n = 0;
+    return p;
+  }
+  p.end = c.ends[b];
+  if (p.end < 0 || p.end > (int64_t)c.max_blocks * c.page_size || (p.n > p.end && !r.lone)) {
+    bad_status(c, SPHKV_ST_BAD_LENGTH);
+    p.end = -1;
+  }
+  return p;
+}
+__device__ __forceinline__ int slot_base(const BlockRows& r, int b, int shift, int extra) {
+  return (min(max(r.cu[b], 0), r.rows) >> shift) + extra * b;
+}
+
+// Called by whole warps; every lane gets the answer.
+__device__ __forceinline__ BlockPiece find_piece(const sphkv_blocks& c, const BlockRows& r, int slot, int shift, int extra) {
+  if (r.cu == nullptr) {
+    const int per = block_slots_even(r.even, shift, extra), b = slot / per;
+    return checked_piece(c, r, b, slot - b * per, b * r.even, (b + 1) * r.even);
+  }
+  int b = -1, base = 0;
+  for (int b0 = 0; b0 < c.B; b0 += 32) {
+    const int i = b0 + (threadIdx.x & 31);
+    const int mine = i < c.B ? slot_base(r, i, shift, extra) : 0x7fffffff;
+    const unsigned below = __ballot_sync(0xffffffffu, mine <= slot);
+    if (below == 0) break;
+    const int last = 31 - __clz(below);
+    b = b0 + last;
+    base = __shfl_sync(0xffffffffu, mine, last);
+    if (last < 31) break;
+  }
+  return checked_piece(c, r, b, slot - base, b < 0 ? 0 : r.cu[b], b < 0 ? 0 : r.cu[b + 1]);
+}
+// The same by one thread.
+__device__ __forceinline__ BlockPiece find_piece_alone(const sphkv_blocks& c, const BlockRows& r, int slot, int shift, int extra) {
+  if (r.cu == nullptr) {
+    const int per = block_slots_even(r.even, shift, extra), b = slot / per;
+    return checked_piece(c, r, b, slot - b * per, b * r.even, (b + 1) * r.even);
+  }
+  int lo = 0, hi = c.B;  // the last sequence whose slots begin at or before this one
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    (slot_base(r, mid, shift, extra) <= slot ? lo : hi) = mid;
+  }
+  return checked_piece(c, r, lo, slot - slot_base(r, lo, shift, extra), r.cu[lo], r.cu[lo + 1]);
+}
+
+// ---- 8-bit codes -> f16 pairs, exactly ------------------------------------------------------------------
+// whole numbers: f16 1024 + (code + 128) has the biased code as its low byte
+__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
+  const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
+  return r;
+}
+// four codes of one word -> (0, 1) and (2, 3)
+template <bool I8>
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& p01, uint32_t& p23) {
+  if (I8) {
+    const uint32_t u = w ^ 0x80808080u;
+    p01 = hsub2(__byte_perm(u, 0x64646464u, 0x4140), 0x64806480u);
+    p23 = hsub2(__byte_perm(u, 0x64646464u, 0x4342), 0x64806480u);
+  } else {
+    p01 = e4m3x2_to_f16x2((uint16_t)w);
+    p23 = e4m3x2_to_f16x2((uint16_t)(w >> 16));
+  }
+}
+
+// one box of a 2-D tensor map, global -> this CTA's shared memory
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar), "l"(policy)
+      : "memory");
+}
+
+// ---- host ------------------------------------------------------------------------------------------------
+int check_blocks(const sphkv_blocks* c, const char* what);
+int block_rows(BlockRows& r, const sphkv_blocks* c, const int32_t* cu, int64_t rows, const char* what);
+// codes as a matrix [n_pages * Hkv * page_size][dh] of bytes, boxes of `box_rows` whole rows, swizzled in shared memory over
+// a row's bytes
+int make_codes_map(CUtensorMap* map, const sphkv_blocks& c, void* codes, int box_rows, const char* what);
+
+}  // namespace sphkv

@@ -1,0 +1,670 @@
+// Attention over the 8-bit block cache for few queries a sequence: one token (decode), or a handful.
+//
+// A unit is up to eight query rows that share a KV head (the head's group, times as many tokens as fit).  Per key and KV head
+// 2 dh bytes are read and 4 dh operations done for each row, so memory bounds it; what the kernel has to watch is
+// instructions, since every code has to become an f16 first.  Both products therefore run on the tensor cores with the
+// cache as the 16-row operand, straight from the codes' own bytes: codes are exact in f16, and the freedom to number an
+// operand's rows and depth lets a lane take whole 16-byte chunks.
+//   logits[16 keys x 8 rows] = codes[16 x dh] . q        (lane 4g + j: keys g, g + 8; dims dh/4 j ..)
+//   out[dh x 8 rows] += codes^T[dh x 16] . weights       (lane 4g + j: dims dh/8 g ..; keys 2j, 2j + 1, 2j + 8, 2j + 9)
+// The logits' layout (row 2j, 2j + 1 of keys g, g + 8) becomes the weights' operand by four transposes of 8 x 8.
+// Precision: a query row is scaled by a power of two so that its largest element lies in [2^13, 2^14): bf16 and f16 rows are
+// exact in f16 then, fp32 rows go in as hi + lo (22 bits); weights are hi + lo as well; sums are fp32.  A page's key scale
+// multiplies its logits, its value scale its weights, relative to the largest value scale seen (a power of two, S).
+//
+// Work: 16-token tiles of all (unit, tile) pairs in one line, cut evenly over the workers (a team of warps each); a worker's
+// share of a unit is a segment.  A segment's tiles go round the team's warps; each warp keeps maxima, sums and outputs of
+// its own, with its own ring of tiles that TMA fills, so nothing is shared until the segment's end.
+#include "blocks.cuh"
+
+namespace sphkv {
+
+constexpr int kBdWarps = 16, kBdThreads = 32 * kBdWarps;
+constexpr int kBdPlanned = 512;  // slots whose tile counts a CTA sums itself; more are summed by a launch before
+constexpr float kLazy = 8.f;     // a reference maximum moves when a logit passes it by 2^8
+constexpr float kWeight = 64.f;  // weights are 2^6 p v / S <= 2^14: f16 keeps 22 bits (hi + lo) of those above 2^-3
+
+struct BdArgs {
+  alignas(64) CUtensorMap k_map, v_map;
+  sphkv_blocks c;
+  BlockRows r;
+  const void* q;
+  int64_t q_row_stride, q_head_stride;
+  const int32_t* first;
+  void* out;
+  float* out_partial;
+  const int64_t* prefix;  // tiles of the slots before each, where a launch has summed them; else NULL
+  float* parts;           // [workers + units][8][dh + 2]
+  int q_dtype, out_dtype, Hq, group, slots, tshift, workers;
+  float scale_log2;       // sm_scale * log2 e
+};
+
+template <int DH>
+struct Bd {
+  static constexpr int kTile = 16 * DH;                            // bytes of a tile's keys, or values
+  static constexpr int kStages = DH == 128 ? 3 : 6;
+  static constexpr int kRing = 2 * kTile * kStages;                // of a warp
+  static constexpr int kGroupDims = DH / 8;                        // output dims of a lane
+  static constexpr int kCol = 8 * (kGroupDims + 2) + 4;            // floats of an output row in shared memory: no bank twice
+  static constexpr int kPrefixOff = kBdWarps * kRing;
+  static constexpr int kStatOff = kPrefixOff + (kBdPlanned + 1) * 8;
+  static constexpr int kStat = 3 * 8 + 8;                          // floats of a warp: maxima, sums, true maxima, S
+  static constexpr int kBarOff = kStatOff + kBdWarps * kStat * 4;
+  static constexpr int kSmem = kBarOff + kBdWarps * kStages * 8 + 1024;
+};
+static_assert(Bd<128>::kSmem <= 232448 && Bd<64>::kSmem <= 232448, "shared memory of a CTA");
+static_assert((kBdWarps / 2) * 8 * Bd<128>::kCol * 4 <= kBdWarps * Bd<128>::kRing, "outputs are joined in the rings' place");
+
+// The keys of one unit's queries.
+struct BdUnit {
+  int b, row0, tokens;      // dense rows of the unit's queries; tokens = 0: none
+  int pos0, first, limit;   // position of the first of them; keys first .. limit - 1 are seen by some
+  int tile0, tiles;
+};
+__device__ __forceinline__ BdUnit unit_of(const BdArgs& a, const BlockPiece& p) {
+  BdUnit u = {p.b, 0, 0, 0, 0, 0, 0, 0};
+  const int i0 = p.j << a.tshift;
+  if (p.b < 0 || i0 >= p.n) return u;
+  u.row0 = p.row0 + i0;
+  u.tokens = min(1 << a.tshift, p.n - i0);
+  if (p.end < 0) return u;
+  u.pos0 = p.end - p.n + i0;
+  u.limit = u.pos0 + u.tokens;
+  u.first = a.first ? min(max(a.first[p.b], 0), u.limit) : 0;
+  u.tile0 = u.first >> 4;
+  u.tiles = u.first < u.limit ? ((u.limit + 15) >> 4) - u.tile0 : 0;
+  return u;
+}
+
+// prefix[s] = tiles of the slots before s, prefix[slots] = all; by one block
+__device__ __forceinline__ void sum_tiles(const BdArgs& a, int64_t* prefix) {
+  __shared__ int64_t warp_sums[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int64_t before = 0;
+  for (int s0 = 0; s0 < a.slots; s0 += blockDim.x) {
+    const int s = s0 + tid;
+    int64_t v = s < a.slots ? unit_of(a, find_piece_alone(a.c, a.r, s, a.tshift, 1)).tiles : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += up;
+    }
+    if (lane == 31) warp_sums[warp] = v;
+    __syncthreads();
+    int64_t add = before;
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) {
+      if (w < warp) add += warp_sums[w];
+      before += warp_sums[w];
+    }
+    if (s < a.slots) prefix[s + 1] = v + add;
+    __syncthreads();
+  }
+  if (tid == 0) prefix[0] = 0;
+  __syncthreads();
+}
+__global__ void __launch_bounds__(1024) blocks_plan_kernel(const __grid_constant__ BdArgs a, int64_t* prefix) {
+  griddep_wait();
+  sum_tiles(a, prefix);
+}
+// the workers that share the tiles: none goes without, so that a unit's segments are those of consecutive workers
+__device__ __forceinline__ int64_t workers_of(const BdArgs& a, int64_t total) { return min((int64_t)a.workers, total); }
+__device__ __forceinline__ int slot_at(const int64_t* prefix, int slots, int64_t tile) {  // prefix[s] <= tile < prefix[s + 1]
+  int lo = 0, hi = slots;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    (prefix[mid] <= tile ? lo : hi) = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint4 lds_u4(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ uint2 lds_u2(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// where 16-byte chunk c of row t lies in a tile that a tensor copy has swizzled
+template <int DH>
+__device__ __forceinline__ uint32_t chunk_at(int t, int c) {
+  return DH == 128 ? t * 128 + ((c ^ (t & 7)) << 4) : t * 64 + ((c ^ ((t >> 1) & 3)) << 4);
+}
+// codes of two keys at four dims -> f16 pairs (key 0, key 1) for each dim
+template <bool I8>
+__device__ __forceinline__ void pair_codes(uint32_t k0, uint32_t k1, uint32_t (&d)[4]) {
+  const uint32_t lo = __byte_perm(k0, k1, 0x5140), hi = __byte_perm(k0, k1, 0x7362);
+  codes_to_f16<I8>(lo, d[0], d[1]);
+  codes_to_f16<I8>(hi, d[2], d[3]);
+}
+
+// WARPS: warps of a team
+template <int DH, bool I8, bool QLO, int WARPS>
+__global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __grid_constant__ BdArgs a) {
+  using L = Bd<DH>;
+  constexpr int S = L::kStages, KS = DH / 16, GD = L::kGroupDims, W4 = GD / 4;  // words of a value row per lane
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j = lane & 3;
+  const int team = warp / WARPS, tw = warp % WARPS;
+  const uint32_t ring = smem_u32(smem) + warp * L::kRing;
+  const uint32_t bars = smem_u32(smem) + L::kBarOff + warp * S * 8;
+  int64_t* const prefix_smem = reinterpret_cast<int64_t*>(smem + L::kPrefixOff);
+  float* const stats = reinterpret_cast<float*>(smem + L::kStatOff) + team * WARPS * L::kStat;  // of the team
+  float* const joined = reinterpret_cast<float*>(smem + team * WARPS * L::kRing);               // in its rings' place
+  if (lane == 0) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) mbar_init(bars + 8 * s, 1);
+    fence_async_smem();
+  }
+  __syncthreads();
+  griddep_launch();
+  griddep_wait();
+  const int64_t* prefix = a.prefix;
+  if (prefix == nullptr) {
+    sum_tiles(a, prefix_smem);
+    prefix = prefix_smem;
+  }
+  const int64_t total = prefix[a.slots] * a.c.Hkv;
+  const int worker = blockIdx.x * (kBdWarps / WARPS) + team;
+  const int64_t workers = workers_of(a, total);
+  int64_t pos = worker < workers ? worker * total / workers : 0;
+  const int64_t stop = worker < workers ? (worker + 1) * total / workers : 0;
+  const uint64_t policy = policy_evict_first();
+  const int shift = 31 - __clz(a.c.page_size);
+  uint32_t issued = 0, taken = 0;  // tiles since the kernel began: stage = n % S, the barrier's phase n / S
+  bool lost = false;
+
+  auto team_sync = [&] {
+    if constexpr (WARPS > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(32 * WARPS) : "memory");
+    else __syncwarp();
+  };
+
+  while (pos < stop) {
+    // ---- the segment ----
+    const int slot = slot_at(prefix, a.slots, pos / a.c.Hkv);
+    const BdUnit u = unit_of(a, find_piece_alone(a.c, a.r, slot, a.tshift, 1));
+    const int64_t in_slot = pos - prefix[slot] * a.c.Hkv;
+    const int head = (int)(in_slot / u.tiles), from = (int)(in_slot - (int64_t)head * u.tiles);
+    const int count = (int)min((int64_t)(u.tiles - from), stop - pos);
+    const int unit = slot * a.c.Hkv + head;
+    pos += count;
+    const int cols = u.tokens * a.group;
+
+    // ---- where this warp's tiles lie: lane i holds tile 32 r + i of them ----
+    const int mine = tw < count ? (count - tw + WARPS - 1) / WARPS : 0;
+    const int32_t* table = a.c.block_table + (int64_t)u.b * a.c.max_blocks;
+    struct Meta {
+      int row;  // of the pools; negative: a bad table entry
+      float ks, vs;
+    };
+    auto lookup = [&](int k) {
+      Meta m = {0, 0.f, 0.f};
+      if (k >= mine) return m;
+      const int tok = (u.tile0 + from + tw + k * WARPS) << 4;
+      const int page = table[tok >> shift];
+      if (page < 0 || page >= a.c.n_pages) {
+        bad_status(a.c, SPHKV_ST_BAD_BLOCK);
+        m.row = -1;
+        return m;
+      }
+      const int at = page * a.c.Hkv + head;
+      m.row = (at << shift) + (tok & (a.c.page_size - 1));
+      m.ks = a.c.k_scale[at];
+      m.vs = a.c.v_scale[at];
+      return m;
+    };
+    Meta cur = lookup(lane), nxt = lookup(32 + lane);
+    auto issue = [&](int k, int base) {  // tile k; `cur` holds tiles base .. base + 31
+      const int row = __shfl_sync(0xffffffffu, k - base < 32 ? cur.row : nxt.row, k & 31);
+      if (lane == 0) {
+        const uint32_t s = issued % S, bar = bars + 8 * s, at = ring + s * 2 * L::kTile;
+        mbar_expect_tx(bar, 2 * L::kTile);
+        tma_load_2d(at, &a.k_map, 0, max(row, 0), bar, policy);
+        tma_load_2d(at + L::kTile, &a.v_map, 0, max(row, 0), bar, policy);
+      }
+      ++issued;
+    };
+    if (!lost)
+      for (int k = 0; k < min(S, mine); ++k) issue(k, 0);
+
+    // ---- queries: lane 4g + j takes dims DH/4 j .. of row g ----
+    uint32_t qh[KS][2], ql[QLO ? KS : 1][2];
+    float f0, f1;      // logit factors of rows 2j, 2j + 1
+    int lim0, lim1;    // the keys that they see end here
+    int least = u.limit;
+    {
+      float v[DH / 4];
+      float top = 0.f;
+      const int tok = g / a.group, h = head * a.group + g - tok * a.group;
+      const bool there = g < cols;
+      const int64_t at = there ? (int64_t)(u.row0 + tok) * a.q_row_stride + (int64_t)h * a.q_head_stride + (DH / 4) * j : 0;
+#pragma unroll
+      for (int i = 0; i < DH / 4; ++i) {
+        v[i] = there ? load_as_float(a.q, a.q_dtype, at + i) : 0.f;
+        top = fmaxf(top, fabsf(v[i]));
+        if (isnan(v[i])) top = INFINITY;
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      int e = (int)(__float_as_uint(top) >> 23);
+      e = e == 255 ? 140 : max(e, 14);  // infinities and NaN go in as they are
+      const float up = __uint_as_float((uint32_t)(267 - e) << 23), down = __uint_as_float((uint32_t)(e - 13) << 23);
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const float x = v[4 * s + 2 * p] * up, y = v[4 * s + 2 * p + 1] * up;
+          if constexpr (QLO)
+            split_f16x2(x, y, qh[s][p], ql[s][p]);
+          else
+            qh[s][p] = pack_f16x2(x, y);
+        }
+      const float f = down * a.scale_log2;
+      f0 = __shfl_sync(0xffffffffu, f, 8 * j);
+      f1 = __shfl_sync(0xffffffffu, f, 8 * j + 4);
+      lim0 = 2 * j < cols ? u.pos0 + 2 * j / a.group + 1 : u.limit;
+      lim1 = 2 * j + 1 < cols ? u.pos0 + (2 * j + 1) / a.group + 1 : u.limit;
+      if (u.tokens > 1) least = u.pos0 + 1;
+    }
+
+    float acc[KS][4];  // [DH / 16 row tiles of dims]
+#pragma unroll
+    for (int i = 0; i < KS; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+    const float kNone = -3.402823466e38f;
+    float m0 = kNone, m1 = kNone, l0 = 0.f, l1 = 0.f, t0 = -INFINITY, t1 = -INFINITY;
+    float big = 0.f, per_big = 0.f;  // S and 1 / S
+
+    for (int k = 0, base = 0; k < mine; ++k) {
+      if (k - base == 32) {
+        base += 32;
+        cur = nxt;
+        nxt = lookup(base + 32 + lane);
+      }
+      const int src = k & 31;
+      const int row = __shfl_sync(0xffffffffu, cur.row, src);
+      const float ks = __shfl_sync(0xffffffffu, cur.ks, src), vs = __shfl_sync(0xffffffffu, cur.vs, src);
+      const uint32_t stage = taken % S;
+      if (!lost && !mbar_wait(bars + 8 * stage, (taken / S) & 1)) {
+        lost = true;
+        bad_status(a.c, SPHKV_ST_TIMEOUT);
+      }
+      if (lost) break;
+      ++taken;
+      const uint32_t kt = ring + stage * 2 * L::kTile, vt = kt + L::kTile;
+
+      // logits
+      float c[2][4] = {};
+#pragma unroll
+      for (int q4 = 0; q4 < DH / 64; ++q4) {
+        const uint4 x = lds_u4(kt + chunk_at<DH>(g, (DH / 64) * j + q4)), y = lds_u4(kt + chunk_at<DH>(g + 8, (DH / 64) * j + q4));
+        const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int s = 4 * q4 + w;
+          uint32_t a0, a1, a2, a3;
+          codes_to_f16<I8>(xw[w], a0, a2);
+          codes_to_f16<I8>(yw[w], a1, a3);
+          mma_16x8x16(c[w & 1], a0, a1, a2, a3, qh[s][0], qh[s][1]);
+          if constexpr (QLO) mma_16x8x16(c[w & 1], a0, a1, a2, a3, ql[s][0], ql[s][1]);
+        }
+      }
+      uint32_t vw[4][W4];  // keys 2j, 2j + 1, 2j + 8, 2j + 9; dims GD g ..
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int t = 2 * j + (n & 1) + 8 * (n >> 1);
+        if constexpr (DH == 128) {
+          const uint4 v = lds_u4(vt + chunk_at<DH>(t, g));
+          vw[n][0] = v.x, vw[n][1] = v.y, vw[n][2] = v.z, vw[n][3] = v.w;
+        } else {
+          const uint2 v = lds_u2(vt + chunk_at<DH>(t, g >> 1) + 8 * (g & 1));
+          vw[n][0] = v.x, vw[n][1] = v.y;
+        }
+      }
+      __syncwarp();
+      if (k + S < mine) issue(k + S, base);
+
+      const float e0 = f0 * ks, e1 = f1 * ks;
+      float x[4] = {(c[0][0] + c[1][0]) * e0, (c[0][1] + c[1][1]) * e1, (c[0][2] + c[1][2]) * e0, (c[0][3] + c[1][3]) * e1};
+      const int tok = (u.tile0 + from + tw + k * WARPS) << 4;
+      const bool edge = row < 0 || tok < u.first || tok + 16 > least;
+      bool seen[4] = {true, true, true, true};
+      if (edge) {  // some keys of the tile are not seen by every row, or by none
+        const int ta = tok + g, tb = ta + 8;
+        seen[0] = row >= 0 && ta >= u.first && ta < lim0;
+        seen[1] = row >= 0 && ta >= u.first && ta < lim1;
+        seen[2] = row >= 0 && tb >= u.first && tb < lim0;
+        seen[3] = row >= 0 && tb >= u.first && tb < lim1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!seen[i]) x[i] = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {  // what lies behind the last token may be any byte
+          const int t = tok + 2 * j + (n & 1) + 8 * (n >> 1);
+          if (row < 0 || t < u.first || t >= u.limit)
+#pragma unroll
+            for (int w = 0; w < W4; ++w) vw[n][w] = 0;
+        }
+      }
+      const float x0 = fmaxf(x[0], x[2]), x1 = fmaxf(x[1], x[3]);
+      t0 = fmaxf(t0, x0);
+      t1 = fmaxf(t1, x1);
+      const bool larger = vs > big && row >= 0;
+      if (__any_sync(0xffffffffu, x0 > m0 + kLazy || x1 > m1 + kLazy) || larger) {
+        float n0 = x0, n1 = x1;
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
+          n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
+        }
+        n0 = fmaxf(n0, m0);
+        n1 = fmaxf(n1, m1);
+        float down = 1.f;
+        if (larger) {
+          const float b = __uint_as_float((__float_as_uint(vs) + 0x7fffffu) & 0x7f800000u);
+          per_big = __uint_as_float(0x7f000000u - __float_as_uint(b));
+          if (__float_as_uint(b) > 0x7e800000u) per_big = 0.f;
+          down = big * per_big;
+          big = b;
+        }
+        const float d0 = ex2(m0 - n0), d1 = ex2(m1 - n1);
+        l0 *= d0;
+        l1 *= d1;
+        const float r0 = d0 * down, r1 = d1 * down;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) acc[i][0] *= r0, acc[i][1] *= r1, acc[i][2] *= r0, acc[i][3] *= r1;
+        m0 = n0;
+        m1 = n1;
+      }
+      float w[4] = {ex2(x[0] - m0), ex2(x[1] - m1), ex2(x[2] - m0), ex2(x[3] - m1)};
+      l0 += w[0] + w[2];
+      l1 += w[1] + w[3];
+      const float ve = vs * per_big * kWeight;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] *= ve;
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!seen[i]) w[i] = 0.f;  // the scale may be NaN
+      }
+      uint32_t ph[2], pl[2];
+      split_f16x2(w[0], w[1], ph[0], pl[0]);
+      split_f16x2(w[2], w[3], ph[1], pl[1]);
+      const uint32_t bh0 = transposed(ph[0]), bh1 = transposed(ph[1]), bl0 = transposed(pl[0]), bl1 = transposed(pl[1]);
+#pragma unroll
+      for (int q4 = 0; q4 < W4; ++q4) {  // four dims of the lane: two row tiles
+        uint32_t d01[4], d89[4];
+        pair_codes<I8>(vw[0][q4], vw[1][q4], d01);
+        pair_codes<I8>(vw[2][q4], vw[3][q4], d89);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          mma_16x8x16(acc[2 * q4 + h], d01[2 * h], d01[2 * h + 1], d89[2 * h], d89[2 * h + 1], bh0, bh1);
+          mma_16x8x16(acc[2 * q4 + h], d01[2 * h], d01[2 * h + 1], d89[2 * h], d89[2 * h + 1], bl0, bl1);
+        }
+      }
+    }
+
+    // ---- the team's warps are joined ----
+    {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+        t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
+        t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
+      }
+      float* const st = stats + tw * L::kStat;
+      if (g == 0) {
+        st[2 * j] = m0, st[2 * j + 1] = m1;
+        st[8 + 2 * j] = l0, st[9 + 2 * j] = l1;
+        st[16 + 2 * j] = t0, st[17 + 2 * j] = t1;
+      }
+      team_sync();  // every tile of the segment has been taken: the rings' place is free
+      float top0 = kNone, top1 = kNone;
+      for (int w = 0; w < WARPS; ++w) {
+        top0 = fmaxf(top0, stats[w * L::kStat + 2 * j]);
+        top1 = fmaxf(top1, stats[w * L::kStat + 2 * j + 1]);
+      }
+      const float r0 = ex2(m0 - top0) * (big / kWeight), r1 = ex2(m1 - top1) * (big / kWeight);
+      constexpr int HALF = WARPS > 1 ? WARPS / 2 : 1;
+      auto place = [&](int i, int col) { return reinterpret_cast<float2*>(joined + ((tw % HALF) * 8 + col) * L::kCol + g * (GD + 2) + 2 * i); };
+      if (tw < HALF) {
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          *place(i, 2 * j) = make_float2(acc[i][0] * r0, acc[i][2] * r0);
+          *place(i, 2 * j + 1) = make_float2(acc[i][1] * r1, acc[i][3] * r1);
+        }
+      }
+      team_sync();
+      if (tw >= HALF) {
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          float2 p = *place(i, 2 * j);
+          *place(i, 2 * j) = make_float2(p.x + acc[i][0] * r0, p.y + acc[i][2] * r0);
+          p = *place(i, 2 * j + 1);
+          *place(i, 2 * j + 1) = make_float2(p.x + acc[i][1] * r1, p.y + acc[i][3] * r1);
+        }
+      }
+      team_sync();
+      const bool whole = count == u.tiles;
+      float* const part = a.parts + (int64_t)(worker + unit) * 8 * (DH + 2);
+      for (int i = tw * 32 + lane; i < cols * DH; i += WARPS * 32) {
+        const int col = i / DH, d = i - col * DH;
+        float top = kNone, true_top = -INFINITY, sum = 0.f, v = 0.f;
+        for (int w = 0; w < WARPS; ++w) {
+          top = fmaxf(top, stats[w * L::kStat + col]);
+          true_top = fmaxf(true_top, stats[w * L::kStat + 16 + col]);
+        }
+        for (int w = 0; w < WARPS; ++w) sum += stats[w * L::kStat + 8 + col] * ex2(stats[w * L::kStat + col] - top);
+        for (int w = 0; w < HALF; ++w) v += joined[(w * 8 + col) * L::kCol + (d / GD) * (GD + 2) + d % GD];
+        const float to_true = true_top == -INFINITY ? 0.f : ex2(top - true_top);
+        if (whole) {
+          const int tok = col / a.group, h = head * a.group + col - tok * a.group;
+          const int64_t at = (int64_t)(u.row0 + tok) * a.Hq + h;
+          if (a.out) store_from_float(a.out, a.out_dtype, at * DH + d, sum == 0.f ? 0.f : v / sum);
+          if (a.out_partial) {
+            float* o = a.out_partial + at * (DH + 2);
+            o[2 + d] = v * to_true;
+            if (d == 0) o[0] = true_top * kLn2, o[1] = sum * to_true;
+          }
+        } else {
+          part[col * (DH + 2) + 2 + d] = v * to_true;
+          if (d == 0) part[col * (DH + 2)] = true_top, part[col * (DH + 2) + 1] = sum * to_true;
+        }
+      }
+      team_sync();
+      fence_async_smem();  // the next segment's copies come in through the other proxy
+      team_sync();
+    }
+  }
+  if (lost) {  // copies that are still on their way
+    for (; taken != issued; ++taken) (void)mbar_wait(bars + 8 * (taken % S), (taken / S) & 1);
+  }
+}
+
+// A block per unit: joins the segments of units that more than one worker had, and writes the rows of units without keys.
+__global__ void __launch_bounds__(256) blocks_merge_kernel(const __grid_constant__ BdArgs a, int dh) {
+  __shared__ int64_t prefix_smem[kBdPlanned + 1];
+  griddep_launch();
+  griddep_wait();
+  const int64_t* prefix = a.prefix;
+  if (prefix == nullptr) {
+    sum_tiles(a, prefix_smem);
+    prefix = prefix_smem;
+  }
+  const int unit = blockIdx.x, slot = unit / a.c.Hkv, head = unit - slot * a.c.Hkv;
+  const int64_t total = prefix[a.slots] * a.c.Hkv;
+  const BdUnit u = unit_of(a, find_piece_alone(a.c, a.r, slot, a.tshift, 1));
+  if (u.tokens == 0) return;
+  int64_t w0 = 0, w1 = -1;
+  if (u.tiles > 0) {
+    const int64_t p0 = prefix[slot] * a.c.Hkv + (int64_t)head * u.tiles, p1 = p0 + u.tiles - 1;
+    const int64_t workers = workers_of(a, total);
+    w0 = ((p0 + 1) * workers - 1) / total;
+    w1 = ((p1 + 1) * workers - 1) / total;
+    if (w0 == w1) return;
+  }
+  for (int i = threadIdx.x; i < u.tokens * a.group * dh; i += blockDim.x) {
+    const int col = i / dh, d = i - col * dh;
+    float top = -INFINITY, sum = 0.f, v = 0.f;
+    const float* row = a.parts + ((w0 + unit) * 8 + col) * (dh + 2);
+    const int64_t step = (int64_t)8 * (dh + 2);
+    for (int64_t w = 0; w <= w1 - w0; ++w) top = fmaxf(top, row[w * step]);
+    for (int64_t w = 0; w <= w1 - w0; ++w) {
+      const float f = row[w * step] == -INFINITY ? 0.f : ex2(row[w * step] - top);
+      sum += row[w * step + 1] * f;
+      v += row[w * step + 2 + d] * f;
+    }
+    const int tok = col / a.group, h = head * a.group + col - tok * a.group;
+    const int64_t at = (int64_t)(u.row0 + tok) * a.Hq + h;
+    if (a.out) store_from_float(a.out, a.out_dtype, at * dh + d, sum == 0.f ? 0.f : v / sum);
+    if (a.out_partial) {
+      float* o = a.out_partial + at * (dh + 2);
+      o[2 + d] = v;
+      if (d == 0) o[0] = top == -INFINITY ? -INFINITY : top * kLn2, o[1] = sum;
+    }
+  }
+}
+
+static int tokens_shift(int group) { return group == 1 ? 3 : group == 2 ? 2 : group <= 4 ? 1 : 0; }
+static int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+
+static int64_t bd_scratch(int64_t slots, int Hkv, int dh, int workers) {
+  return align256((slots + 1) * 8) + (workers + slots * Hkv) * 8 * (dh + 2) * 4;
+}
+
+template <int DH, bool I8, bool QLO>
+static int launch_bd(const BdArgs& a, int ctas, cudaStream_t st) {
+  static SmemOptIn opt_in;
+  auto kern = blocks_decode_kernel<DH, I8, QLO, kBdWarps>;
+  if (int rc = ensure_dynamic_smem(opt_in, (const void*)kern, Bd<DH>::kSmem, "blocks_decode")) return rc;
+  (void)launch_overlapped(kern, dim3(ctas), dim3(kBdThreads), Bd<DH>::kSmem, st, a);
+  return check_launch("blocks_decode_kernel");
+}
+template <int DH>
+static int launch_bd_types(const BdArgs& a, int ctas, cudaStream_t st) {
+  const bool i8 = a.c.store == SPHKV_BLOCKS_I8;
+  if (a.q_dtype == SPHKV_F32) return i8 ? launch_bd<DH, true, true>(a, ctas, st) : launch_bd<DH, false, true>(a, ctas, st);
+  return i8 ? launch_bd<DH, true, false>(a, ctas, st) : launch_bd<DH, false, false>(a, ctas, st);
+}
+
+// a has the cache, rows, queries and outputs
+static int run_bd(BdArgs& a, void* scratch, int64_t scratch_bytes, const char* what, cudaStream_t st) {
+  const int sms = sm_count_current_device();
+  if (sms <= 0) return sms;
+  const int64_t slots = block_slots(a.r, a.c.B, a.tshift, 1);
+  if (slots == 0) return 0;
+  SPHKV_REQUIRE(slots * a.c.Hkv <= 0x7fffffff, SPHKV_E_LIMIT, "%s: too many queries for one launch", what);
+  a.slots = (int)slots;
+  a.workers = sms;
+  const int64_t need = bd_scratch(slots, a.c.Hkv, a.c.dh, a.workers);
+  SPHKV_REQUIRE(scratch != nullptr && scratch_bytes >= need, SPHKV_E_SCRATCH, "%s: scratch %lld B < %lld B", what,
+                (long long)scratch_bytes, (long long)need);
+  SPHKV_REQUIRE(((uintptr_t)scratch & 255) == 0, SPHKV_E_ALIGN, "%s: scratch needs 256 B", what);
+  a.parts = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(scratch) + align256((slots + 1) * 8));
+  a.prefix = nullptr;
+  if (int rc = make_codes_map(&a.k_map, a.c, a.c.k_codes, 16, what)) return rc;
+  if (int rc = make_codes_map(&a.v_map, a.c, a.c.v_codes, 16, what)) return rc;
+  if (slots > kBdPlanned) {
+    int64_t* prefix = reinterpret_cast<int64_t*>(scratch);
+    (void)launch_overlapped(blocks_plan_kernel, dim3(1), dim3(1024), 0, st, a, prefix);
+    if (int rc = check_launch("blocks_plan_kernel")) return rc;
+    a.prefix = prefix;
+  }
+  if (int rc = a.c.dh == 128 ? launch_bd_types<128>(a, sms, st) : launch_bd_types<64>(a, sms, st)) return rc;
+  (void)launch_overlapped(blocks_merge_kernel, dim3((unsigned)(slots * a.c.Hkv)), dim3(256), 0, st, a, (int)a.c.dh);
+  return check_launch("blocks_merge_kernel");
+}
+
+static int check_queries(BdArgs& a, const void* q, int q_dtype, const void* out, const float* out_partial, int out_dtype, int Hq,
+                         const char* what) {
+  const sphkv_blocks& c = a.c;
+  SPHKV_REQUIRE(out || out_partial, SPHKV_E_ARG, "%s: no output", what);
+  SPHKV_REQUIRE(q_dtype >= 0 && q_dtype <= 2 && out_dtype >= 0 && out_dtype <= 2, SPHKV_E_DTYPE, "%s: q_dtype=%d out_dtype=%d", what,
+                q_dtype, out_dtype);
+  SPHKV_REQUIRE(Hq > 0 && Hq % c.Hkv == 0, SPHKV_E_ARG, "%s: Hq=%d Hkv=%d", what, Hq, c.Hkv);
+  SPHKV_REQUIRE(Hq / c.Hkv <= SPHKV_MAX_GQA, SPHKV_E_LIMIT, "%s: %d query heads per KV head (max %d)", what, Hq / c.Hkv, SPHKV_MAX_GQA);
+  const int64_t q_size = q_dtype == SPHKV_F32 ? 4 : 2, o_size = out_dtype == SPHKV_F32 ? 4 : 2;
+  SPHKV_REQUIRE(((uintptr_t)q & (q_size - 1)) == 0 && ((uintptr_t)out & (o_size - 1)) == 0 && ((uintptr_t)out_partial & 3) == 0,
+                SPHKV_E_ALIGN, "%s: q or an output is not on an element's boundary", what);
+  a.Hq = Hq;
+  a.group = Hq / c.Hkv;
+  a.q = q;
+  a.q_dtype = q_dtype;
+  a.out_dtype = out_dtype;
+  return 0;
+}
+
+}  // namespace sphkv
+
+using namespace sphkv;
+
+extern "C" int64_t sphkv_blocks_decode_scratch_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t dh) {
+  if (B <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq / Hkv > SPHKV_MAX_GQA || (dh != 64 && dh != 128)) return SPHKV_E_ARG;
+  const int sms = sm_count_current_device();
+  return sms <= 0 ? sms : bd_scratch(B, Hkv, dh, sms);
+}
+
+extern "C" int sphkv_blocks_decode(const sphkv_blocks* c, const void* q, int32_t q_dtype, int64_t q_row_stride, int64_t q_head_stride,
+                                   const int32_t* first, void* out, int32_t out_dtype, float* out_partial, void* scratch,
+                                   int64_t scratch_bytes, int32_t Hq, float sm_scale, void* stream) {
+  if (int rc = check_blocks(c, "blocks_decode")) return rc;
+  SPHKV_REQUIRE(q != nullptr, SPHKV_E_ARG, "blocks_decode: q is NULL");
+  BdArgs a = {};
+  a.c = *c;
+  if (int rc = check_queries(a, q, q_dtype, out, out_partial, out_dtype, Hq, "blocks_decode")) return rc;
+  // a sequence without tokens has a query all the same: one row a sequence, whatever ends[] says
+  a.r = {nullptr, c->B, 1, true};
+  a.tshift = 0;
+  a.first = first;
+  a.q_row_stride = q_row_stride;
+  a.q_head_stride = q_head_stride;
+  a.out = out;
+  a.out_partial = out_partial;
+  a.scale_log2 = sm_scale * kLog2e;
+  return run_bd(a, scratch, scratch_bytes, "blocks_decode", reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int64_t sphkv_blocks_attend_scratch_bytes(int32_t B, int64_t rows, int32_t Hq, int32_t Hkv, int32_t dh) {
+  if (B <= 0 || rows < 0 || rows > 0x1fffffff || Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq / Hkv > SPHKV_MAX_GQA || (dh != 64 && dh != 128))
+    return SPHKV_E_ARG;
+  const int sms = sm_count_current_device();
+  return sms <= 0 ? sms : bd_scratch((rows >> tokens_shift(Hq / Hkv)) + B, Hkv, dh, sms);
+}
+
+extern "C" int sphkv_blocks_attend(const sphkv_blocks* c, const void* q, int32_t q_dtype, int64_t q_row_stride, int64_t q_head_stride,
+                                   const int32_t* cu, int64_t rows, const int32_t* first, void* out, int32_t out_dtype, void* scratch,
+                                   int64_t scratch_bytes, int32_t Hq, float sm_scale, void* stream) {
+  if (int rc = check_blocks(c, "blocks_attend")) return rc;
+  BdArgs a = {};
+  a.c = *c;
+  if (int rc = block_rows(a.r, c, cu, rows, "blocks_attend")) return rc;
+  SPHKV_REQUIRE(rows == 0 || q != nullptr, SPHKV_E_ARG, "blocks_attend: q is NULL");
+  if (int rc = check_queries(a, q, q_dtype, out, nullptr, out_dtype, Hq, "blocks_attend")) return rc;
+  SPHKV_REQUIRE(q_dtype != SPHKV_F32, SPHKV_E_DTYPE, "blocks_attend: q_dtype=%d (16-bit types)", q_dtype);
+  if (rows == 0) return 0;
+  a.tshift = tokens_shift(a.group);
+  a.first = first;
+  a.q_row_stride = q_row_stride;
+  a.q_head_stride = q_head_stride;
+  a.out = out;
+  a.scale_log2 = sm_scale * kLog2e;
+  return run_bd(a, scratch, scratch_bytes, "blocks_attend", reinterpret_cast<cudaStream_t>(stream));
+}

@@ -67,6 +67,7 @@ extern "C" int sphkv_struct_size(int which) {
     case 1: return (int)sizeof(sphkv_encode_params);
     case 2: return (int)sizeof(sphkv_decode_params);
     case 4: return (int)sizeof(sphkv_page_lists_params);
+    case 5: return (int)sizeof(sphkv_blocks);
     default: return -1;
   }
 }

@@ -264,9 +264,9 @@ def decode_paged(q: torch.Tensor, cache: PagedCache, rope: Optional[torch.Tensor
     return out
 
 
-def check_status(cache: PagedCache) -> None:
-    """Host read of the cache's status word (synchronises); raises if a decode since the last
-    check met a bad block-table entry, tier slot or key position, or gave up on a copy."""
+def check_status(cache) -> None:
+    """Host read of the status word of a PagedCache or BlockCache (synchronises); raises if a call since the last
+    check met a bad block-table entry, tier slot, key position or length, or gave up on a copy."""
     if cache.status is None:
         return
     st = int(cache.status.item())
@@ -275,7 +275,8 @@ def check_status(cache: PagedCache) -> None:
                                   (_lib.ST_BAD_BLOCK, "block-table entry >= n_pages"),
                                   (_lib.ST_BAD_SLOT, "bits-table entry outside the tier slots"),
                                   (_lib.ST_TIMEOUT, "an asynchronous copy did not complete"),
-                                  (_lib.ST_INTERNAL, "misaligned shared memory")) if st & bit]
+                                  (_lib.ST_INTERNAL, "misaligned shared memory"),
+                                  (_lib.ST_BAD_LENGTH, "token numbers of a sequence that do not fit")) if st & bit]
         cache.status.zero_()
         raise _lib.SphKVError("decode status %d: %s" % (st, "; ".join(names)))
 
