@@ -364,6 +364,7 @@ int block_rows(BlockRows& r, const sphkv_blocks* c, const int32_t* cu, int64_t r
   r.cu = cu;
   r.rows = (int)rows;
   r.even = (int)(rows / c->B);
+  r.mul = 1;
   r.lone = false;
   return 0;
 }

@@ -8,6 +8,7 @@ namespace sphkv {
 struct BlockRows {
   const int32_t* cu;
   int32_t rows, even;  // even: rows / B
+  int32_t mul;         // rows are dealt in units of 1 / mul of a dense row (a query row for each head of a group)
   bool lone;           // one row a sequence that need not be among its tokens: a sequence may be empty
 };
 
@@ -18,8 +19,8 @@ __host__ __device__ inline int block_slots_even(int n, int shift, int extra) {  
   return n <= 0 ? 0 : ((n + (1 << shift) - 1) >> shift) + extra - 1;
 }
 inline int64_t block_slots(const BlockRows& r, int B, int shift, int extra) {
-  if (r.cu == nullptr) return (int64_t)B * block_slots_even(r.even, shift, extra);
-  return ((int64_t)r.rows >> shift) + (int64_t)extra * B;
+  if (r.cu == nullptr) return (int64_t)B * block_slots_even(r.even * r.mul, shift, extra);
+  return ((int64_t)r.rows * r.mul >> shift) + (int64_t)extra * B;
 }
 
 struct BlockPiece {
@@ -46,13 +47,13 @@ __device__ __forceinline__ BlockPiece checked_piece(const sphkv_blocks& c, const
   return p;
 }
 __device__ __forceinline__ int slot_base(const BlockRows& r, int b, int shift, int extra) {
-  return (min(max(r.cu[b], 0), r.rows) >> shift) + extra * b;
+  return (min(max(r.cu[b], 0), r.rows) * r.mul >> shift) + extra * b;
 }
 
 // Called by whole warps; every lane gets the answer.
 __device__ __forceinline__ BlockPiece find_piece(const sphkv_blocks& c, const BlockRows& r, int slot, int shift, int extra) {
   if (r.cu == nullptr) {
-    const int per = block_slots_even(r.even, shift, extra), b = slot / per;
+    const int per = block_slots_even(r.even * r.mul, shift, extra), b = slot / per;
     return checked_piece(c, r, b, slot - b * per, b * r.even, (b + 1) * r.even);
   }
   int b = -1, base = 0;
@@ -71,7 +72,7 @@ __device__ __forceinline__ BlockPiece find_piece(const sphkv_blocks& c, const Bl
 // The same by one thread.
 __device__ __forceinline__ BlockPiece find_piece_alone(const sphkv_blocks& c, const BlockRows& r, int slot, int shift, int extra) {
   if (r.cu == nullptr) {
-    const int per = block_slots_even(r.even, shift, extra), b = slot / per;
+    const int per = block_slots_even(r.even * r.mul, shift, extra), b = slot / per;
     return checked_piece(c, r, b, slot - b * per, b * r.even, (b + 1) * r.even);
   }
   int lo = 0, hi = c.B;  // the last sequence whose slots begin at or before this one
@@ -80,6 +81,48 @@ __device__ __forceinline__ BlockPiece find_piece_alone(const sphkv_blocks& c, co
     (slot_base(r, mid, shift, extra) <= slot ? lo : hi) = mid;
   }
   return checked_piece(c, r, lo, slot - slot_base(r, lo, shift, extra), r.cu[lo], r.cu[lo + 1]);
+}
+
+// ---- work dealt evenly: tiles of all slots and heads in one line ------------------------------------------------
+// prefix[s] = tiles of the slots before s, prefix[slots] = all; by one block.  tiles_of(s): tiles of slot s
+template <typename F>
+__device__ __forceinline__ void sum_tiles(int slots, int64_t* prefix, F tiles_of) {
+  __shared__ int64_t warp_sums[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int64_t before = 0;
+  for (int s0 = 0; s0 < slots; s0 += blockDim.x) {
+    const int s = s0 + tid;
+    int64_t v = s < slots ? tiles_of(s) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += up;
+    }
+    if (lane == 31) warp_sums[warp] = v;
+    __syncthreads();
+    int64_t add = before;
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) {
+      if (w < warp) add += warp_sums[w];
+      before += warp_sums[w];
+    }
+    if (s < slots) prefix[s + 1] = v + add;
+    __syncthreads();
+  }
+  if (tid == 0) prefix[0] = 0;
+  __syncthreads();
+}
+__device__ __forceinline__ int slot_at(const int64_t* prefix, int slots, int64_t tile) {  // prefix[s] <= tile < prefix[s + 1]
+  int lo = 0, hi = slots;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    (prefix[mid] <= tile ? lo : hi) = mid;
+  }
+  return lo;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
 // ---- 8-bit codes -> f16 pairs, exactly ------------------------------------------------------------------
@@ -120,5 +163,13 @@ int block_rows(BlockRows& r, const sphkv_blocks* c, const int32_t* cu, int64_t r
 // codes as a matrix [n_pages * Hkv * page_size][dh] of bytes, boxes of `box_rows` whole rows, swizzled in shared memory over
 // a row's bytes
 int make_codes_map(CUtensorMap* map, const sphkv_blocks& c, void* codes, int box_rows, const char* what);
+int check_queries(const sphkv_blocks& c, const void* q, int q_dtype, const void* out, const float* out_partial, int out_dtype, int Hq,
+                  const char* what);
+// attention of up to eight query rows a unit: 1 << tshift tokens of a sequence, at most 1 << tokens_shift(group)
+int tokens_shift(int group);
+int few_queries(const sphkv_blocks& c, const BlockRows& r, const void* q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride,
+                const int32_t* first, void* out, int out_dtype, float* out_partial, void* scratch, int64_t scratch_bytes, int Hq,
+                float sm_scale, int tshift, const char* what, cudaStream_t st);
+int64_t few_queries_scratch(int64_t rows, int B, int Hkv, int dh, int tshift, int sms);
 
 }  // namespace sphkv

@@ -1,0 +1,694 @@
+// Causal attention of many queries a sequence over the 8-bit block cache (a prompt's chunk, drafted tokens).
+//
+// The query rows of one KV head (tokens x group heads, flat) are cut into blocks of 256, two tensor-core tiles of 128; the
+// keys into tiles of 128.  A CTA walks a block's key tiles with four kinds of warps:
+//   4 warps  fetch codes a tile ahead into registers and turn them into f16 operands in shared memory (codes are exact in
+//            f16; scales stay apart), keys and values double buffered;
+//   1 warp   issues the products: logits S_t = Q_t K^T and outputs O_t += P_t V, for the two tiles t in turn, so that the tensor
+//            cores work on one tile while the other's softmax runs;
+//   8 warps  softmax, a thread to a query row: S from tensor memory, a page's key scale times the row's factor as one
+//            multiplier for its 16 keys and up, weights 2^6 p v / S_v in f16 back over S as the next product's operand.
+//            The page's value scale is part of the exponent, so it costs nothing per element; the sum of p takes it out
+//            again once for 16 keys.  A row's reference maximum moves only when a logit passes it by 2^8; O is then
+//            rescaled in place (every earlier product is complete: S_t(k) is issued behind P_t V(k - 1)).
+// Q rows are scaled by a power of two as in the decode kernel: bf16 and f16 queries are exact in f16.  Weights have f16's 11
+// bits, sums are fp32.
+//
+// Work: (block, head, key tile) in one line, cut evenly over the CTAs; a block that two or more CTAs share is joined by a
+// second launch.  What bounds it: the exponentials (16 a cycle and SM, 2048 cycles for 256 rows x 128 keys) and, as much, the
+// products (2048 cycles at the nominal rate).
+#include "blocks.cuh"
+
+namespace sphkv {
+
+constexpr int kAtRows = 256, kAtKeys = 128;
+constexpr int kAtThreads = 512;  // warps 0-3, 4-7: softmax of tile 0, 1; 8-11: codes to operands; 12: products
+constexpr int kAtPlanned = 128;  // slots whose tile counts a CTA sums itself
+constexpr float kAtLazy = 8.f;
+constexpr float kAtWeight = 6.f;  // log2: weights stay below 2^15 with the lazy maximum
+
+struct AtArgs {
+  sphkv_blocks c;
+  BlockRows r;
+  const void* q;
+  int64_t q_row_stride, q_head_stride;
+  const int32_t* first;
+  void* out;
+  const int64_t* prefix;
+  float* parts;  // [workers][2][dh + 2][256]: a worker's first, cut segment and its last
+  int q_dtype, out_dtype, Hq, group, slots, workers;
+  bool q_vec;
+  float scale_log2;
+};
+
+struct AtItem {
+  int b, row0;      // sequence, its first dense row
+  int r0, rows;     // flat query rows of the block
+  int pos0;         // position of the sequence's first query
+  int first, lim[2];  // tile t sees keys first .. lim[t] - 1
+  int kt0, tiles;
+};
+__device__ __forceinline__ AtItem item_of(const AtArgs& a, int slot) {
+  const BlockPiece p = find_piece_alone(a.c, a.r, slot, 8, 1);
+  AtItem u = {p.b, p.row0, 0, 0, 0, 0, {0, 0}, 0, 0};
+  const int all = p.n * a.group, r0 = p.j * kAtRows;
+  if (p.b < 0 || r0 >= all) return u;
+  u.r0 = r0;
+  u.rows = min(kAtRows, all - r0);
+  if (p.end < 0) return u;
+  u.pos0 = p.end - p.n;
+  u.lim[0] = u.pos0 + (r0 + min(u.rows, 128) - 1) / a.group + 1;
+  u.lim[1] = u.rows > 128 ? u.pos0 + (r0 + u.rows - 1) / a.group + 1 : 0;
+  const int limit = max(u.lim[0], u.lim[1]);
+  u.first = a.first ? min(max(a.first[p.b], 0), limit) : 0;
+  u.kt0 = u.first / kAtKeys;
+  u.tiles = u.first < limit ? (limit + kAtKeys - 1) / kAtKeys - u.kt0 : 0;
+  return u;
+}
+__global__ void __launch_bounds__(1024) blocks_attend_plan_kernel(const __grid_constant__ AtArgs a, int64_t* prefix) {
+  griddep_wait();
+  sum_tiles(a.slots, prefix, [&](int s) { return item_of(a, s).tiles; });
+}
+
+// ---- shared memory ----------------------------------------------------------------------------------------
+struct AtMeta {       // of a key tile, for the softmax
+  float ks[8];        // key scale of 16 keys
+  float lv[8];        // log2(value scale / S) + 6
+  float up[8];        // 1 / (that, not as a logarithm): takes the value scale out of the sum of weights
+  float down, big;    // S before / S; S
+  uint32_t bad;       // groups without a page
+  uint32_t pad;
+};
+template <int DH>
+struct At {
+  static constexpr int kSlab = 128 * 128;             // 128 rows of 64 f16
+  static constexpr int kOperand = kSlab * (DH / 64);  // keys or values of a tile, or a tile of queries
+  static constexpr int kQ = 0, kK = 2 * kOperand, kV = kK + 2 * kOperand, kMeta = kV + 2 * kOperand;
+  static constexpr int kBars = kMeta + 4 * (int)sizeof(AtMeta);
+  static constexpr int kPrefix = kBars + 24 * 8;
+  static constexpr int kSmem = kPrefix + (kAtPlanned + 1) * 8 + 16 + 1024;
+};
+static_assert(At<128>::kSmem <= 232448, "shared memory of a CTA");
+enum { kKFull = 0, kKFree = 2, kVFull = 4, kVFree = 6, kMFull = 8, kQFull = 12, kSFull = 14, kPFull = 16, kODone = 18, kLast = 20 };
+
+__device__ __forceinline__ void tmem_ld_x32(uint32_t addr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
+      "%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+        "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]),
+        "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]),
+        "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st_x16u(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void sts_u4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// 16-byte chunk `c` (8 of dh f16) of row t: slabs of 64 columns, 128-byte swizzle
+__device__ __forceinline__ uint32_t operand_at(int t, int c) { return (c >> 3) * (128 * 128) + t * 128 + (((c & 7) ^ (t & 7)) << 4); }
+
+// The segments of one worker; every warp walks them by itself.
+struct AtWalk {
+  int64_t pos, stop;
+  AtItem u;
+  int head, from, count, cnt[2], unit;
+  bool cut_front, whole;
+  __device__ __forceinline__ bool next(const AtArgs& a, const int64_t* prefix) {
+    if (pos >= stop) return false;
+    const int slot = slot_at(prefix, a.slots, pos / a.c.Hkv);
+    u = item_of(a, slot);
+    const int64_t in_slot = pos - prefix[slot] * a.c.Hkv;
+    head = (int)(in_slot / u.tiles);
+    from = (int)(in_slot - (int64_t)head * u.tiles);
+    count = (int)min((int64_t)(u.tiles - from), stop - pos);
+    unit = slot * a.c.Hkv + head;
+    pos += count;
+    cut_front = from > 0;
+    whole = count == u.tiles;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) cnt[t] = min(max((u.lim[t] + kAtKeys - 1) / kAtKeys - (u.kt0 + from), 0), count);
+    return true;
+  }
+};
+
+__device__ __forceinline__ void store_row16(void* out, int dtype, int64_t at, const float* v) {  // 16 elements
+  if (dtype == SPHKV_F32) {
+    float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    return;
+  }
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (dtype == SPHKV_BF16) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      w[i] = pack_f16x2(v[2 * i], v[2 * i + 1]);
+    }
+  }
+  uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + at);
+  o[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  o[1] = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
+template <int DH, bool I8>
+__global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __grid_constant__ AtArgs a) {
+  using L = At<DH>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  const uint32_t base = smem_u32(smem), bars = base + L::kBars;
+  int64_t* const prefix_smem = reinterpret_cast<int64_t*>(smem + L::kPrefix);
+  AtMeta* const metas = reinterpret_cast<AtMeta*>(smem + L::kMeta);
+  __shared__ uint32_t tmem_at;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bars + 8 * (kKFull + i), 4), mbar_init(bars + 8 * (kKFree + i), 1);
+      mbar_init(bars + 8 * (kVFull + i), 4), mbar_init(bars + 8 * (kVFree + i), 1);
+      mbar_init(bars + 8 * (kQFull + i), 4), mbar_init(bars + 8 * (kSFull + i), 1);
+      mbar_init(bars + 8 * (kPFull + i), 4), mbar_init(bars + 8 * (kODone + i), 1);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(bars + 8 * (kMFull + i), 1);
+    mbar_init(bars + 8 * kLast, 1);
+    fence_async_smem();
+  }
+  if (warp == 12) tmem_alloc(smem_u32(&tmem_at), 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_at;
+  griddep_launch();
+  griddep_wait();
+  const int64_t* prefix = a.prefix;
+  if (prefix == nullptr) {
+    sum_tiles(a.slots, prefix_smem, [&](int s) { return item_of(a, s).tiles; });
+    prefix = prefix_smem;
+  }
+  AtWalk walk;
+  {
+    const int64_t total = prefix[a.slots] * a.c.Hkv, workers = min((int64_t)a.workers, total);
+    const bool in = blockIdx.x < workers;
+    walk.pos = in ? blockIdx.x * total / workers : 0;
+    walk.stop = in ? (blockIdx.x + 1) * total / workers : 0;
+  }
+  bool lost = false;
+  auto wait = [&](int bar, uint32_t n) {  // the n-th phase, from 0
+    if (!lost && !mbar_wait(bars + 8 * bar, n & 1)) {
+      lost = true;
+      bad_status(a.c, SPHKV_ST_TIMEOUT);
+    }
+    return !lost;
+  };
+  auto warp_wait = [&](int bar, uint32_t n) { return __all_sync(0xffffffffu, wait(bar, n)); };
+
+  if (warp < 8) {
+    // ---------------------------------------------------------------- softmax
+    regs_up<176>();
+    const int t = warp >> 2, row = (warp & 3) * 32 + lane;  // of the tile
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+    const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
+    const float kNone = -3.402823466e38f;
+    uint32_t tile = 0, taken = 0, segs = 0;  // key tiles of the worker; those with this row tile; segments with it
+    while (!lost && walk.next(a, prefix)) {
+      const AtItem& u = walk.u;
+      const int cnt = walk.cnt[t], flat = 128 * t + row;
+      const bool live = flat < u.rows;
+      const int tok = (u.r0 + flat) / a.group, hd = walk.head * a.group + (u.r0 + flat) - tok * a.group;
+      const int64_t dense = (int64_t)u.row0 + tok;
+      const int lim = live ? u.pos0 + tok + 1 : u.lim[t];
+      float m = kNone, l = 0.f, big = 0.f;
+      if (cnt > 0) {
+        // the row of queries: scaled by a power of two into f16
+        uint4 raw[DH / 8];
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (live ? dense * a.q_row_stride + (int64_t)hd * a.q_head_stride : 0);
+        uint32_t top2 = 0;
+#pragma unroll
+        for (int i = 0; i < DH / 8; ++i) {
+          raw[i] = make_uint4(0, 0, 0, 0);
+          if (live) {
+            if (a.q_vec) {
+              raw[i] = *reinterpret_cast<const uint4*>(src + 8 * i);
+            } else {
+              uint32_t w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) w[k] = (uint32_t)src[8 * i + 2 * k] | ((uint32_t)src[8 * i + 2 * k + 1] << 16);
+              raw[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+          top2 = __vmaxu2(__vmaxu2(top2, raw[i].x & 0x7fff7fffu), __vmaxu2(raw[i].y & 0x7fff7fffu, __vmaxu2(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu)));
+        }
+        const uint32_t th = max(top2 >> 16, top2 & 0xffffu);
+        const bool bf = a.q_dtype == SPHKV_BF16;
+        const uint16_t th16 = (uint16_t)th;
+        const uint32_t tb = bf ? th << 16 : __float_as_uint(__half2float(*reinterpret_cast<const __half*>(&th16)));
+        int e = (int)(tb >> 23);
+        e = e == 255 ? 140 : max(e, 14);
+        const float sc = __uint_as_float((uint32_t)(267 - e) << 23), f = __uint_as_float((uint32_t)(e - 13) << 23) * a.scale_log2;
+        const uint32_t q_at = base + L::kQ + t * L::kOperand;
+#pragma unroll
+        for (int i = 0; i < DH / 8; ++i) {
+          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+          uint32_t h[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float2 x;
+            if (bf)
+              x = make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
+            else
+              x = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+            h[k] = pack_f16x2(x.x * sc, x.y * sc);
+          }
+          sts_u4(q_at + operand_at(row, i), h[0], h[1], h[2], h[3]);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars + 8 * (kQFull + t));
+
+        for (int k = 0; k < cnt; ++k) {
+          const uint32_t n = tile + k;
+          // in this order: logits are there only when the key tile is, so that the barrier of its scales is at this phase
+          // or the one before, even where this row tile has skipped some
+          if (!warp_wait(kSFull + t, taken)) break;
+          if (!warp_wait(kMFull + (n & 3), n >> 2)) break;
+          ++taken;
+          tc_fence_after();
+          const AtMeta& meta = metas[n & 3];
+          float s[128];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tmem_ld_x32(s_at + 32 * i, s + 32 * i);
+          tmem_wait_ld();
+          const int key0 = (u.kt0 + walk.from + k) * kAtKeys;
+          const uint32_t bad = meta.bad;
+          const bool edge = __any_sync(0xffffffffu, key0 < u.first || key0 + kAtKeys > lim || bad != 0);
+          if (edge) {
+#pragma unroll
+            for (int c = 0; c < 128; ++c)
+              if (key0 + c < u.first || key0 + c >= lim || ((bad >> (c / 16)) & 1)) s[c] = -INFINITY;
+          }
+          float mx = kNone;
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            float x = s[16 * g];
+#pragma unroll
+            for (int c = 1; c < 16; ++c) x = fmaxf(x, s[16 * g + c]);
+            mx = fmaxf(mx, x * (meta.ks[g] * f));
+          }
+          const float down = meta.down;
+          big = meta.big;
+          if (__any_sync(0xffffffffu, mx > m + kAtLazy) || down != 1.f) {
+            const float to = fmaxf(m, mx), d = ex2(m - to);
+            m = to;
+            l *= d;
+            if (k > 0) {  // O holds something
+              const float r = d * down;
+#pragma unroll
+              for (int i = 0; i < DH / 16; ++i) {
+                float o[16];
+                tmem_ld_x16(o_at + 16 * i, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 16; ++c) o[c] *= r;
+                tmem_st_x16(o_at + 16 * i, o);
+              }
+              tmem_wait_st();
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {  // 32 keys: 16 columns of weights
+            uint32_t p[16];
+#pragma unroll
+            for (int gg = 0; gg < 2; ++gg) {
+              const int g = 2 * h + gg;
+              const float c = meta.ks[g] * f, add = meta.lv[g] - m;
+              float w[16], sum = 0.f;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) w[i] = ex2(fmaf(s[16 * g + i], c, add));
+              if (edge) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) w[i] = s[16 * g + i] == -INFINITY ? 0.f : w[i];
+              }
+#pragma unroll
+              for (int i = 0; i < 16; ++i) sum += w[i];
+              l += sum == 0.f ? 0.f : sum * meta.up[g];  // the scale of keys that are not seen may be NaN
+#pragma unroll
+              for (int i = 0; i < 8; ++i) p[8 * gg + i] = pack_f16x2(w[2 * i], w[2 * i + 1]);
+            }
+            tmem_st_x16u(s_at + 16 * h, p);
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bars + 8 * (kPFull + t));
+        }
+        if (!lost) (void)warp_wait(kODone + t, segs);
+        lost = __any_sync(0xffffffffu, lost);
+        ++segs;
+      }
+      tile += walk.count;
+      if (lost) break;
+      // ---- the segment's outputs ----
+      if (128 * t < u.rows) {
+        const float scale = big * 0x1p-6f;
+        float* const part = a.parts + ((int64_t)blockIdx.x * 2 + (walk.cut_front ? 0 : 1)) * (DH + 2) * kAtRows + flat;
+        const float per = l == 0.f ? 0.f : scale / l;
+        tc_fence_after();
+#pragma unroll 1
+        for (int i = 0; i < DH / 16; ++i) {
+          float o[16];
+          __syncwarp();
+          if (cnt > 0) {
+            tmem_ld_x16(o_at + 16 * i, o);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int c = 0; c < 16; ++c) o[c] = 0.f;
+          }
+          if (live && walk.whole) {
+#pragma unroll
+            for (int c = 0; c < 16; ++c) o[c] = l == 0.f ? 0.f : o[c] * per;
+            store_row16(a.out, a.out_dtype, (dense * a.Hq + hd) * DH + 16 * i, o);
+          } else if (live) {
+#pragma unroll
+            for (int c = 0; c < 16; ++c) part[(2 + 16 * i + c) * kAtRows] = o[c] * scale;
+          }
+        }
+        if (live && !walk.whole) part[0] = l == 0.f ? -INFINITY : m, part[kAtRows] = l;
+        tc_fence_before();
+      }
+    }
+  } else if (warp < 12) {
+    // ---------------------------------------------------------------- codes to operands
+    regs_down<104>();
+    constexpr int NL = DH / 16, TPL = 512 / DH;  // loads of a lane; tokens of a load
+    const int w = warp - 8;
+    // a quarter warp stores 16-byte chunks of two rows that differ in the swizzle's last bit: no bank twice
+    const int ts = DH == 128 ? ((lane >> 2) & 1) + 2 * (lane >> 4) : lane >> 2;
+    const int ch = DH == 128 ? (lane & 3) + 4 * ((lane >> 3) & 1) : lane & 3;
+    const int shift = 31 - __clz(a.c.page_size);
+    uint32_t n = 0;  // key tiles of the worker
+    while (!lost && walk.next(a, prefix)) {
+      const AtItem& u = walk.u;
+      const int limit = max(u.lim[0], u.lim[1]), key_begin = (u.kt0 + walk.from) * kAtKeys;
+      const int32_t* table = a.c.block_table + (int64_t)u.b * a.c.max_blocks;
+      // lanes 0 .. 7 look after a tile's eight groups of 16 keys
+      auto page_of = [&](int k) {
+        const int t0 = key_begin + k * kAtKeys + 16 * (lane & 7);
+        return k < walk.count && t0 < limit ? table[t0 >> shift] : -2;
+      };
+      auto checked = [&](int page) {
+        if (page == -2) return -2;  // behind the keys
+        if (page < 0 || page >= a.c.n_pages) {
+          bad_status(a.c, SPHKV_ST_BAD_BLOCK);
+          return -1;
+        }
+        return page;
+      };
+      uint4 kr[NL], vr[NL];
+      auto load = [&](uint4 (&r)[NL], const void* codes, int k, int page) {
+        const int at_row = page >= 0 ? ((page * a.c.Hkv + walk.head) << shift) + ((key_begin + k * kAtKeys + 16 * (lane & 7)) & (a.c.page_size - 1)) : -1;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+          const int in = TPL * i + ts;  // of this warp's 32 tokens
+          const int r0 = __shfl_sync(0xffffffffu, at_row, 2 * w + (TPL * i) / 16);
+          r[i] = make_uint4(0, 0, 0, 0);  // rows behind the last key may hold anything
+          if (r0 >= 0 && key_begin + k * kAtKeys + 32 * w + in < limit) {
+            const float4 v = ldg_stream_f4(reinterpret_cast<const uint8_t*>(codes) + (int64_t)(r0 + (in & 15)) * DH + 16 * ch);
+            r[i] = make_uint4(__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w));
+          }
+        }
+      };
+      auto store = [&](const uint4 (&r)[NL], uint32_t at) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+          const uint32_t c[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+          uint32_t h[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) codes_to_f16<I8>(c[k], h[2 * k], h[2 * k + 1]);
+          const int t = 32 * w + TPL * i + ts;
+          sts_u4(at + operand_at(t, 2 * ch), h[0], h[1], h[2], h[3]);
+          sts_u4(at + operand_at(t, 2 * ch + 1), h[4], h[5], h[6], h[7]);
+        }
+        fence_async_smem();
+        __syncwarp();
+      };
+      float big = 0.f;
+      int page = checked(page_of(0)), next_page = page_of(1);
+      load(kr, a.c.k_codes, 0, page);
+      for (int k = 0; k < walk.count; ++k, ++n) {
+        const uint32_t st = n & 1;
+        load(vr, a.c.v_codes, k, page);
+        float ks = 0.f, vs = 0.f;
+        if (w == 0 && page >= 0) {
+          ks = a.c.k_scale[page * a.c.Hkv + walk.head];
+          vs = a.c.v_scale[page * a.c.Hkv + walk.head];
+        }
+        if (n >= 2 && !warp_wait(kKFree + st, (n >> 1) - 1)) break;
+        store(kr, base + L::kK + st * L::kOperand);
+        if (lane == 0) mbar_arrive(bars + 8 * (kKFull + st));
+        if (w == 0) {  // the tile's scales
+          float top = vs < INFINITY ? vs : 0.f;  // rows that do not see a page without a scale keep theirs
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          float down = 1.f;
+          if (top > big) {
+            const float b = __uint_as_float((__float_as_uint(top) + 0x7fffffu) & 0x7f800000u);
+            down = big > 0.f ? big / b : 0.f;
+            big = b;
+          }
+          const unsigned bad = __ballot_sync(0xffffffffu, page == -1) & 0xffu;
+          // pages of zeros have scale 0: any other value serves
+          const float ref = big > 0.f ? big : 1.f, v = vs == 0.f ? 1.f : vs * (1.f / ref);
+          AtMeta& mt = metas[n & 3];
+          if (lane < 8) {
+            mt.ks[lane] = ks;
+            mt.lv[lane] = log2f(v) + kAtWeight;
+            mt.up[lane] = 0x1p-6f / v;
+          }
+          if (lane == 0) mt.down = k == 0 ? 1.f : down, mt.big = ref, mt.bad = bad;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bars + 8 * (kMFull + (n & 3)));
+        }
+        page = checked(next_page);
+        next_page = page_of(k + 2);
+        if (k + 1 < walk.count) load(kr, a.c.k_codes, k + 1, page);
+        if (n >= 2 && !warp_wait(kVFree + st, (n >> 1) - 1)) break;
+        store(vr, base + L::kV + st * L::kOperand);
+        if (lane == 0) mbar_arrive(bars + 8 * (kVFull + st));
+      }
+      lost = __any_sync(0xffffffffu, lost);
+    }
+  } else {
+    regs_down<56>();
+    if (warp == 12) {
+      // -------------------------------------------------------------- products
+      constexpr uint32_t kIdescS = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+      constexpr uint32_t kIdescO = (1u << 4) | (((uint32_t)DH >> 3) << 17) | ((128u >> 4) << 24) | (1u << 16);
+      uint32_t n = 0, p_taken[2] = {0, 0}, q_taken[2] = {0, 0};
+      bool issued = false;
+      while (!lost && walk.next(a, prefix)) {
+        const int count = walk.count;
+        bool ok = true;
+        for (int t = 0; t < 2 && ok; ++t)
+          if (walk.cnt[t] > 0) ok = warp_wait(kQFull + t, q_taken[t]++);
+        for (int k = 0; k <= count && ok; ++k) {
+          const uint32_t st = (n + k) & 1, before = (n + k - 1) & 1;
+          if (k < count) ok = warp_wait(kKFull + st, (n + k) >> 1);
+          if (ok && k > 0) ok = warp_wait(kVFull + before, (n + k - 1) >> 1);
+          for (int t = 0; t < 2 && ok; ++t) {
+            if (k > 0 && k - 1 < walk.cnt[t]) {
+              ok = warp_wait(kPFull + t, p_taken[t]++);
+              if (!ok) break;
+              tc_fence_after();
+              if (elect_one()) {
+                const uint64_t v_desc = smem_desc(base + L::kV + before * L::kOperand, DH == 128 ? L::kSlab : 0, 1024, 2);
+#pragma unroll
+                for (int i = 0; i < kAtKeys / 16; ++i)
+                  mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * i, v_desc + (uint64_t)((i * 2048) >> 4), kIdescO, k > 1 || i > 0);
+                if (k == walk.cnt[t]) mma_commit(bars + 8 * (kODone + t));
+              }
+              __syncwarp();
+            }
+            if (k < walk.cnt[t]) {
+              tc_fence_after();
+              if (elect_one()) {
+                const uint64_t q_desc = smem_desc(base + L::kQ + t * L::kOperand, 0, 1024, 2);
+                const uint64_t k_desc = smem_desc(base + L::kK + st * L::kOperand, 0, 1024, 2);
+#pragma unroll
+                for (int i = 0; i < DH / 16; ++i) {
+                  const uint64_t step = (uint64_t)(((i >> 2) * L::kSlab + (i & 3) * 32) >> 4);
+                  mma_ss(tmem + t * 128, q_desc + step, k_desc + step, kIdescS, i > 0);
+                }
+                mma_commit(bars + 8 * (kSFull + t));
+              }
+              __syncwarp();
+              issued = true;
+            }
+          }
+          if (ok && elect_one()) {
+            if (k < count) mma_commit(bars + 8 * (kKFree + st));
+            if (k > 0) mma_commit(bars + 8 * (kVFree + before));
+          }
+          __syncwarp();
+        }
+        lost = __any_sync(0xffffffffu, lost);
+        n += count;
+      }
+      if (issued) {  // nothing may be on its way when tensor and shared memory are given back
+        if (elect_one()) mma_commit(bars + 8 * kLast);
+        __syncwarp();
+        (void)mbar_wait(bars + 8 * kLast, 0);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+// CTA (w, y): the block that worker w begins and others go on with, dims 16 y .. of it; and rows of blocks without keys.
+__global__ void __launch_bounds__(256) blocks_attend_merge_kernel(const __grid_constant__ AtArgs a, int dh) {
+  __shared__ int64_t prefix_smem[kAtPlanned + 1];
+  griddep_launch();
+  griddep_wait();
+  const int64_t* prefix = a.prefix;
+  if (prefix == nullptr) {
+    sum_tiles(a.slots, prefix_smem, [&](int s) { return item_of(a, s).tiles; });
+    prefix = prefix_smem;
+  }
+  const int64_t total = prefix[a.slots] * a.c.Hkv, workers = min((int64_t)a.workers, total);
+  const int flat = threadIdx.x, w = blockIdx.x, d0 = 16 * blockIdx.y;
+  float o[16];
+  for (int s = w; s < a.slots; s += gridDim.x) {
+    if (prefix[s + 1] != prefix[s]) continue;
+    const AtItem u = item_of(a, s);
+    if (flat >= u.rows) continue;
+#pragma unroll
+    for (int c = 0; c < 16; ++c) o[c] = 0.f;
+    const int tok = (u.r0 + flat) / a.group, g = u.r0 + flat - tok * a.group;
+    for (int h = 0; h < a.c.Hkv; ++h) store_row16(a.out, a.out_dtype, ((int64_t)(u.row0 + tok) * a.Hq + h * a.group + g) * dh + d0, o);
+  }
+  if (w >= workers) return;
+  const int64_t start = w * total / workers, stop = (w + 1) * total / workers;
+  const int slot = slot_at(prefix, a.slots, (stop - 1) / a.c.Hkv);
+  const AtItem u = item_of(a, slot);
+  const int64_t in_slot = stop - 1 - prefix[slot] * a.c.Hkv;
+  const int head = (int)(in_slot / u.tiles);
+  const int64_t p0 = prefix[slot] * a.c.Hkv + (int64_t)head * u.tiles, p1 = p0 + u.tiles - 1;
+  if (p0 < start || p1 < stop || flat >= u.rows) return;
+  const int64_t last = ((p1 + 1) * workers - 1) / total;
+  const int64_t size = (int64_t)(dh + 2) * kAtRows;
+  float top = -INFINITY, sum = 0.f;
+  auto part = [&](int64_t x) { return a.parts + (2 * x + (x == w ? 1 : 0)) * size + flat; };
+  for (int64_t x = w; x <= last; ++x) top = fmaxf(top, part(x)[0]);
+#pragma unroll
+  for (int c = 0; c < 16; ++c) o[c] = 0.f;
+  for (int64_t x = w; x <= last; ++x) {
+    const float* p = part(x);
+    if (p[0] == -INFINITY) continue;  // nothing seen there
+    const float f = ex2(p[0] - top);
+    sum += p[kAtRows] * f;
+#pragma unroll
+    for (int c = 0; c < 16; ++c) o[c] += p[(2 + d0 + c) * kAtRows] * f;
+  }
+#pragma unroll
+  for (int c = 0; c < 16; ++c) o[c] = sum == 0.f ? 0.f : o[c] / sum;
+  const int tok = (u.r0 + flat) / a.group, hd = head * a.group + u.r0 + flat - tok * a.group;
+  store_row16(a.out, a.out_dtype, ((int64_t)(u.row0 + tok) * a.Hq + hd) * dh + d0, o);
+}
+
+static int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+static int64_t at_slots(int64_t rows, int B, int group) { return (rows * group >> 8) + B; }  // at least block_slots()
+static int64_t at_scratch(int64_t rows, int B, int group, int dh, int sms) {
+  return align256((at_slots(rows, B, group) + 1) * 8) + (int64_t)sms * 2 * (dh + 2) * kAtRows * 4;
+}
+
+template <int DH, bool I8>
+static int launch_at(const AtArgs& a, cudaStream_t st) {
+  static SmemOptIn opt_in;
+  auto kern = blocks_attend_kernel<DH, I8>;
+  if (int rc = ensure_dynamic_smem(opt_in, (const void*)kern, At<DH>::kSmem, "blocks_attend")) return rc;
+  (void)launch_overlapped(kern, dim3(a.workers), dim3(kAtThreads), At<DH>::kSmem, st, a);
+  return check_launch("blocks_attend_kernel");
+}
+
+// One sequence's tokens in the decode kernel's eight rows: there the codes are not turned into operands in shared memory.
+static bool few_rows(const BlockRows& r, int B, int group) { return r.rows <= (int64_t)B << tokens_shift(group); }
+
+}  // namespace sphkv
+
+using namespace sphkv;
+
+extern "C" int64_t sphkv_blocks_attend_scratch_bytes(int32_t B, int64_t rows, int32_t Hq, int32_t Hkv, int32_t dh) {
+  if (B <= 0 || rows < 0 || rows > 0x7ffffff || Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq / Hkv > SPHKV_MAX_GQA || (dh != 64 && dh != 128))
+    return SPHKV_E_ARG;
+  const int sms = sm_count_current_device();
+  if (sms <= 0) return sms;
+  const int group = Hq / Hkv;
+  const int64_t many = at_scratch(rows, B, group, dh, sms);
+  const BlockRows r = {nullptr, (int)rows, 0, 1, false};
+  return few_rows(r, B, group) ? max(many, few_queries_scratch(rows, B, Hkv, dh, tokens_shift(group), sms)) : many;
+}
+
+extern "C" int sphkv_blocks_attend(const sphkv_blocks* c, const void* q, int32_t q_dtype, int64_t q_row_stride, int64_t q_head_stride,
+                                   const int32_t* cu, int64_t rows, const int32_t* first, void* out, int32_t out_dtype, void* scratch,
+                                   int64_t scratch_bytes, int32_t Hq, float sm_scale, void* stream) {
+  if (int rc = check_blocks(c, "blocks_attend")) return rc;
+  AtArgs a = {};
+  a.c = *c;
+  if (int rc = block_rows(a.r, c, cu, rows, "blocks_attend")) return rc;
+  SPHKV_REQUIRE(rows <= 0x7ffffff, SPHKV_E_LIMIT, "blocks_attend: rows=%lld (max 2^27 - 1)", (long long)rows);
+  SPHKV_REQUIRE(rows == 0 || q != nullptr, SPHKV_E_ARG, "blocks_attend: q is NULL");
+  if (int rc = check_queries(*c, q, q_dtype, out, nullptr, out_dtype, Hq, "blocks_attend")) return rc;
+  SPHKV_REQUIRE(q_dtype != SPHKV_F32, SPHKV_E_DTYPE, "blocks_attend: q_dtype=%d (16-bit types)", q_dtype);
+  SPHKV_REQUIRE(((uintptr_t)out & 15) == 0, SPHKV_E_ALIGN, "blocks_attend: out needs 16 B");
+  if (rows == 0) return 0;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int group = Hq / c->Hkv, sms = sm_count_current_device();
+  if (sms <= 0) return sms;
+  if (few_rows(a.r, c->B, group))
+    return few_queries(*c, a.r, q, q_dtype, q_row_stride, q_head_stride, first, out, out_dtype, nullptr, scratch, scratch_bytes, Hq, sm_scale,
+                       tokens_shift(group), "blocks_attend", st);
+  a.r.mul = group;
+  a.q = q;
+  a.q_dtype = q_dtype;
+  a.q_row_stride = q_row_stride;
+  a.q_head_stride = q_head_stride;
+  a.q_vec = ((uintptr_t)q & 15) == 0 && (((q_row_stride | q_head_stride) * 2) & 15) == 0;
+  a.first = first;
+  a.out = out;
+  a.out_dtype = out_dtype;
+  a.Hq = Hq;
+  a.group = group;
+  a.scale_log2 = sm_scale * kLog2e;
+  a.workers = sms;
+  const int64_t slots = block_slots(a.r, c->B, 8, 1);
+  SPHKV_REQUIRE(slots * c->Hkv <= 0x7fffffff, SPHKV_E_LIMIT, "blocks_attend: too many queries for one launch");
+  a.slots = (int)slots;
+  const int64_t need = at_scratch(rows, c->B, group, c->dh, sms);
+  SPHKV_REQUIRE(scratch != nullptr && scratch_bytes >= need, SPHKV_E_SCRATCH, "blocks_attend: scratch %lld B < %lld B",
+                (long long)scratch_bytes, (long long)need);
+  SPHKV_REQUIRE(((uintptr_t)scratch & 255) == 0, SPHKV_E_ALIGN, "blocks_attend: scratch needs 256 B");
+  a.parts = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(scratch) + align256((at_slots(rows, c->B, group) + 1) * 8));
+  if (slots > kAtPlanned) {
+    int64_t* prefix = reinterpret_cast<int64_t*>(scratch);
+    (void)launch_overlapped(blocks_attend_plan_kernel, dim3(1), dim3(1024), 0, st, a, prefix);
+    if (int rc = check_launch("blocks_attend_plan_kernel")) return rc;
+    a.prefix = prefix;
+  }
+  const bool i8 = c->store == SPHKV_BLOCKS_I8;
+  const int rc = c->dh == 128 ? (i8 ? launch_at<128, true>(a, st) : launch_at<128, false>(a, st))
+                              : (i8 ? launch_at<64, true>(a, st) : launch_at<64, false>(a, st));
+  if (rc) return rc;
+  (void)launch_overlapped(blocks_attend_merge_kernel, dim3(a.workers, c->dh / 16), dim3(256), 0, st, a, (int)c->dh);
+  return check_launch("blocks_attend_merge_kernel");
+}

@@ -76,47 +76,15 @@ __device__ __forceinline__ BdUnit unit_of(const BdArgs& a, const BlockPiece& p) 
   return u;
 }
 
-// prefix[s] = tiles of the slots before s, prefix[slots] = all; by one block
-__device__ __forceinline__ void sum_tiles(const BdArgs& a, int64_t* prefix) {
-  __shared__ int64_t warp_sums[32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int64_t before = 0;
-  for (int s0 = 0; s0 < a.slots; s0 += blockDim.x) {
-    const int s = s0 + tid;
-    int64_t v = s < a.slots ? unit_of(a, find_piece_alone(a.c, a.r, s, a.tshift, 1)).tiles : 0;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += up;
-    }
-    if (lane == 31) warp_sums[warp] = v;
-    __syncthreads();
-    int64_t add = before;
-    for (int w = 0; w < (int)blockDim.x / 32; ++w) {
-      if (w < warp) add += warp_sums[w];
-      before += warp_sums[w];
-    }
-    if (s < a.slots) prefix[s + 1] = v + add;
-    __syncthreads();
-  }
-  if (tid == 0) prefix[0] = 0;
-  __syncthreads();
+__device__ __forceinline__ void sum_unit_tiles(const BdArgs& a, int64_t* prefix) {
+  sum_tiles(a.slots, prefix, [&](int s) { return unit_of(a, find_piece_alone(a.c, a.r, s, a.tshift, 1)).tiles; });
 }
 __global__ void __launch_bounds__(1024) blocks_plan_kernel(const __grid_constant__ BdArgs a, int64_t* prefix) {
   griddep_wait();
-  sum_tiles(a, prefix);
+  sum_unit_tiles(a, prefix);
 }
 // the workers that share the tiles: none goes without, so that a unit's segments are those of consecutive workers
 __device__ __forceinline__ int64_t workers_of(const BdArgs& a, int64_t total) { return min((int64_t)a.workers, total); }
-__device__ __forceinline__ int slot_at(const int64_t* prefix, int slots, int64_t tile) {  // prefix[s] <= tile < prefix[s + 1]
-  int lo = 0, hi = slots;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    (prefix[mid] <= tile ? lo : hi) = mid;
-  }
-  return lo;
-}
-
 __device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -136,11 +104,6 @@ __device__ __forceinline__ uint2 lds_u2(uint32_t at) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
   return v;
-}
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
 }
 // where 16-byte chunk c of row t lies in a tile that a tensor copy has swizzled
 template <int DH>
@@ -179,7 +142,7 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
   griddep_wait();
   const int64_t* prefix = a.prefix;
   if (prefix == nullptr) {
-    sum_tiles(a, prefix_smem);
+    sum_unit_tiles(a, prefix_smem);
     prefix = prefix_smem;
   }
   const int64_t total = prefix[a.slots] * a.c.Hkv;
@@ -366,7 +329,7 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
       const float x0 = fmaxf(x[0], x[2]), x1 = fmaxf(x[1], x[3]);
       t0 = fmaxf(t0, x0);
       t1 = fmaxf(t1, x1);
-      const bool larger = vs > big && row >= 0;
+      const bool larger = vs > big && vs < INFINITY && row >= 0;
       if (__any_sync(0xffffffffu, x0 > m0 + kLazy || x1 > m1 + kLazy) || larger) {
         float n0 = x0, n1 = x1;
 #pragma unroll
@@ -380,7 +343,6 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
         if (larger) {
           const float b = __uint_as_float((__float_as_uint(vs) + 0x7fffffu) & 0x7f800000u);
           per_big = __uint_as_float(0x7f000000u - __float_as_uint(b));
-          if (__float_as_uint(b) > 0x7e800000u) per_big = 0.f;
           down = big * per_big;
           big = b;
         }
@@ -506,7 +468,7 @@ __global__ void __launch_bounds__(256) blocks_merge_kernel(const __grid_constant
   griddep_wait();
   const int64_t* prefix = a.prefix;
   if (prefix == nullptr) {
-    sum_tiles(a, prefix_smem);
+    sum_unit_tiles(a, prefix_smem);
     prefix = prefix_smem;
   }
   const int unit = blockIdx.x, slot = unit / a.c.Hkv, head = unit - slot * a.c.Hkv;
@@ -543,7 +505,7 @@ __global__ void __launch_bounds__(256) blocks_merge_kernel(const __grid_constant
   }
 }
 
-static int tokens_shift(int group) { return group == 1 ? 3 : group == 2 ? 2 : group <= 4 ? 1 : 0; }
+int tokens_shift(int group) { return group == 1 ? 3 : group == 2 ? 2 : group <= 4 ? 1 : 0; }
 static int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
 static int64_t bd_scratch(int64_t slots, int Hkv, int dh, int workers) {
@@ -593,9 +555,8 @@ static int run_bd(BdArgs& a, void* scratch, int64_t scratch_bytes, const char* w
   return check_launch("blocks_merge_kernel");
 }
 
-static int check_queries(BdArgs& a, const void* q, int q_dtype, const void* out, const float* out_partial, int out_dtype, int Hq,
-                         const char* what) {
-  const sphkv_blocks& c = a.c;
+int check_queries(const sphkv_blocks& c, const void* q, int q_dtype, const void* out, const float* out_partial, int out_dtype, int Hq,
+                  const char* what) {
   SPHKV_REQUIRE(out || out_partial, SPHKV_E_ARG, "%s: no output", what);
   SPHKV_REQUIRE(q_dtype >= 0 && q_dtype <= 2 && out_dtype >= 0 && out_dtype <= 2, SPHKV_E_DTYPE, "%s: q_dtype=%d out_dtype=%d", what,
                 q_dtype, out_dtype);
@@ -604,12 +565,32 @@ static int check_queries(BdArgs& a, const void* q, int q_dtype, const void* out,
   const int64_t q_size = q_dtype == SPHKV_F32 ? 4 : 2, o_size = out_dtype == SPHKV_F32 ? 4 : 2;
   SPHKV_REQUIRE(((uintptr_t)q & (q_size - 1)) == 0 && ((uintptr_t)out & (o_size - 1)) == 0 && ((uintptr_t)out_partial & 3) == 0,
                 SPHKV_E_ALIGN, "%s: q or an output is not on an element's boundary", what);
-  a.Hq = Hq;
-  a.group = Hq / c.Hkv;
+  return 0;
+}
+
+// Attention of the queries of `r` through this kernel.
+int few_queries(const sphkv_blocks& c, const BlockRows& r, const void* q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride,
+                const int32_t* first, void* out, int out_dtype, float* out_partial, void* scratch, int64_t scratch_bytes, int Hq,
+                float sm_scale, int tshift, const char* what, cudaStream_t st) {
+  BdArgs a = {};
+  a.c = c;
+  a.r = r;
   a.q = q;
   a.q_dtype = q_dtype;
+  a.q_row_stride = q_row_stride;
+  a.q_head_stride = q_head_stride;
+  a.first = first;
+  a.out = out;
   a.out_dtype = out_dtype;
-  return 0;
+  a.out_partial = out_partial;
+  a.Hq = Hq;
+  a.group = Hq / c.Hkv;
+  a.tshift = tshift;
+  a.scale_log2 = sm_scale * kLog2e;
+  return run_bd(a, scratch, scratch_bytes, what, st);
+}
+int64_t few_queries_scratch(int64_t rows, int B, int Hkv, int dh, int tshift, int sms) {
+  return bd_scratch((rows >> tshift) + B, Hkv, dh, sms);
 }
 
 }  // namespace sphkv
@@ -627,44 +608,9 @@ extern "C" int sphkv_blocks_decode(const sphkv_blocks* c, const void* q, int32_t
                                    int64_t scratch_bytes, int32_t Hq, float sm_scale, void* stream) {
   if (int rc = check_blocks(c, "blocks_decode")) return rc;
   SPHKV_REQUIRE(q != nullptr, SPHKV_E_ARG, "blocks_decode: q is NULL");
-  BdArgs a = {};
-  a.c = *c;
-  if (int rc = check_queries(a, q, q_dtype, out, out_partial, out_dtype, Hq, "blocks_decode")) return rc;
-  // a sequence without tokens has a query all the same: one row a sequence, whatever ends[] says
-  a.r = {nullptr, c->B, 1, true};
-  a.tshift = 0;
-  a.first = first;
-  a.q_row_stride = q_row_stride;
-  a.q_head_stride = q_head_stride;
-  a.out = out;
-  a.out_partial = out_partial;
-  a.scale_log2 = sm_scale * kLog2e;
-  return run_bd(a, scratch, scratch_bytes, "blocks_decode", reinterpret_cast<cudaStream_t>(stream));
-}
-
-extern "C" int64_t sphkv_blocks_attend_scratch_bytes(int32_t B, int64_t rows, int32_t Hq, int32_t Hkv, int32_t dh) {
-  if (B <= 0 || rows < 0 || rows > 0x1fffffff || Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq / Hkv > SPHKV_MAX_GQA || (dh != 64 && dh != 128))
-    return SPHKV_E_ARG;
-  const int sms = sm_count_current_device();
-  return sms <= 0 ? sms : bd_scratch((rows >> tokens_shift(Hq / Hkv)) + B, Hkv, dh, sms);
-}
-
-extern "C" int sphkv_blocks_attend(const sphkv_blocks* c, const void* q, int32_t q_dtype, int64_t q_row_stride, int64_t q_head_stride,
-                                   const int32_t* cu, int64_t rows, const int32_t* first, void* out, int32_t out_dtype, void* scratch,
-                                   int64_t scratch_bytes, int32_t Hq, float sm_scale, void* stream) {
-  if (int rc = check_blocks(c, "blocks_attend")) return rc;
-  BdArgs a = {};
-  a.c = *c;
-  if (int rc = block_rows(a.r, c, cu, rows, "blocks_attend")) return rc;
-  SPHKV_REQUIRE(rows == 0 || q != nullptr, SPHKV_E_ARG, "blocks_attend: q is NULL");
-  if (int rc = check_queries(a, q, q_dtype, out, nullptr, out_dtype, Hq, "blocks_attend")) return rc;
-  SPHKV_REQUIRE(q_dtype != SPHKV_F32, SPHKV_E_DTYPE, "blocks_attend: q_dtype=%d (16-bit types)", q_dtype);
-  if (rows == 0) return 0;
-  a.tshift = tokens_shift(a.group);
-  a.first = first;
-  a.q_row_stride = q_row_stride;
-  a.q_head_stride = q_head_stride;
-  a.out = out;
-  a.scale_log2 = sm_scale * kLog2e;
-  return run_bd(a, scratch, scratch_bytes, "blocks_attend", reinterpret_cast<cudaStream_t>(stream));
+  if (int rc = check_queries(*c, q, q_dtype, out, out_partial, out_dtype, Hq, "blocks_decode")) return rc;
+  // one row a sequence, whatever ends[] says: one without tokens has a query all the same
+  const BlockRows r = {nullptr, c->B, 1, 1, true};
+  return few_queries(*c, r, q, q_dtype, q_row_stride, q_head_stride, first, out, out_dtype, out_partial, scratch, scratch_bytes, Hq,
+                     sm_scale, 0, "blocks_decode", reinterpret_cast<cudaStream_t>(stream));
 }
