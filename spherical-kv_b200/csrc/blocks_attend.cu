@@ -22,7 +22,13 @@
 namespace sphkv {
 
 constexpr int kAtRows = 256, kAtKeys = 128;
-constexpr int kAtThreads = 512;  // warps 0-3, 4-7: softmax of tile 0, 1; 8-11: codes to operands; 12: products
+constexpr int kAtThreads = 640;  // warps 0-3, 4-7: softmax of tile 0, 1; 8-11, 12-15: keys, values to operands; 16: products;
+// 17: scales; 18, 19 have no work
+constexpr int kAtProducts = 16;
+// Registers of a thread: at launch; after the softmax has taken what the others gave up.  The file is four quarters, with
+// five warps each (two of softmax, two of codes, one of 16 .. 19), so what goes up has to come down quarter by quarter.
+constexpr int kAtRegs = 96, kAtRegsSoftmax = 120, kAtRegsCodes = 80, kAtRegsRest = 80;
+static_assert(2 * kAtRegsSoftmax + 2 * kAtRegsCodes + kAtRegsRest <= 5 * kAtRegs && 20 * 32 * kAtRegs <= 65536, "registers");
 constexpr int kAtPlanned = 128;  // slots whose tile counts a CTA sums itself
 constexpr float kAtLazy = 8.f;
 constexpr float kAtWeight = 6.f;  // log2: weights stay below 2^15 with the lazy maximum
@@ -72,13 +78,13 @@ __global__ void __launch_bounds__(1024) blocks_attend_plan_kernel(const __grid_c
 
 // ---- shared memory ----------------------------------------------------------------------------------------
 struct AtMeta {       // of a key tile, for the softmax
-  float ks[8];        // key scale of 16 keys
-  float lv[8];        // log2(value scale / S) + 6
-  float up[8];        // 1 / (that, not as a logarithm): takes the value scale out of the sum of weights
+  float4 of[8];       // of 16 keys: key scale; log2(value scale / S) + 6; 1 / (that, not as a logarithm), which takes the value
+                      // scale out of the sum of weights; unused
   float down, big;    // S before / S; S
   uint32_t bad;       // groups without a page
   uint32_t pad;
 };
+constexpr int kAtWalkBytes = 96;
 template <int DH>
 struct At {
   static constexpr int kSlab = 128 * 128;             // 128 rows of 64 f16
@@ -86,10 +92,11 @@ struct At {
   static constexpr int kQ = 0, kK = 2 * kOperand, kV = kK + 2 * kOperand, kMeta = kV + 2 * kOperand;
   static constexpr int kBars = kMeta + 4 * (int)sizeof(AtMeta);
   static constexpr int kPrefix = kBars + 24 * 8;
-  static constexpr int kSmem = kPrefix + (kAtPlanned + 1) * 8 + 16 + 1024;
+  static constexpr int kWalks = kPrefix + (kAtPlanned + 1) * 8;
+  static constexpr int kSmem = kWalks + kAtThreads / 32 * kAtWalkBytes + 1024;
 };
 static_assert(At<128>::kSmem <= 232448, "shared memory of a CTA");
-enum { kKFull = 0, kKFree = 2, kVFull = 4, kVFree = 6, kMFull = 8, kQFull = 12, kSFull = 14, kPFull = 16, kODone = 18, kLast = 20 };
+enum { kKFull = 0, kKFree = 2, kVFull = 4, kVFree = 6, kMFull = 8, kQFull = 12, kSFull = 14, kPFull = 16, kODone = 18, kPHalf = 20, kLast = 22 };
 
 __device__ __forceinline__ void tmem_ld_x32(uint32_t addr, float* v) {
   asm volatile(
@@ -108,35 +115,75 @@ __device__ __forceinline__ void tmem_st_x16u(uint32_t addr, const uint32_t* v) {
       "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st_x8u(uint32_t addr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 __device__ __forceinline__ void sts_u4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// 2^x without the exponential unit: x = n + r, n whole (Cody and Waite), a polynomial of degree 4 for 2^r on [-1/2, 1/2] (fitted
+// by Remez' exchange: 2^-18.5 relative), and the product with 2^n, which leaves NaN as it is.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));  // -126
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
+  const float2 magic = make_float2(12582912.f, 12582912.f), minus = make_float2(-1.f, -1.f);  // 1.5 * 2^23
+  const float2 t = __fadd2_rn(x, magic);
+  const float2 n = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
+  const float2 r = __ffma2_rn(n, minus, x);
+  float2 p = make_float2(0.009570102207362652f, 0.009570102207362652f);
+  p = __ffma2_rn(p, r, make_float2(0.05591785907745361f, 0.05591785907745361f));
+  p = __ffma2_rn(p, r, make_float2(0.240247443318367f, 0.240247443318367f));
+  p = __ffma2_rn(p, r, make_float2(0.6931217908859253f, 0.6931217908859253f));
+  p = __ffma2_rn(p, r, make_float2(0.9999992847442627f, 0.9999992847442627f));
+  const float2 two_n = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
+                                   __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
+  return __fmul2_rn(p, two_n);
 }
 // 16-byte chunk `c` (8 of dh f16) of row t: slabs of 64 columns, 128-byte swizzle
 __device__ __forceinline__ uint32_t operand_at(int t, int c) { return (c >> 3) * (128 * 128) + t * 128 + (((c & 7) ^ (t & 7)) << 4); }
 
-// The segments of one worker; every warp walks them by itself.
+// The segments of one worker; every warp walks them by itself, in a place of its own in shared memory: registers are what the
+// loops are short of, and local memory is L2 where shared memory takes all of L1.
 struct AtWalk {
-  int64_t pos, stop;
+  int64_t left;  // tiles
   AtItem u;
-  int head, from, count, cnt[2], unit;
-  bool cut_front, whole;
-  __device__ __forceinline__ bool next(const AtArgs& a, const int64_t* prefix) {
-    if (pos >= stop) return false;
-    const int slot = slot_at(prefix, a.slots, pos / a.c.Hkv);
+  int slot, head, from, count, cnt[2];
+  bool whole;
+  __device__ __forceinline__ void begin(const AtArgs& a, const int64_t* prefix, int64_t worker) {
+    const int64_t total = prefix[a.slots] * a.c.Hkv, workers = min((int64_t)a.workers, total);
+    left = 0;
+    count = 0;
+    if (worker >= workers) return;
+    const int64_t pos = worker * total / workers;
+    left = (worker + 1) * total / workers - pos;
+    slot = slot_at(prefix, a.slots, pos / a.c.Hkv);
     u = item_of(a, slot);
     const int64_t in_slot = pos - prefix[slot] * a.c.Hkv;
     head = (int)(in_slot / u.tiles);
     from = (int)(in_slot - (int64_t)head * u.tiles);
-    count = (int)min((int64_t)(u.tiles - from), stop - pos);
-    unit = slot * a.c.Hkv + head;
-    pos += count;
-    cut_front = from > 0;
+  }
+  __device__ __forceinline__ bool next(const AtArgs& a) {
+    if (left == 0) return false;
+    if (count > 0) {  // behind a segment: the next head, or the next block with keys
+      from = 0;
+      if (++head == a.c.Hkv) {
+        head = 0;
+        do u = item_of(a, ++slot);
+        while (u.tiles == 0);  // there is one: left > 0
+      }
+    }
+    count = (int)min((int64_t)(u.tiles - from), left);
+    left -= count;
     whole = count == u.tiles;
 #pragma unroll
     for (int t = 0; t < 2; ++t) cnt[t] = min(max((u.lim[t] + kAtKeys - 1) / kAtKeys - (u.kt0 + from), 0), count);
     return true;
   }
 };
+
+static_assert(sizeof(AtWalk) <= kAtWalkBytes, "a warp's place");
 
 __device__ __forceinline__ void store_row16(void* out, int dtype, int64_t at, const float* v) {  // 16 elements
   if (dtype == SPHKV_F32) {
@@ -175,13 +222,13 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
       mbar_init(bars + 8 * (kKFull + i), 4), mbar_init(bars + 8 * (kKFree + i), 1);
       mbar_init(bars + 8 * (kVFull + i), 4), mbar_init(bars + 8 * (kVFree + i), 1);
       mbar_init(bars + 8 * (kQFull + i), 4), mbar_init(bars + 8 * (kSFull + i), 1);
-      mbar_init(bars + 8 * (kPFull + i), 4), mbar_init(bars + 8 * (kODone + i), 1);
+      mbar_init(bars + 8 * (kPFull + i), 4), mbar_init(bars + 8 * (kPHalf + i), 4), mbar_init(bars + 8 * (kODone + i), 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(bars + 8 * (kMFull + i), 1);
     mbar_init(bars + 8 * kLast, 1);
     fence_async_smem();
   }
-  if (warp == 12) tmem_alloc(smem_u32(&tmem_at), 512);
+  if (warp == kAtProducts) tmem_alloc(smem_u32(&tmem_at), 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -193,13 +240,9 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
     sum_tiles(a.slots, prefix_smem, [&](int s) { return item_of(a, s).tiles; });
     prefix = prefix_smem;
   }
-  AtWalk walk;
-  {
-    const int64_t total = prefix[a.slots] * a.c.Hkv, workers = min((int64_t)a.workers, total);
-    const bool in = blockIdx.x < workers;
-    walk.pos = in ? blockIdx.x * total / workers : 0;
-    walk.stop = in ? (blockIdx.x + 1) * total / workers : 0;
-  }
+  AtWalk& walk = *reinterpret_cast<AtWalk*>(smem + L::kWalks + warp * kAtWalkBytes);
+  const AtItem& u = walk.u;
+  if (lane == 0) walk.begin(a, prefix, blockIdx.x);
   bool lost = false;
   auto wait = [&](int bar, uint32_t n) {  // the n-th phase, from 0
     if (!lost && !mbar_wait(bars + 8 * bar, n & 1)) {
@@ -209,24 +252,30 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
     return !lost;
   };
   auto warp_wait = [&](int bar, uint32_t n) { return __all_sync(0xffffffffu, wait(bar, n)); };
+  auto next_segment = [&] {
+    __syncwarp();
+    const int more = lane == 0 ? walk.next(a) : 0;
+    return __shfl_sync(0xffffffffu, more, 0) != 0;  // and what lane 0 wrote is there for all
+  };
 
   if (warp < 8) {
     // ---------------------------------------------------------------- softmax
-    regs_up<176>();
+    regs_up<kAtRegsSoftmax>();
     const int t = warp >> 2, row = (warp & 3) * 32 + lane;  // of the tile
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
     const float kNone = -3.402823466e38f;
     uint32_t tile = 0, taken = 0, segs = 0;  // key tiles of the worker; those with this row tile; segments with it
-    while (!lost && walk.next(a, prefix)) {
-      const AtItem& u = walk.u;
+    while (!lost && next_segment()) {
       const int cnt = walk.cnt[t], flat = 128 * t + row;
-      const bool live = flat < u.rows;
-      const int tok = (u.r0 + flat) / a.group, hd = walk.head * a.group + (u.r0 + flat) - tok * a.group;
-      const int64_t dense = (int64_t)u.row0 + tok;
-      const int lim = live ? u.pos0 + tok + 1 : u.lim[t];
       float m = kNone, l = 0.f, big = 0.f;
       if (cnt > 0) {
+        const bool live = flat < u.rows;
+        const int tok = (u.r0 + flat) / a.group, hd = walk.head * a.group + (u.r0 + flat) - tok * a.group;
+        const int64_t dense = (int64_t)u.row0 + tok;
+        const int lim = live ? u.pos0 + tok + 1 : u.lim[t], first = u.first;
+        const int least = u.pos0 + (u.r0 + 128 * t) / a.group + 1;  // of the tile's rows
+        const int seg_key0 = (u.kt0 + walk.from) * kAtKeys;
         // the row of queries: scaled by a power of two into f16
         uint4 raw[DH / 8];
         const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (live ? dense * a.q_row_stride + (int64_t)hd * a.q_head_stride : 0);
@@ -281,36 +330,57 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
           if (!warp_wait(kMFull + (n & 3), n >> 2)) break;
           ++taken;
           tc_fence_after();
-          const AtMeta& meta = metas[n & 3];
-          float s[128];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) tmem_ld_x32(s_at + 32 * i, s + 32 * i);
-          tmem_wait_ld();
-          const int key0 = (u.kt0 + walk.from + k) * kAtKeys;
-          const uint32_t bad = meta.bad;
-          const bool edge = __any_sync(0xffffffffu, key0 < u.first || key0 + kAtKeys > lim || bad != 0);
-          if (edge) {
-#pragma unroll
-            for (int c = 0; c < 128; ++c)
-              if (key0 + c < u.first || key0 + c >= lim || ((bad >> (c / 16)) & 1)) s[c] = -INFINITY;
-          }
+          const uint32_t meta_at = base + L::kMeta + (n & 3) * (uint32_t)sizeof(AtMeta);  // read anew in every pass: kept, 32 registers would not be there for logits
+          const int key0 = seg_key0 + k * kAtKeys;
+          const float4 tail = lds_f4(meta_at + 128);
+          const float down = tail.x;
+          big = tail.y;
+          const uint32_t bad = __float_as_uint(tail.z);
+          const bool edge = key0 < first || key0 + kAtKeys > least || bad != 0;  // the same for all rows of the tile
           float mx = kNone;
+          auto highest = [&](const float* x, int g) {
+            float top = fmaxf(fmaxf(x[0], x[1]), x[2]);
 #pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            float x = s[16 * g];
+            for (int i = 3; i < 15; i += 2) top = fmaxf(fmaxf(top, x[i]), x[i + 1]);
+            mx = fmaxf(mx, fmaxf(top, x[15]) * (lds_f4(meta_at + 16 * g).x * f));
+          };
+          if (edge) {  // logits of keys that are not seen become -inf, in place
+#pragma unroll 1
+            for (int g = 0; g < 8; ++g) {
+              float x[16];
+              tmem_ld_x16(s_at + 16 * g, x);
+              tmem_wait_ld();
 #pragma unroll
-            for (int c = 1; c < 16; ++c) x = fmaxf(x, s[16 * g + c]);
-            mx = fmaxf(mx, x * (meta.ks[g] * f));
+              for (int c = 0; c < 16; ++c)
+                if (key0 + 16 * g + c < first || key0 + 16 * g + c >= lim || ((bad >> g) & 1)) x[c] = -INFINITY;
+              highest(x, g);
+              tmem_st_x16(s_at + 16 * g, x);
+            }
+            tmem_wait_st();
+          } else {
+            // loops that stay loops: with all 128 keys in sight the compiler starts more than it has registers for
+            float s[2][32];
+            tmem_ld_x32(s_at, s[0]);
+#pragma unroll 1
+            for (int h = 0; h < 4; h += 2) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                tmem_wait_ld();
+                if (i == 0 || h == 0) tmem_ld_x32(s_at + 32 * (h + i + 1), s[i ^ 1]);
+                highest(s[i], 2 * (h + i));
+                highest(s[i] + 16, 2 * (h + i) + 1);
+              }
+            }
           }
-          const float down = meta.down;
-          big = meta.big;
+          float x[2][16];
+          tmem_ld_x16(s_at, x[0]);
           if (__any_sync(0xffffffffu, mx > m + kAtLazy) || down != 1.f) {
-            const float to = fmaxf(m, mx), d = ex2(m - to);
+            const float to = mx > m + kAtLazy ? mx : m, d = ex2(m - to);
             m = to;
             l *= d;
             if (k > 0) {  // O holds something
               const float r = d * down;
-#pragma unroll
+#pragma unroll 1
               for (int i = 0; i < DH / 16; ++i) {
                 float o[16];
                 tmem_ld_x16(o_at + 16 * i, o);
@@ -319,35 +389,65 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
                 for (int c = 0; c < 16; ++c) o[c] *= r;
                 tmem_st_x16(o_at + 16 * i, o);
               }
-              tmem_wait_st();
             }
           }
+          auto weighed = [&](int bar) {  // the weights of half the keys, or of all, are in tensor memory
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bars + 8 * (bar + t));
+          };
+          // weights of 16 keys; returns their sum
+          auto weigh = [&](const float* v, const float4& of, uint32_t* p) {
+            const float c = of.x * f, add = of.y - m;
+            float2 part = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int h = 0; h < 4; ++h) {  // 32 keys: 16 columns of weights
-            uint32_t p[16];
+            for (int i = 0; i < 8; ++i) {
+              float2 e = __ffma2_rn(make_float2(v[2 * i], v[2 * i + 1]), make_float2(c, c), make_float2(add, add));
+              if (i == 1 || i == 4 || i == 6)  // the exponential unit's share and the fma pipe's take equally long
+                e = ex2_poly(e);
+              else
+                e.x = ex2(e.x), e.y = ex2(e.y);
+              part = __fadd2_rn(part, e);
+              p[i] = pack_f16x2(e.x, e.y);
+            }
+            return part.x + part.y;
+          };
+          if (edge) {
+#pragma unroll 1
+            for (int g = 0; g < 8; ++g) {
+              tmem_wait_ld();
+              const float4 of = lds_f4(meta_at + 16 * g);
+              float all = 0.f;
+              uint32_t p[8];
 #pragma unroll
-            for (int gg = 0; gg < 2; ++gg) {
-              const int g = 2 * h + gg;
-              const float c = meta.ks[g] * f, add = meta.lv[g] - m;
-              float w[16], sum = 0.f;
-#pragma unroll
-              for (int i = 0; i < 16; ++i) w[i] = ex2(fmaf(s[16 * g + i], c, add));
-              if (edge) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) w[i] = s[16 * g + i] == -INFINITY ? 0.f : w[i];
+              for (int i = 0; i < 8; ++i) {  // scales may be zero or NaN where nothing is seen
+                const float y = x[0][2 * i], z = x[0][2 * i + 1];
+                const float e = y == -INFINITY ? 0.f : ex2(fmaf(y, of.x * f, of.y - m)), h = z == -INFINITY ? 0.f : ex2(fmaf(z, of.x * f, of.y - m));
+                all += e + h;
+                p[i] = pack_f16x2(e, h);
               }
-#pragma unroll
-              for (int i = 0; i < 16; ++i) sum += w[i];
-              l += sum == 0.f ? 0.f : sum * meta.up[g];  // the scale of keys that are not seen may be NaN
-#pragma unroll
-              for (int i = 0; i < 8; ++i) p[8 * gg + i] = pack_f16x2(w[2 * i], w[2 * i + 1]);
+              l += all == 0.f ? 0.f : all * of.z;
+              if (g < 7) tmem_ld_x16(s_at + 16 * (g + 1), x[0]);
+              tmem_st_x8u(s_at + 8 * g, p);  // over logits that have been read
+              if (g == 3) weighed(kPHalf);
             }
-            tmem_st_x16u(s_at + 16 * h, p);
+          } else {
+#pragma unroll 1
+            for (int h = 0; h < 4; ++h) {
+              uint32_t p[16];
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                tmem_wait_ld();
+                if (i == 0 || h < 3) tmem_ld_x16(s_at + 16 * (2 * h + i + 1), x[i ^ 1]);
+                const float4 of = lds_f4(meta_at + 16 * (2 * h + i));
+                l += weigh(x[i], of, p + 8 * i) * of.z;
+              }
+              tmem_st_x16u(s_at + 16 * h, p);
+              if (h == 1) weighed(kPHalf);
+            }
           }
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bars + 8 * (kPFull + t));
+          weighed(kPFull);
         }
         if (!lost) (void)warp_wait(kODone + t, segs);
         lost = __any_sync(0xffffffffu, lost);
@@ -357,8 +457,11 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
       if (lost) break;
       // ---- the segment's outputs ----
       if (128 * t < u.rows) {
+        const bool live = flat < u.rows;
+        const int tok = (u.r0 + flat) / a.group, hd = walk.head * a.group + (u.r0 + flat) - tok * a.group;
+        const int64_t dense = (int64_t)u.row0 + tok;
         const float scale = big * 0x1p-6f;
-        float* const part = a.parts + ((int64_t)blockIdx.x * 2 + (walk.cut_front ? 0 : 1)) * (DH + 2) * kAtRows + flat;
+        float* const part = a.parts + ((int64_t)blockIdx.x * 2 + (walk.from > 0 ? 0 : 1)) * (DH + 2) * kAtRows + flat;
         const float per = l == 0.f ? 0.f : scale / l;
         tc_fence_after();
 #pragma unroll 1
@@ -385,18 +488,21 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
         tc_fence_before();
       }
     }
-  } else if (warp < 12) {
-    // ---------------------------------------------------------------- codes to operands
-    regs_down<104>();
+  } else if (warp < kAtProducts) {
+    // ---------------------------------------------------------------- codes to operands: four warps for keys, four for values
+    regs_down<kAtRegsCodes>();
     constexpr int NL = DH / 16, TPL = 512 / DH;  // loads of a lane; tokens of a load
-    const int w = warp - 8;
+    const bool values = warp >= 12;
+    const int w = warp & 3;
     // a quarter warp stores 16-byte chunks of two rows that differ in the swizzle's last bit: no bank twice
     const int ts = DH == 128 ? ((lane >> 2) & 1) + 2 * (lane >> 4) : lane >> 2;
     const int ch = DH == 128 ? (lane & 3) + 4 * ((lane >> 3) & 1) : lane & 3;
     const int shift = 31 - __clz(a.c.page_size);
+    const uint8_t* const codes = reinterpret_cast<const uint8_t*>(values ? a.c.v_codes : a.c.k_codes) + ts * DH + 16 * ch;
+    const int full = values ? kVFull : kKFull, free = values ? kVFree : kKFree;
+    const uint32_t to = base + (values ? L::kV : L::kK);
     uint32_t n = 0;  // key tiles of the worker
-    while (!lost && walk.next(a, prefix)) {
-      const AtItem& u = walk.u;
+    while (!lost && next_segment()) {
       const int limit = max(u.lim[0], u.lim[1]), key_begin = (u.kt0 + walk.from) * kAtKeys;
       const int32_t* table = a.c.block_table + (int64_t)u.b * a.c.max_blocks;
       // lanes 0 .. 7 look after a tile's eight groups of 16 keys
@@ -412,50 +518,146 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
         }
         return page;
       };
-      uint4 kr[NL], vr[NL];
-      auto load = [&](uint4 (&r)[NL], const void* codes, int k, int page) {
-        const int at_row = page >= 0 ? ((page * a.c.Hkv + walk.head) << shift) + ((key_begin + k * kAtKeys + 16 * (lane & 7)) & (a.c.page_size - 1)) : -1;
+      // Every load is made, from a row that exists: a load that may be skipped ends in a copy that waits for it.
+      uint4 raw[NL];
+      auto load = [&](int k, int page) {
+        const int at_row = page >= 0 ? ((page * a.c.Hkv + walk.head) << shift) + ((key_begin + k * kAtKeys + 16 * (lane & 7)) & (a.c.page_size - 1)) : 0;
+        const uint8_t* const at[2] = {codes + (int64_t)__shfl_sync(0xffffffffu, at_row, 2 * w) * DH,
+                                      codes + (int64_t)__shfl_sync(0xffffffffu, at_row, 2 * w + 1) * DH};
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-          const int in = TPL * i + ts;  // of this warp's 32 tokens
-          const int r0 = __shfl_sync(0xffffffffu, at_row, 2 * w + (TPL * i) / 16);
-          r[i] = make_uint4(0, 0, 0, 0);  // rows behind the last key may hold anything
-          if (r0 >= 0 && key_begin + k * kAtKeys + 32 * w + in < limit) {
-            const float4 v = ldg_stream_f4(reinterpret_cast<const uint8_t*>(codes) + (int64_t)(r0 + (in & 15)) * DH + 16 * ch);
-            r[i] = make_uint4(__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w));
-          }
+          const float4 v = ldg_stream_f4(at[TPL * i / 16] + (TPL * i & 15) * DH);
+          raw[i] = make_uint4(__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w));
         }
       };
-      auto store = [&](const uint4 (&r)[NL], uint32_t at) {
+      int page = checked(page_of(0)), next_page = page_of(1);
+      load(0, page);
+      for (int k = 0; k < walk.count; ++k, ++n) {
+        const uint32_t st = n & 1;
+        const int now = page;
+        if (n >= 2 && !warp_wait(free + st, (n >> 1) - 1)) break;
+        const int there = limit - (key_begin + k * kAtKeys + 32 * w);
+        if (there < 32 || __any_sync(0xffffffffu, now < 0)) {  // rows behind the last key, or of no page, may be any bytes
+#pragma unroll
+          for (int i = 0; i < NL; ++i) {
+            const int its = __shfl_sync(0xffffffffu, now, 2 * w + (TPL * i) / 16);
+            if (TPL * i + ts >= there || its < 0) raw[i] = make_uint4(0, 0, 0, 0);
+          }
+        }
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-          const uint32_t c[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+          const uint32_t c[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
           uint32_t h[8];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) codes_to_f16<I8>(c[k], h[2 * k], h[2 * k + 1]);
+          for (int q = 0; q < 4; ++q) codes_to_f16<I8>(c[q], h[2 * q], h[2 * q + 1]);
+          const uint32_t place = to + st * L::kOperand;
           const int t = 32 * w + TPL * i + ts;
-          sts_u4(at + operand_at(t, 2 * ch), h[0], h[1], h[2], h[3]);
-          sts_u4(at + operand_at(t, 2 * ch + 1), h[4], h[5], h[6], h[7]);
+          sts_u4(place + operand_at(t, 2 * ch), h[0], h[1], h[2], h[3]);
+          sts_u4(place + operand_at(t, 2 * ch + 1), h[4], h[5], h[6], h[7]);
         }
         fence_async_smem();
         __syncwarp();
+        if (lane == 0) mbar_arrive(bars + 8 * (full + st));
+        // the next tile's codes are asked for as soon as their registers are free
+        page = checked(next_page);
+        next_page = page_of(k + 2);
+        if (k + 1 < walk.count) load(k + 1, page);
+      }
+      lost = __any_sync(0xffffffffu, lost);
+    }
+  } else {
+    regs_down<kAtRegsRest>();
+    if (warp == kAtProducts) {
+      // -------------------------------------------------------------- products
+      constexpr uint32_t kIdescS = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+      constexpr uint32_t kIdescO = (1u << 4) | (((uint32_t)DH >> 3) << 17) | ((128u >> 4) << 24) | (1u << 16);
+      // descriptors: what is constant above the address bits, and addresses in units of 16 bytes
+      const uint64_t rows_of_64 = smem_desc(0, 0, 1024, 2), values_of = smem_desc(0, DH == 128 ? L::kSlab : 0, 1024, 2);
+      const uint32_t unit = base >> 4;
+      uint32_t n = 0, p_phase = 0, q_phase = 0;  // bit t: the phase that row tile t's barrier is in
+      auto phase_wait = [&](int bar, uint32_t& phases, int t) {
+        const bool ok = wait(bar + t, phases >> t);
+        phases ^= 1u << t;
+        return ok;
       };
-      float big = 0.f;
-      int page = checked(page_of(0)), next_page = page_of(1);
-      load(kr, a.c.k_codes, 0, page);
-      for (int k = 0; k < walk.count; ++k, ++n) {
-        const uint32_t st = n & 1;
-        load(vr, a.c.v_codes, k, page);
-        float ks = 0.f, vs = 0.f;
-        if (w == 0 && page >= 0) {
-          ks = a.c.k_scale[page * a.c.Hkv + walk.head];
-          vs = a.c.v_scale[page * a.c.Hkv + walk.head];
+      bool issued = false;
+      if (lane == 0) {  // one thread waits and issues
+        while (!lost && walk.next(a)) {
+          const int count = walk.count;
+#pragma unroll 1
+          for (int t = 0; t < 2; ++t)
+            if (walk.cnt[t] > 0 && !phase_wait(kQFull, q_phase, t)) break;
+#pragma unroll 1
+          for (int k = 0; k <= count && !lost; ++k) {
+            const uint32_t st = (n + k) & 1, before = st ^ 1;
+            if (k < count && !wait(kKFull + st, (n + k) >> 1)) break;
+            if (k > 0 && !wait(kVFull + before, (n + k - 1) >> 1)) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int t = 0; t < 2; ++t) {
+              const int cnt = walk.cnt[t];
+              if (k > 0 && k <= cnt) {
+                const uint64_t v_desc = values_of | (unit + ((L::kV + before * L::kOperand) >> 4));
+                if (!wait(kPHalf + t, p_phase >> t)) break;
+                tc_fence_after();
+#pragma unroll
+                for (int i = 0; i < kAtKeys / 32; ++i)
+                  mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * i, v_desc + (uint64_t)((i * 2048) >> 4), kIdescO, k > 1 || i > 0);
+                if (!phase_wait(kPFull, p_phase, t)) break;
+                tc_fence_after();
+#pragma unroll
+                for (int i = kAtKeys / 32; i < kAtKeys / 16; ++i)
+                  mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * i, v_desc + (uint64_t)((i * 2048) >> 4), kIdescO, true);
+                if (k == cnt) mma_commit(bars + 8 * (kODone + t));
+              }
+              if (k < cnt) {
+                const uint64_t q_desc = rows_of_64 | (unit + ((L::kQ + t * L::kOperand) >> 4));
+                const uint64_t k_desc = rows_of_64 | (unit + ((L::kK + st * L::kOperand) >> 4));
+#pragma unroll
+                for (int i = 0; i < DH / 16; ++i) {
+                  const uint64_t step = (uint64_t)(((i >> 2) * L::kSlab + (i & 3) * 32) >> 4);
+                  mma_ss(tmem + t * 128, q_desc + step, k_desc + step, kIdescS, i > 0);
+                }
+                mma_commit(bars + 8 * (kSFull + t));
+                issued = true;
+              }
+            }
+            if (!lost) {
+              if (k < count) mma_commit(bars + 8 * (kKFree + st));
+              if (k > 0) mma_commit(bars + 8 * (kVFree + before));
+            }
+          }
+          n += count;
         }
-        if (n >= 2 && !warp_wait(kKFree + st, (n >> 1) - 1)) break;
-        store(kr, base + L::kK + st * L::kOperand);
-        if (lane == 0) mbar_arrive(bars + 8 * (kKFull + st));
-        if (w == 0) {  // the tile's scales
-          float top = vs < INFINITY ? vs : 0.f;  // rows that do not see a page without a scale keep theirs
+        if (issued) {  // nothing may be on its way when tensor and shared memory are given back
+          mma_commit(bars + 8 * kLast);
+          (void)mbar_wait(bars + 8 * kLast, 0);
+        }
+      }
+      __syncwarp();
+    } else if (warp == kAtProducts + 1) {
+      // -------------------------------------------------------------- scales of the key tiles, for the softmax
+      const int shift = 31 - __clz(a.c.page_size);
+      uint32_t n = 0;
+      while (!lost && next_segment()) {
+          const int limit = max(u.lim[0], u.lim[1]), key_begin = (u.kt0 + walk.from) * kAtKeys + 16 * (lane & 7);
+        const int32_t* table = a.c.block_table + (int64_t)u.b * a.c.max_blocks;
+        auto page_of = [&](int k) {
+          const int t0 = key_begin + k * kAtKeys;
+          return k < walk.count && t0 < limit ? table[t0 >> shift] : -2;
+        };
+        auto scale_of = [&](const float* scales, int page) {
+          return page >= 0 && page < a.c.n_pages ? scales[page * a.c.Hkv + walk.head] : 0.f;
+        };
+        int page = page_of(0), next_page = page_of(1);
+        float big = 0.f, ks = scale_of(a.c.k_scale, page), vs = scale_of(a.c.v_scale, page);
+        for (int k = 0; k < walk.count; ++k, ++n) {
+          const unsigned bad = __ballot_sync(0xffffffffu, page != -2 && (page < 0 || page >= a.c.n_pages)) & 0xffu;
+          const float ks_now = ks, vs_now = vs;
+          page = next_page;
+          next_page = page_of(k + 2);
+          ks = scale_of(a.c.k_scale, page), vs = scale_of(a.c.v_scale, page);
+          float top = vs_now < INFINITY ? vs_now : 0.f;  // rows that do not see a page without a scale keep theirs
 #pragma unroll
           for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
           float down = 1.f;
@@ -464,95 +666,24 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
             down = big > 0.f ? big / b : 0.f;
             big = b;
           }
-          const unsigned bad = __ballot_sync(0xffffffffu, page == -1) & 0xffu;
           // pages of zeros have scale 0: any other value serves
-          const float ref = big > 0.f ? big : 1.f, v = vs == 0.f ? 1.f : vs * (1.f / ref);
+          const float ref = big > 0.f ? big : 1.f, v = vs_now == 0.f ? 1.f : vs_now * (1.f / ref);
+          // as far ahead as keys may be: the softmax has left tile n - 3 behind, and this place held n - 4
+          if (n >= 2 && !warp_wait(kKFree + (n & 1), (n >> 1) - 1)) break;
           AtMeta& mt = metas[n & 3];
-          if (lane < 8) {
-            mt.ks[lane] = ks;
-            mt.lv[lane] = log2f(v) + kAtWeight;
-            mt.up[lane] = 0x1p-6f / v;
-          }
+          if (lane < 8) mt.of[lane] = make_float4(ks_now, log2f(v) + kAtWeight, 0x1p-6f / v, 0.f);
           if (lane == 0) mt.down = k == 0 ? 1.f : down, mt.big = ref, mt.bad = bad;
           __syncwarp();
           if (lane == 0) mbar_arrive(bars + 8 * (kMFull + (n & 3)));
         }
-        page = checked(next_page);
-        next_page = page_of(k + 2);
-        if (k + 1 < walk.count) load(kr, a.c.k_codes, k + 1, page);
-        if (n >= 2 && !warp_wait(kVFree + st, (n >> 1) - 1)) break;
-        store(vr, base + L::kV + st * L::kOperand);
-        if (lane == 0) mbar_arrive(bars + 8 * (kVFull + st));
-      }
-      lost = __any_sync(0xffffffffu, lost);
-    }
-  } else {
-    regs_down<56>();
-    if (warp == 12) {
-      // -------------------------------------------------------------- products
-      constexpr uint32_t kIdescS = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
-      constexpr uint32_t kIdescO = (1u << 4) | (((uint32_t)DH >> 3) << 17) | ((128u >> 4) << 24) | (1u << 16);
-      uint32_t n = 0, p_taken[2] = {0, 0}, q_taken[2] = {0, 0};
-      bool issued = false;
-      while (!lost && walk.next(a, prefix)) {
-        const int count = walk.count;
-        bool ok = true;
-        for (int t = 0; t < 2 && ok; ++t)
-          if (walk.cnt[t] > 0) ok = warp_wait(kQFull + t, q_taken[t]++);
-        for (int k = 0; k <= count && ok; ++k) {
-          const uint32_t st = (n + k) & 1, before = (n + k - 1) & 1;
-          if (k < count) ok = warp_wait(kKFull + st, (n + k) >> 1);
-          if (ok && k > 0) ok = warp_wait(kVFull + before, (n + k - 1) >> 1);
-          for (int t = 0; t < 2 && ok; ++t) {
-            if (k > 0 && k - 1 < walk.cnt[t]) {
-              ok = warp_wait(kPFull + t, p_taken[t]++);
-              if (!ok) break;
-              tc_fence_after();
-              if (elect_one()) {
-                const uint64_t v_desc = smem_desc(base + L::kV + before * L::kOperand, DH == 128 ? L::kSlab : 0, 1024, 2);
-#pragma unroll
-                for (int i = 0; i < kAtKeys / 16; ++i)
-                  mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * i, v_desc + (uint64_t)((i * 2048) >> 4), kIdescO, k > 1 || i > 0);
-                if (k == walk.cnt[t]) mma_commit(bars + 8 * (kODone + t));
-              }
-              __syncwarp();
-            }
-            if (k < walk.cnt[t]) {
-              tc_fence_after();
-              if (elect_one()) {
-                const uint64_t q_desc = smem_desc(base + L::kQ + t * L::kOperand, 0, 1024, 2);
-                const uint64_t k_desc = smem_desc(base + L::kK + st * L::kOperand, 0, 1024, 2);
-#pragma unroll
-                for (int i = 0; i < DH / 16; ++i) {
-                  const uint64_t step = (uint64_t)(((i >> 2) * L::kSlab + (i & 3) * 32) >> 4);
-                  mma_ss(tmem + t * 128, q_desc + step, k_desc + step, kIdescS, i > 0);
-                }
-                mma_commit(bars + 8 * (kSFull + t));
-              }
-              __syncwarp();
-              issued = true;
-            }
-          }
-          if (ok && elect_one()) {
-            if (k < count) mma_commit(bars + 8 * (kKFree + st));
-            if (k > 0) mma_commit(bars + 8 * (kVFree + before));
-          }
-          __syncwarp();
-        }
         lost = __any_sync(0xffffffffu, lost);
-        n += count;
-      }
-      if (issued) {  // nothing may be on its way when tensor and shared memory are given back
-        if (elect_one()) mma_commit(bars + 8 * kLast);
-        __syncwarp();
-        (void)mbar_wait(bars + 8 * kLast, 0);
       }
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_dealloc(tmem, 512);
+  if (warp == kAtProducts) tmem_dealloc(tmem, 512);
 }
 
 // CTA (w, y): the block that worker w begins and others go on with, dims 16 y .. of it; and rows of blocks without keys.
@@ -617,6 +748,12 @@ static int launch_at(const AtArgs& a, cudaStream_t st) {
   static SmemOptIn opt_in;
   auto kern = blocks_attend_kernel<DH, I8>;
   if (int rc = ensure_dynamic_smem(opt_in, (const void*)kern, At<DH>::kSmem, "blocks_attend")) return rc;
+  // a launch with fewer registers could not hand out what the softmax asks for, and would wait for them
+  static const int regs = [&] {
+    cudaFuncAttributes f;
+    return cudaFuncGetAttributes(&f, (const void*)kern) == cudaSuccess ? f.numRegs : -1;
+  }();
+  SPHKV_REQUIRE(regs == kAtRegs, SPHKV_E_LIMIT, "blocks_attend: compiled for %d registers, needs %d", regs, kAtRegs);
   (void)launch_overlapped(kern, dim3(a.workers), dim3(kAtThreads), At<DH>::kSmem, st, a);
   return check_launch("blocks_attend_kernel");
 }
