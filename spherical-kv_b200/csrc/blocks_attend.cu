@@ -27,7 +27,7 @@ constexpr int kAtThreads = 640;  // warps 0-3, 4-7: softmax of tile 0, 1; 8-11, 
 constexpr int kAtProducts = 16;
 // Registers of a thread: at launch; after the softmax has taken what the others gave up.  The file is four quarters, with
 // five warps each (two of softmax, two of codes, one of 16 .. 19), so what goes up has to come down quarter by quarter.
-constexpr int kAtRegs = 96, kAtRegsSoftmax = 120, kAtRegsCodes = 80, kAtRegsRest = 80;
+constexpr int kAtRegs = 96, kAtRegsSoftmax = 128, kAtRegsCodes = 80, kAtRegsRest = 64;
 static_assert(2 * kAtRegsSoftmax + 2 * kAtRegsCodes + kAtRegsRest <= 5 * kAtRegs && 20 * 32 * kAtRegs <= 65536, "registers");
 constexpr int kAtPlanned = 128;  // slots whose tile counts a CTA sums itself
 constexpr float kAtLazy = 8.f;
@@ -96,7 +96,7 @@ struct At {
   static constexpr int kSmem = kWalks + kAtThreads / 32 * kAtWalkBytes + 1024;
 };
 static_assert(At<128>::kSmem <= 232448, "shared memory of a CTA");
-enum { kKFull = 0, kKFree = 2, kVFull = 4, kVFree = 6, kMFull = 8, kQFull = 12, kSFull = 14, kPFull = 16, kODone = 18, kPHalf = 20, kLast = 22 };
+enum { kKFull = 0, kKFree = 2, kVFull = 4, kVFree = 6, kMFull = 8, kQFull = 12, kSFull = 14, kPFull = 16, kODone = 18, kLast = 20 };
 
 __device__ __forceinline__ void tmem_ld_x32(uint32_t addr, float* v) {
   asm volatile(
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
       mbar_init(bars + 8 * (kKFull + i), 4), mbar_init(bars + 8 * (kKFree + i), 1);
       mbar_init(bars + 8 * (kVFull + i), 4), mbar_init(bars + 8 * (kVFree + i), 1);
       mbar_init(bars + 8 * (kQFull + i), 4), mbar_init(bars + 8 * (kSFull + i), 1);
-      mbar_init(bars + 8 * (kPFull + i), 4), mbar_init(bars + 8 * (kPHalf + i), 4), mbar_init(bars + 8 * (kODone + i), 1);
+      mbar_init(bars + 8 * (kPFull + i), 4), mbar_init(bars + 8 * (kODone + i), 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(bars + 8 * (kMFull + i), 1);
     mbar_init(bars + 8 * kLast, 1);
@@ -324,10 +324,8 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
 
         for (int k = 0; k < cnt; ++k) {
           const uint32_t n = tile + k;
-          // in this order: logits are there only when the key tile is, so that the barrier of its scales is at this phase
-          // or the one before, even where this row tile has skipped some
+          // the products' warp saw the tile's scales before it asked for the logits
           if (!warp_wait(kSFull + t, taken)) break;
-          if (!warp_wait(kMFull + (n & 3), n >> 2)) break;
           ++taken;
           tc_fence_after();
           const uint32_t meta_at = base + L::kMeta + (n & 3) * (uint32_t)sizeof(AtMeta);  // read anew in every pass: kept, 32 registers would not be there for logits
@@ -337,49 +335,14 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
           big = tail.y;
           const uint32_t bad = __float_as_uint(tail.z);
           const bool edge = key0 < first || key0 + kAtKeys > least || bad != 0;  // the same for all rows of the tile
-          float mx = kNone;
-          auto highest = [&](const float* x, int g) {
-            float top = fmaxf(fmaxf(x[0], x[1]), x[2]);
-#pragma unroll
-            for (int i = 3; i < 15; i += 2) top = fmaxf(fmaxf(top, x[i]), x[i + 1]);
-            mx = fmaxf(mx, fmaxf(top, x[15]) * (lds_f4(meta_at + 16 * g).x * f));
-          };
-          if (edge) {  // logits of keys that are not seen become -inf, in place
-#pragma unroll 1
-            for (int g = 0; g < 8; ++g) {
-              float x[16];
-              tmem_ld_x16(s_at + 16 * g, x);
-              tmem_wait_ld();
-#pragma unroll
-              for (int c = 0; c < 16; ++c)
-                if (key0 + 16 * g + c < first || key0 + 16 * g + c >= lim || ((bad >> g) & 1)) x[c] = -INFINITY;
-              highest(x, g);
-              tmem_st_x16(s_at + 16 * g, x);
-            }
-            tmem_wait_st();
-          } else {
-            // loops that stay loops: with all 128 keys in sight the compiler starts more than it has registers for
-            float s[2][32];
-            tmem_ld_x32(s_at, s[0]);
-#pragma unroll 1
-            for (int h = 0; h < 4; h += 2) {
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                tmem_wait_ld();
-                if (i == 0 || h == 0) tmem_ld_x32(s_at + 32 * (h + i + 1), s[i ^ 1]);
-                highest(s[i], 2 * (h + i));
-                highest(s[i] + 16, 2 * (h + i) + 1);
-              }
-            }
-          }
-          float x[2][16];
-          tmem_ld_x16(s_at, x[0]);
-          if (__any_sync(0xffffffffu, mx > m + kAtLazy) || down != 1.f) {
-            const float to = mx > m + kAtLazy ? mx : m, d = ex2(m - to);
+          // The row's reference moves to `to` in front of 32 keys: sums, outputs (with `down`: the value scales' reference) and
+          // the weights of the tile's keys before them follow.
+          auto move = [&](float to, float by, int done) {
+            const float d = ex2(m - to);
             m = to;
             l *= d;
             if (k > 0) {  // O holds something
-              const float r = d * down;
+              const float r = d * by;
 #pragma unroll 1
               for (int i = 0; i < DH / 16; ++i) {
                 float o[16];
@@ -390,64 +353,105 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
                 tmem_st_x16(o_at + 16 * i, o);
               }
             }
-          }
-          auto weighed = [&](int bar) {  // the weights of half the keys, or of all, are in tensor memory
+            const uint32_t dd = pack_f16x2(d, d);
             tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bars + 8 * (bar + t));
-          };
-          // weights of 16 keys; returns their sum
-          auto weigh = [&](const float* v, const float4& of, uint32_t* p) {
-            const float c = of.x * f, add = of.y - m;
-            float2 part = make_float2(0.f, 0.f);
+#pragma unroll 1
+            for (int h = 0; h < done; ++h) {
+              float w[16];
+              tmem_ld_x16(s_at + 16 * h, w);
+              tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              float2 e = __ffma2_rn(make_float2(v[2 * i], v[2 * i + 1]), make_float2(c, c), make_float2(add, add));
-              if (i == 1 || i == 4 || i == 6)  // the exponential unit's share and the fma pipe's take equally long
-                e = ex2_poly(e);
-              else
-                e.x = ex2(e.x), e.y = ex2(e.y);
-              part = __fadd2_rn(part, e);
-              p[i] = pack_f16x2(e.x, e.y);
+              for (int c = 0; c < 16; ++c) {
+                const uint32_t v = __float_as_uint(w[c]);
+                const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&dd));
+                w[c] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&r));
+              }
+              tmem_st_x16(s_at + 16 * h, w);
             }
-            return part.x + part.y;
           };
+          if (down != 1.f) move(m, down, 0);
           if (edge) {
 #pragma unroll 1
             for (int g = 0; g < 8; ++g) {
+              float v[16];
+              tmem_ld_x16(s_at + 16 * g, v);
               tmem_wait_ld();
               const float4 of = lds_f4(meta_at + 16 * g);
+              float top = -INFINITY;
+#pragma unroll
+              for (int c = 0; c < 16; ++c) {
+                if (key0 + 16 * g + c < first || key0 + 16 * g + c >= lim || ((bad >> g) & 1)) v[c] = -INFINITY;
+                top = fmaxf(top, v[c]);
+              }
+              top *= of.x * f;
+              const bool up = top > m + kAtLazy;
+              // 16 keys are half of what move() counts in: an odd group's first half has not been stored yet
+              if (__any_sync(0xffffffffu, up)) move(up ? top : m, 1.f, (g + 1) >> 1);
               float all = 0.f;
               uint32_t p[8];
 #pragma unroll
               for (int i = 0; i < 8; ++i) {  // scales may be zero or NaN where nothing is seen
-                const float y = x[0][2 * i], z = x[0][2 * i + 1];
+                const float y = v[2 * i], z = v[2 * i + 1];
                 const float e = y == -INFINITY ? 0.f : ex2(fmaf(y, of.x * f, of.y - m)), h = z == -INFINITY ? 0.f : ex2(fmaf(z, of.x * f, of.y - m));
                 all += e + h;
                 p[i] = pack_f16x2(e, h);
               }
               l += all == 0.f ? 0.f : all * of.z;
-              if (g < 7) tmem_ld_x16(s_at + 16 * (g + 1), x[0]);
               tmem_st_x8u(s_at + 8 * g, p);  // over logits that have been read
-              if (g == 3) weighed(kPHalf);
+              tmem_wait_st();
             }
           } else {
+            // 32 keys at a time, in a loop that stays one: with all 128 in sight the compiler starts more than it has registers
+            // for.  The next 32 travel while the exponentials are taken.
+            float x[32];
+            tmem_ld_x32(s_at, x);
 #pragma unroll 1
             for (int h = 0; h < 4; ++h) {
+              float2 e[16], part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
               uint32_t p[16];
+              const float4 of[2] = {lds_f4(meta_at + 32 * h), lds_f4(meta_at + 32 * h + 16)};
+              const float c[2] = {of[0].x * f, of[1].x * f};
+              tmem_wait_ld();
+              float top[2];
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                tmem_wait_ld();
-                if (i == 0 || h < 3) tmem_ld_x16(s_at + 16 * (2 * h + i + 1), x[i ^ 1]);
-                const float4 of = lds_f4(meta_at + 16 * (2 * h + i));
-                l += weigh(x[i], of, p + 8 * i) * of.z;
+              for (int gg = 0; gg < 2; ++gg) {
+                const float* const v = x + 16 * gg;
+                top[gg] = fmaxf(fmaxf(v[0], v[1]), v[2]);
+                float odd = fmaxf(fmaxf(v[3], v[4]), v[5]);
+#pragma unroll
+                for (int i = 6; i < 14; i += 4) top[gg] = fmaxf(fmaxf(top[gg], v[i]), v[i + 1]), odd = fmaxf(fmaxf(odd, v[i + 2]), v[i + 3]);
+                top[gg] = fmaxf(fmaxf(fmaxf(top[gg], v[14]), v[15]), odd) * c[gg];
               }
-              tmem_st_x16u(s_at + 16 * h, p);
-              if (h == 1) weighed(kPHalf);
+              const float mx = fmaxf(top[0], top[1]);
+              const bool up = mx > m + kAtLazy;
+              if (__any_sync(0xffffffffu, up)) move(up ? mx : m, 1.f, h);
+#pragma unroll
+              for (int gg = 0; gg < 2; ++gg) {
+                const float add = of[gg].y - m;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  e[8 * gg + i] = __ffma2_rn(make_float2(x[16 * gg + 2 * i], x[16 * gg + 2 * i + 1]), make_float2(c[gg], c[gg]), make_float2(add, add));
+              }
+              if (h < 3) tmem_ld_x32(s_at + 32 * (h + 1), x);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                if ((i & 3) == 1)  // a quarter: 64 keys take a warp 535 cycles instead of 622, three or four of eight no less
+                  e[i] = ex2_poly(e[i]);
+                else
+                  e[i].x = ex2(e[i].x), e[i].y = ex2(e[i].y);
+                part[i >> 3] = __fadd2_rn(part[i >> 3], e[i]);
+                p[i] = pack_f16x2(e[i].x, e[i].y);
+              }
+              l += (part[0].x + part[0].y) * of[0].z;
+              l += (part[1].x + part[1].y) * of[1].z;
+              tmem_wait_ld();
+              tmem_st_x16u(s_at + 16 * h, p);  // over logits that have been read
             }
           }
-          weighed(kPFull);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bars + 8 * (kPFull + t));
         }
         if (!lost) (void)warp_wait(kODone + t, segs);
         lost = __any_sync(0xffffffffu, lost);
@@ -576,41 +580,41 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
       const uint32_t unit = base >> 4;
       uint32_t n = 0, p_phase = 0, q_phase = 0;  // bit t: the phase that row tile t's barrier is in
       auto phase_wait = [&](int bar, uint32_t& phases, int t) {
-        const bool ok = wait(bar + t, phases >> t);
+        const bool ok = warp_wait(bar + t, phases >> t);
         phases ^= 1u << t;
         return ok;
       };
+      // the whole warp waits, one elected thread issues: under a condition on the lane the compiler does not see that it is one
       bool issued = false;
-      if (lane == 0) {  // one thread waits and issues
-        while (!lost && walk.next(a)) {
-          const int count = walk.count;
+      while (!lost && next_segment()) {
+        const int count = walk.count;
 #pragma unroll 1
-          for (int t = 0; t < 2; ++t)
-            if (walk.cnt[t] > 0 && !phase_wait(kQFull, q_phase, t)) break;
+        for (int t = 0; t < 2; ++t)
+          if (walk.cnt[t] > 0 && !phase_wait(kQFull, q_phase, t)) break;
 #pragma unroll 1
-          for (int k = 0; k <= count && !lost; ++k) {
-            const uint32_t st = (n + k) & 1, before = st ^ 1;
-            if (k < count && !wait(kKFull + st, (n + k) >> 1)) break;
-            if (k > 0 && !wait(kVFull + before, (n + k - 1) >> 1)) break;
-            tc_fence_after();
+        for (int k = 0; k <= count; ++k) {
+          const uint32_t st = (n + k) & 1, before = st ^ 1;
+          if (k < count && !(warp_wait(kKFull + st, (n + k) >> 1) && warp_wait(kMFull + ((n + k) & 3), (n + k) >> 2))) break;
+          if (k > 0 && !warp_wait(kVFull + before, (n + k - 1) >> 1)) break;
+          bool ok = true;
 #pragma unroll 1
-            for (int t = 0; t < 2; ++t) {
-              const int cnt = walk.cnt[t];
-              if (k > 0 && k <= cnt) {
+          for (int t = 0; t < 2; ++t) {
+            const int cnt = walk.cnt[t];
+            if (ok && k > 0 && k <= cnt) {
+              ok = phase_wait(kPFull, p_phase, t);
+              tc_fence_after();
+              if (ok && elect_one()) {
                 const uint64_t v_desc = values_of | (unit + ((L::kV + before * L::kOperand) >> 4));
-                if (!wait(kPHalf + t, p_phase >> t)) break;
-                tc_fence_after();
 #pragma unroll
-                for (int i = 0; i < kAtKeys / 32; ++i)
+                for (int i = 0; i < kAtKeys / 16; ++i)
                   mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * i, v_desc + (uint64_t)((i * 2048) >> 4), kIdescO, k > 1 || i > 0);
-                if (!phase_wait(kPFull, p_phase, t)) break;
-                tc_fence_after();
-#pragma unroll
-                for (int i = kAtKeys / 32; i < kAtKeys / 16; ++i)
-                  mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * i, v_desc + (uint64_t)((i * 2048) >> 4), kIdescO, true);
                 if (k == cnt) mma_commit(bars + 8 * (kODone + t));
               }
-              if (k < cnt) {
+              __syncwarp();
+            }
+            if (ok && k < cnt) {
+              tc_fence_after();
+              if (elect_one()) {
                 const uint64_t q_desc = rows_of_64 | (unit + ((L::kQ + t * L::kOperand) >> 4));
                 const uint64_t k_desc = rows_of_64 | (unit + ((L::kK + st * L::kOperand) >> 4));
 #pragma unroll
@@ -619,22 +623,26 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
                   mma_ss(tmem + t * 128, q_desc + step, k_desc + step, kIdescS, i > 0);
                 }
                 mma_commit(bars + 8 * (kSFull + t));
-                issued = true;
               }
-            }
-            if (!lost) {
-              if (k < count) mma_commit(bars + 8 * (kKFree + st));
-              if (k > 0) mma_commit(bars + 8 * (kVFree + before));
+              __syncwarp();
+              issued = true;
             }
           }
-          n += count;
+          if (!ok) break;
+          if (elect_one()) {
+            if (k < count) mma_commit(bars + 8 * (kKFree + st));
+            if (k > 0) mma_commit(bars + 8 * (kVFree + before));
+          }
+          __syncwarp();
         }
-        if (issued) {  // nothing may be on its way when tensor and shared memory are given back
-          mma_commit(bars + 8 * kLast);
-          (void)mbar_wait(bars + 8 * kLast, 0);
-        }
+        lost = __any_sync(0xffffffffu, lost);
+        n += count;
       }
-      __syncwarp();
+      if (issued) {  // nothing may be on its way when tensor and shared memory are given back
+        if (elect_one()) mma_commit(bars + 8 * kLast);
+        __syncwarp();
+        (void)mbar_wait(bars + 8 * kLast, 0);
+      }
     } else if (warp == kAtProducts + 1) {
       // -------------------------------------------------------------- scales of the key tiles, for the softmax
       const int shift = 31 - __clz(a.c.page_size);
