@@ -84,15 +84,15 @@ __device__ __forceinline__ BlockPiece find_piece_alone(const sphkv_blocks& c, co
 }
 
 // ---- work dealt evenly: tiles of all slots and heads in one line ------------------------------------------------
-// prefix[s] = tiles of the slots before s, prefix[slots] = all; by one block.  tiles_of(s): tiles of slot s
+// prefix[s] = tiles of the slots before s, prefix[slots] = all; by one block, of up to any number of slots.
 template <typename F>
-__device__ __forceinline__ void sum_tiles(int slots, int64_t* prefix, F tiles_of) {
+__device__ __forceinline__ void sum_tiles(int slots, int64_t* prefix, F item) {
   __shared__ int64_t warp_sums[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int64_t before = 0;
   for (int s0 = 0; s0 < slots; s0 += blockDim.x) {
     const int s = s0 + tid;
-    int64_t v = s < slots ? tiles_of(s) : 0;
+    int64_t v = s < slots ? item(s).tiles : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t up = __shfl_up_sync(0xffffffffu, v, o);
@@ -109,6 +109,32 @@ __device__ __forceinline__ void sum_tiles(int slots, int64_t* prefix, F tiles_of
     __syncthreads();
   }
   if (tid == 0) prefix[0] = 0;
+}
+// The same for at most kDealt slots by the block's first warp, and the slots' items beside it: a block that shares in the work
+// begins with this, and one warp's shuffles take a third of what a block's barriers take.
+constexpr int kDealt = 128;
+template <typename Item, typename F>
+__device__ __forceinline__ void deal_tiles(int slots, int64_t* prefix, Item* items, F item) {
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    int64_t before = 0;
+    for (int s0 = 0; s0 < slots; s0 += 32) {
+      int64_t v = 0;
+      if (s0 + lane < slots) {
+        const Item u = item(s0 + lane);
+        items[s0 + lane] = u;
+        v = u.tiles;
+      }
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += up;
+      }
+      if (s0 + lane < slots) prefix[s0 + lane + 1] = before + v;
+      before += __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (lane == 0) prefix[0] = 0;
+  }
   __syncthreads();
 }
 __device__ __forceinline__ int slot_at(const int64_t* prefix, int slots, int64_t tile) {  // prefix[s] <= tile < prefix[s + 1]

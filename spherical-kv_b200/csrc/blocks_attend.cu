@@ -29,7 +29,6 @@ constexpr int kAtProducts = 16;
 // five warps each (two of softmax, two of codes, one of 16 .. 19), so what goes up has to come down quarter by quarter.
 constexpr int kAtRegs = 96, kAtRegsSoftmax = 128, kAtRegsCodes = 80, kAtRegsRest = 64;
 static_assert(2 * kAtRegsSoftmax + 2 * kAtRegsCodes + kAtRegsRest <= 5 * kAtRegs && 20 * 32 * kAtRegs <= 65536, "registers");
-constexpr int kAtPlanned = 128;  // slots whose tile counts a CTA sums itself
 constexpr float kAtLazy = 8.f;
 constexpr float kAtWeight = 6.f;  // log2: weights stay below 2^15 with the lazy maximum
 
@@ -73,7 +72,7 @@ __device__ __forceinline__ AtItem item_of(const AtArgs& a, int slot) {
 }
 __global__ void __launch_bounds__(1024) blocks_attend_plan_kernel(const __grid_constant__ AtArgs a, int64_t* prefix) {
   griddep_wait();
-  sum_tiles(a.slots, prefix, [&](int s) { return item_of(a, s).tiles; });
+  sum_tiles(a.slots, prefix, [&](int s) { return item_of(a, s); });
 }
 
 // ---- shared memory ----------------------------------------------------------------------------------------
@@ -92,7 +91,8 @@ struct At {
   static constexpr int kQ = 0, kK = 2 * kOperand, kV = kK + 2 * kOperand, kMeta = kV + 2 * kOperand;
   static constexpr int kBars = kMeta + 4 * (int)sizeof(AtMeta);
   static constexpr int kPrefix = kBars + 24 * 8;
-  static constexpr int kWalks = kPrefix + (kAtPlanned + 1) * 8;
+  static constexpr int kItems = kPrefix + (kDealt + 2) * 8;
+  static constexpr int kWalks = kItems + kDealt * (int)sizeof(AtItem);
   static constexpr int kSmem = kWalks + kAtThreads / 32 * kAtWalkBytes + 1024;
 };
 static_assert(At<128>::kSmem <= 232448, "shared memory of a CTA");
@@ -151,7 +151,7 @@ struct AtWalk {
   AtItem u;
   int slot, head, from, count, cnt[2];
   bool whole;
-  __device__ __forceinline__ void begin(const AtArgs& a, const int64_t* prefix, int64_t worker) {
+  __device__ __forceinline__ void begin(const AtArgs& a, const int64_t* prefix, const AtItem* items, int64_t worker) {
     const int64_t total = prefix[a.slots] * a.c.Hkv, workers = min((int64_t)a.workers, total);
     left = 0;
     count = 0;
@@ -159,19 +159,21 @@ struct AtWalk {
     const int64_t pos = worker * total / workers;
     left = (worker + 1) * total / workers - pos;
     slot = slot_at(prefix, a.slots, pos / a.c.Hkv);
-    u = item_of(a, slot);
+    u = items ? items[slot] : item_of(a, slot);
     const int64_t in_slot = pos - prefix[slot] * a.c.Hkv;
     head = (int)(in_slot / u.tiles);
     from = (int)(in_slot - (int64_t)head * u.tiles);
   }
-  __device__ __forceinline__ bool next(const AtArgs& a) {
+  __device__ __forceinline__ bool next(const AtArgs& a, const AtItem* items) {
     if (left == 0) return false;
     if (count > 0) {  // behind a segment: the next head, or the next block with keys
       from = 0;
       if (++head == a.c.Hkv) {
         head = 0;
-        do u = item_of(a, ++slot);
-        while (u.tiles == 0);  // there is one: left > 0
+        do {
+          ++slot;
+          u = items ? items[slot] : item_of(a, slot);
+        } while (u.tiles == 0);  // there is one: left > 0
       }
     }
     count = (int)min((int64_t)(u.tiles - from), left);
@@ -236,13 +238,14 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
   griddep_launch();
   griddep_wait();
   const int64_t* prefix = a.prefix;
+  const AtItem* const items = prefix == nullptr ? reinterpret_cast<const AtItem*>(smem + L::kItems) : nullptr;
   if (prefix == nullptr) {
-    sum_tiles(a.slots, prefix_smem, [&](int s) { return item_of(a, s).tiles; });
+    deal_tiles(a.slots, prefix_smem, reinterpret_cast<AtItem*>(smem + L::kItems), [&](int s) { return item_of(a, s); });
     prefix = prefix_smem;
   }
   AtWalk& walk = *reinterpret_cast<AtWalk*>(smem + L::kWalks + warp * kAtWalkBytes);
   const AtItem& u = walk.u;
-  if (lane == 0) walk.begin(a, prefix, blockIdx.x);
+  if (lane == 0) walk.begin(a, prefix, items, blockIdx.x);
   bool lost = false;
   auto wait = [&](int bar, uint32_t n) {  // the n-th phase, from 0
     if (!lost && !mbar_wait(bars + 8 * bar, n & 1)) {
@@ -254,7 +257,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
   auto warp_wait = [&](int bar, uint32_t n) { return __all_sync(0xffffffffu, wait(bar, n)); };
   auto next_segment = [&] {
     __syncwarp();
-    const int more = lane == 0 ? walk.next(a) : 0;
+    const int more = lane == 0 ? walk.next(a, items) : 0;
     return __shfl_sync(0xffffffffu, more, 0) != 0;  // and what lane 0 wrote is there for all
   };
 
@@ -696,12 +699,14 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
 
 // CTA (w, y): the block that worker w begins and others go on with, dims 16 y .. of it; and rows of blocks without keys.
 __global__ void __launch_bounds__(256) blocks_attend_merge_kernel(const __grid_constant__ AtArgs a, int dh) {
-  __shared__ int64_t prefix_smem[kAtPlanned + 1];
+  __shared__ int64_t prefix_smem[kDealt + 1];
+  __shared__ AtItem items[kDealt];
   griddep_launch();
   griddep_wait();
   const int64_t* prefix = a.prefix;
-  if (prefix == nullptr) {
-    sum_tiles(a.slots, prefix_smem, [&](int s) { return item_of(a, s).tiles; });
+  const bool dealt = prefix == nullptr;
+  if (dealt) {
+    deal_tiles(a.slots, prefix_smem, items, [&](int s) { return item_of(a, s); });
     prefix = prefix_smem;
   }
   const int64_t total = prefix[a.slots] * a.c.Hkv, workers = min((int64_t)a.workers, total);
@@ -709,7 +714,7 @@ __global__ void __launch_bounds__(256) blocks_attend_merge_kernel(const __grid_c
   float o[16];
   for (int s = w; s < a.slots; s += gridDim.x) {
     if (prefix[s + 1] != prefix[s]) continue;
-    const AtItem u = item_of(a, s);
+    const AtItem u = dealt ? items[s] : item_of(a, s);
     if (flat >= u.rows) continue;
 #pragma unroll
     for (int c = 0; c < 16; ++c) o[c] = 0.f;
@@ -719,7 +724,7 @@ __global__ void __launch_bounds__(256) blocks_attend_merge_kernel(const __grid_c
   if (w >= workers) return;
   const int64_t start = w * total / workers, stop = (w + 1) * total / workers;
   const int slot = slot_at(prefix, a.slots, (stop - 1) / a.c.Hkv);
-  const AtItem u = item_of(a, slot);
+  const AtItem u = dealt ? items[slot] : item_of(a, slot);
   const int64_t in_slot = stop - 1 - prefix[slot] * a.c.Hkv;
   const int head = (int)(in_slot / u.tiles);
   const int64_t p0 = prefix[slot] * a.c.Hkv + (int64_t)head * u.tiles, p1 = p0 + u.tiles - 1;
@@ -824,7 +829,7 @@ extern "C" int sphkv_blocks_attend(const sphkv_blocks* c, const void* q, int32_t
                 (long long)scratch_bytes, (long long)need);
   SPHKV_REQUIRE(((uintptr_t)scratch & 255) == 0, SPHKV_E_ALIGN, "blocks_attend: scratch needs 256 B");
   a.parts = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(scratch) + align256((at_slots(rows, c->B, group) + 1) * 8));
-  if (slots > kAtPlanned) {
+  if (slots > kDealt) {
     int64_t* prefix = reinterpret_cast<int64_t*>(scratch);
     (void)launch_overlapped(blocks_attend_plan_kernel, dim3(1), dim3(1024), 0, st, a, prefix);
     if (int rc = check_launch("blocks_attend_plan_kernel")) return rc;

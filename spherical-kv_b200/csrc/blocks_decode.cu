@@ -20,7 +20,6 @@
 namespace sphkv {
 
 constexpr int kBdWarps = 16, kBdThreads = 32 * kBdWarps;
-constexpr int kBdPlanned = 512;  // slots whose tile counts a CTA sums itself; more are summed by a launch before
 constexpr float kLazy = 8.f;     // a reference maximum moves when a logit passes it by 2^8
 constexpr float kWeight = 64.f;  // weights are 2^6 p v / S <= 2^14: f16 keeps 22 bits (hi + lo) of those above 2^-3
 
@@ -37,6 +36,7 @@ struct BdArgs {
   float* parts;           // [workers + units][8][dh + 2]
   int q_dtype, out_dtype, Hq, group, slots, tshift, workers;
   float scale_log2;       // sm_scale * log2 e
+  bool q_vec;             // rows of queries on 16-byte boundaries
 };
 
 template <int DH>
@@ -47,13 +47,14 @@ struct Bd {
   static constexpr int kGroupDims = DH / 8;                        // output dims of a lane
   static constexpr int kCol = 8 * (kGroupDims + 2) + 4;            // floats of an output row in shared memory: no bank twice
   static constexpr int kPrefixOff = kBdWarps * kRing;
-  static constexpr int kStatOff = kPrefixOff + (kBdPlanned + 1) * 8;
-  static constexpr int kStat = 3 * 8 + 8;                          // floats of a warp: maxima, sums, true maxima, S
-  static constexpr int kBarOff = kStatOff + kBdWarps * kStat * 4;
+  static constexpr int kItemsOff = kPrefixOff + (kDealt + 2) * 8;
+  static constexpr int kStatOff = kItemsOff + kDealt * 32;
+  static constexpr int kStat = 5 * 8;                              // floats of a warp: maxima, sums, true maxima, S (8 times), factors
+  static constexpr int kBarOff = kStatOff + kBdWarps * (kStat + 8 * 3) * 4;
   static constexpr int kSmem = kBarOff + kBdWarps * kStages * 8 + 1024;
 };
 static_assert(Bd<128>::kSmem <= 232448 && Bd<64>::kSmem <= 232448, "shared memory of a CTA");
-static_assert((kBdWarps / 2) * 8 * Bd<128>::kCol * 4 <= kBdWarps * Bd<128>::kRing, "outputs are joined in the rings' place");
+static_assert(8 * Bd<128>::kCol * 4 <= Bd<128>::kRing, "a warp's outputs are joined in its ring's place");
 
 // The keys of one unit's queries.
 struct BdUnit {
@@ -76,12 +77,11 @@ __device__ __forceinline__ BdUnit unit_of(const BdArgs& a, const BlockPiece& p) 
   return u;
 }
 
-__device__ __forceinline__ void sum_unit_tiles(const BdArgs& a, int64_t* prefix) {
-  sum_tiles(a.slots, prefix, [&](int s) { return unit_of(a, find_piece_alone(a.c, a.r, s, a.tshift, 1)).tiles; });
-}
+static_assert(sizeof(BdUnit) == 32, "a slot's place");
+__device__ __forceinline__ BdUnit unit_of_slot(const BdArgs& a, int s) { return unit_of(a, find_piece_alone(a.c, a.r, s, a.tshift, 1)); }
 __global__ void __launch_bounds__(1024) blocks_plan_kernel(const __grid_constant__ BdArgs a, int64_t* prefix) {
   griddep_wait();
-  sum_unit_tiles(a, prefix);
+  sum_tiles(a.slots, prefix, [&](int s) { return unit_of_slot(a, s); });
 }
 // the workers that share the tiles: none goes without, so that a unit's segments are those of consecutive workers
 __device__ __forceinline__ int64_t workers_of(const BdArgs& a, int64_t total) { return min((int64_t)a.workers, total); }
@@ -131,7 +131,9 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
   const uint32_t bars = smem_u32(smem) + L::kBarOff + warp * S * 8;
   int64_t* const prefix_smem = reinterpret_cast<int64_t*>(smem + L::kPrefixOff);
   float* const stats = reinterpret_cast<float*>(smem + L::kStatOff) + team * WARPS * L::kStat;  // of the team
-  float* const joined = reinterpret_cast<float*>(smem + team * WARPS * L::kRing);               // in its rings' place
+  float* const cols_of = reinterpret_cast<float*>(smem + L::kStatOff) + kBdWarps * L::kStat + team * WARPS * 24;  // max, sum, true max
+  float* const joined = reinterpret_cast<float*>(smem + team * WARPS * L::kRing);  // a warp's outputs: in its ring's place
+  constexpr int JOIN = L::kRing / 4;
   if (lane == 0) {
 #pragma unroll
     for (int s = 0; s < S; ++s) mbar_init(bars + 8 * s, 1);
@@ -141,8 +143,10 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
   griddep_launch();
   griddep_wait();
   const int64_t* prefix = a.prefix;
-  if (prefix == nullptr) {
-    sum_unit_tiles(a, prefix_smem);
+  BdUnit* const items = reinterpret_cast<BdUnit*>(smem + L::kItemsOff);
+  const bool dealt = prefix == nullptr;
+  if (dealt) {
+    deal_tiles(a.slots, prefix_smem, items, [&](int s) { return unit_of_slot(a, s); });
     prefix = prefix_smem;
   }
   const int64_t total = prefix[a.slots] * a.c.Hkv;
@@ -163,7 +167,7 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
   while (pos < stop) {
     // ---- the segment ----
     const int slot = slot_at(prefix, a.slots, pos / a.c.Hkv);
-    const BdUnit u = unit_of(a, find_piece_alone(a.c, a.r, slot, a.tshift, 1));
+    const BdUnit u = dealt ? items[slot] : unit_of_slot(a, slot);
     const int64_t in_slot = pos - prefix[slot] * a.c.Hkv;
     const int head = (int)(in_slot / u.tiles), from = (int)(in_slot - (int64_t)head * u.tiles);
     const int count = (int)min((int64_t)(u.tiles - from), stop - pos);
@@ -217,11 +221,36 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
       float v[DH / 4];
       float top = 0.f;
       const int tok = g / a.group, h = head * a.group + g - tok * a.group;
-      const bool there = g < cols;
-      const int64_t at = there ? (int64_t)(u.row0 + tok) * a.q_row_stride + (int64_t)h * a.q_head_stride + (DH / 4) * j : 0;
+      const bool there = g < cols;  // the others read row 0 of the unit, and are nothing
+      const int64_t at = (int64_t)(u.row0 + (there ? tok : 0)) * a.q_row_stride + (int64_t)(there ? h : head * a.group) * a.q_head_stride + (DH / 4) * j;
+      if (a.q_vec) {
+        constexpr int N = QLO ? DH / 16 : DH / 32;  // 16-byte loads, all on their way at once
+        uint4 raw[N];
+        const uint4* const from = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.q) + at * (QLO ? 4 : 2));
+#pragma unroll
+        for (int i = 0; i < N; ++i) raw[i] = from[i];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if constexpr (QLO) {
+              v[4 * i + q] = __uint_as_float(w[q]);
+            } else if (a.q_dtype == SPHKV_BF16) {
+              v[8 * i + 2 * q] = __uint_as_float(w[q] << 16), v[8 * i + 2 * q + 1] = __uint_as_float(w[q] & 0xffff0000u);
+            } else {
+              const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[q]));
+              v[8 * i + 2 * q] = x.x, v[8 * i + 2 * q + 1] = x.y;
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < DH / 4; ++i) v[i] = load_as_float(a.q, a.q_dtype, at + i);
+      }
 #pragma unroll
       for (int i = 0; i < DH / 4; ++i) {
-        v[i] = there ? load_as_float(a.q, a.q_dtype, at + i) : 0.f;
+        if (!there) v[i] = 0.f;
         top = fmaxf(top, fabsf(v[i]));
         if (isnan(v[i])) top = INFINITY;
       }
@@ -397,45 +426,43 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
         st[2 * j] = m0, st[2 * j + 1] = m1;
         st[8 + 2 * j] = l0, st[9 + 2 * j] = l1;
         st[16 + 2 * j] = t0, st[17 + 2 * j] = t1;
+        st[24 + 2 * j] = st[25 + 2 * j] = big;
       }
-      team_sync();  // every tile of the segment has been taken: the rings' place is free
-      float top0 = kNone, top1 = kNone;
-      for (int w = 0; w < WARPS; ++w) {
-        top0 = fmaxf(top0, stats[w * L::kStat + 2 * j]);
-        top1 = fmaxf(top1, stats[w * L::kStat + 2 * j + 1]);
-      }
-      const float r0 = ex2(m0 - top0) * (big / kWeight), r1 = ex2(m1 - top1) * (big / kWeight);
-      constexpr int HALF = WARPS > 1 ? WARPS / 2 : 1;
-      auto place = [&](int i, int col) { return reinterpret_cast<float2*>(joined + ((tw % HALF) * 8 + col) * L::kCol + g * (GD + 2) + 2 * i); };
-      if (tw < HALF) {
+      float* const mine_at = joined + tw * JOIN + g * (GD + 2);  // this warp has taken every tile of its own
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          *place(i, 2 * j) = make_float2(acc[i][0] * r0, acc[i][2] * r0);
-          *place(i, 2 * j + 1) = make_float2(acc[i][1] * r1, acc[i][3] * r1);
-        }
+      for (int i = 0; i < KS; ++i) {
+        *reinterpret_cast<float2*>(mine_at + 2 * j * L::kCol + 2 * i) = make_float2(acc[i][0], acc[i][2]);
+        *reinterpret_cast<float2*>(mine_at + (2 * j + 1) * L::kCol + 2 * i) = make_float2(acc[i][1], acc[i][3]);
       }
       team_sync();
-      if (tw >= HALF) {
+      const int n_warps = min(count, WARPS);
+      for (int col = tw; col < cols; col += WARPS) {  // a warp to a query row: lane w looks after warp w
+        const float* const of = stats + (lane % WARPS) * L::kStat + col;
+        const bool have = lane < n_warps;
+        float top = have ? of[0] : kNone, true_top = have ? of[16] : -INFINITY;
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          float2 p = *place(i, 2 * j);
-          *place(i, 2 * j) = make_float2(p.x + acc[i][0] * r0, p.y + acc[i][2] * r0);
-          p = *place(i, 2 * j + 1);
-          *place(i, 2 * j + 1) = make_float2(p.x + acc[i][1] * r1, p.y + acc[i][3] * r1);
+        for (int o = 1; o < 32; o <<= 1) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          true_top = fmaxf(true_top, __shfl_xor_sync(0xffffffffu, true_top, o));
         }
+        const float f = have ? ex2(of[0] - top) : 0.f;
+        float sum = have ? of[8] * f : 0.f;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (have) stats[lane * L::kStat + 32 + col] = f * (of[24] * (1.f / kWeight));
+        if (lane == 0) cols_of[3 * col] = top, cols_of[3 * col + 1] = sum, cols_of[3 * col + 2] = true_top;
       }
       team_sync();
       const bool whole = count == u.tiles;
       float* const part = a.parts + (int64_t)(worker + unit) * 8 * (DH + 2);
       for (int i = tw * 32 + lane; i < cols * DH; i += WARPS * 32) {
         const int col = i / DH, d = i - col * DH;
-        float top = kNone, true_top = -INFINITY, sum = 0.f, v = 0.f;
-        for (int w = 0; w < WARPS; ++w) {
-          top = fmaxf(top, stats[w * L::kStat + col]);
-          true_top = fmaxf(true_top, stats[w * L::kStat + 16 + col]);
-        }
-        for (int w = 0; w < WARPS; ++w) sum += stats[w * L::kStat + 8 + col] * ex2(stats[w * L::kStat + col] - top);
-        for (int w = 0; w < HALF; ++w) v += joined[(w * 8 + col) * L::kCol + (d / GD) * (GD + 2) + d % GD];
+        const float* const from = joined + col * L::kCol + (d / GD) * (GD + 2) + d % GD;
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w)
+          if (w < n_warps) v += from[w * JOIN] * stats[w * L::kStat + 32 + col];
+        const float top = cols_of[3 * col], sum = cols_of[3 * col + 1], true_top = cols_of[3 * col + 2];
         const float to_true = true_top == -INFINITY ? 0.f : ex2(top - true_top);
         if (whole) {
           const int tok = col / a.group, h = head * a.group + col - tok * a.group;
@@ -462,18 +489,22 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
 }
 
 // A block per unit: joins the segments of units that more than one worker had, and writes the rows of units without keys.
+constexpr int kBdParts = 32;  // segments whose maxima and sums are in shared memory at a time
 __global__ void __launch_bounds__(256) blocks_merge_kernel(const __grid_constant__ BdArgs a, int dh) {
-  __shared__ int64_t prefix_smem[kBdPlanned + 1];
+  __shared__ int64_t prefix_smem[kDealt + 1];
+  __shared__ BdUnit items[kDealt];
+  __shared__ float factor[kBdParts][8], sums[8];
   griddep_launch();
   griddep_wait();
   const int64_t* prefix = a.prefix;
-  if (prefix == nullptr) {
-    sum_unit_tiles(a, prefix_smem);
+  const bool dealt = prefix == nullptr;
+  if (dealt) {
+    deal_tiles(a.slots, prefix_smem, items, [&](int s) { return unit_of_slot(a, s); });
     prefix = prefix_smem;
   }
   const int unit = blockIdx.x, slot = unit / a.c.Hkv, head = unit - slot * a.c.Hkv;
   const int64_t total = prefix[a.slots] * a.c.Hkv;
-  const BdUnit u = unit_of(a, find_piece_alone(a.c, a.r, slot, a.tshift, 1));
+  const BdUnit u = dealt ? items[slot] : unit_of_slot(a, slot);
   if (u.tokens == 0) return;
   int64_t w0 = 0, w1 = -1;
   if (u.tiles > 0) {
@@ -483,25 +514,55 @@ __global__ void __launch_bounds__(256) blocks_merge_kernel(const __grid_constant
     w1 = ((p1 + 1) * workers - 1) / total;
     if (w0 == w1) return;
   }
-  for (int i = threadIdx.x; i < u.tokens * a.group * dh; i += blockDim.x) {
-    const int col = i / dh, d = i - col * dh;
-    float top = -INFINITY, sum = 0.f, v = 0.f;
-    const float* row = a.parts + ((w0 + unit) * 8 + col) * (dh + 2);
-    const int64_t step = (int64_t)8 * (dh + 2);
-    for (int64_t w = 0; w <= w1 - w0; ++w) top = fmaxf(top, row[w * step]);
-    for (int64_t w = 0; w <= w1 - w0; ++w) {
-      const float f = row[w * step] == -INFINITY ? 0.f : ex2(row[w * step] - top);
-      sum += row[w * step + 1] * f;
-      v += row[w * step + 2 + d] * f;
+  const int n = (int)(w1 - w0 + 1), cols = u.tokens * a.group, step = 8 * (dh + 2);
+  const float* const rows = a.parts + (w0 + unit) * step;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // a warp to a query row: the largest maximum, every segment's factor, the sum
+  float top = -INFINITY;
+  if (warp < cols) {
+    for (int w = lane; w < n; w += 32) top = fmaxf(top, rows[w * step + warp * (dh + 2)]);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+  constexpr int kOut = 4;  // outputs of a thread: 8 rows of 128 by 256 threads
+  float v[kOut] = {};
+  float sum = 0.f;
+  for (int p0 = 0; p0 < n; p0 += kBdParts) {
+    __syncthreads();
+    if (warp < cols && p0 + lane < n) {
+      const float* const row = rows + (p0 + lane) * step + warp * (dh + 2);
+      const float f = row[0] == -INFINITY ? 0.f : ex2(row[0] - top);
+      factor[lane][warp] = f;
+      sum += row[1] * f;
     }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kOut; ++q) {
+      const int i = threadIdx.x + 256 * q, col = i / dh, d = i - col * dh;
+      if (i >= cols * dh) break;
+#pragma unroll 8
+      for (int p = 0; p < min(kBdParts, n - p0); ++p) v[q] += rows[(p0 + p) * step + col * (dh + 2) + 2 + d] * factor[p][col];
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (warp < cols && lane == 0) {
+    sums[warp] = sum;
+    if (a.out_partial) {
+      const int tok = warp / a.group, h = head * a.group + warp - tok * a.group;
+      float* const o = a.out_partial + ((int64_t)(u.row0 + tok) * a.Hq + h) * (dh + 2);
+      o[0] = top == -INFINITY ? -INFINITY : top * kLn2, o[1] = sum;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < kOut; ++q) {
+    const int i = threadIdx.x + 256 * q, col = i / dh, d = i - col * dh;
+    if (i >= cols * dh) break;
     const int tok = col / a.group, h = head * a.group + col - tok * a.group;
     const int64_t at = (int64_t)(u.row0 + tok) * a.Hq + h;
-    if (a.out) store_from_float(a.out, a.out_dtype, at * dh + d, sum == 0.f ? 0.f : v / sum);
-    if (a.out_partial) {
-      float* o = a.out_partial + at * (dh + 2);
-      o[2 + d] = v;
-      if (d == 0) o[0] = top == -INFINITY ? -INFINITY : top * kLn2, o[1] = sum;
-    }
+    if (a.out) store_from_float(a.out, a.out_dtype, at * dh + d, sums[col] == 0.f ? 0.f : v[q] / sums[col]);
+    if (a.out_partial) a.out_partial[at * (dh + 2) + 2 + d] = v[q];
   }
 }
 
@@ -544,7 +605,7 @@ static int run_bd(BdArgs& a, void* scratch, int64_t scratch_bytes, const char* w
   a.prefix = nullptr;
   if (int rc = make_codes_map(&a.k_map, a.c, a.c.k_codes, 16, what)) return rc;
   if (int rc = make_codes_map(&a.v_map, a.c, a.c.v_codes, 16, what)) return rc;
-  if (slots > kBdPlanned) {
+  if (slots > kDealt) {
     int64_t* prefix = reinterpret_cast<int64_t*>(scratch);
     (void)launch_overlapped(blocks_plan_kernel, dim3(1), dim3(1024), 0, st, a, prefix);
     if (int rc = check_launch("blocks_plan_kernel")) return rc;
@@ -587,6 +648,7 @@ int few_queries(const sphkv_blocks& c, const BlockRows& r, const void* q, int q_
   a.group = Hq / c.Hkv;
   a.tshift = tshift;
   a.scale_log2 = sm_scale * kLog2e;
+  a.q_vec = ((uintptr_t)q & 15) == 0 && (((q_row_stride | q_head_stride) * (q_dtype == SPHKV_F32 ? 4 : 2)) & 15) == 0;
   return run_bd(a, scratch, scratch_bytes, what, st);
 }
 int64_t few_queries_scratch(int64_t rows, int B, int Hkv, int dh, int tshift, int sms) {
