@@ -36,7 +36,6 @@ struct BdArgs {
   float* parts;           // [workers + units][8][dh + 2]
   int q_dtype, out_dtype, Hq, group, slots, tshift, workers;
   float scale_log2;       // sm_scale * log2 e
-  bool q_vec;             // rows of queries on 16-byte boundaries
 };
 
 template <int DH>
@@ -50,7 +49,10 @@ struct Bd {
   static constexpr int kItemsOff = kPrefixOff + (kDealt + 2) * 8;
   static constexpr int kStatOff = kItemsOff + kDealt * 32;
   static constexpr int kStat = 5 * 8;                              // floats of a warp: maxima, sums, true maxima, S (8 times), factors
-  static constexpr int kBarOff = kStatOff + kBdWarps * (kStat + 8 * 3) * 4;
+  static constexpr int kQOff = kStatOff + kBdWarps * (kStat + 8 * 3) * 4;
+  static constexpr int kQRow = 2 * (DH + 8);                       // bytes of a row of queries in f16
+  static constexpr int kQ = 2 * 8 * kQRow + 32;                    // of a team: hi, lo, factors
+  static constexpr int kBarOff = kQOff + 2 * kQ;
   static constexpr int kSmem = kBarOff + kBdWarps * kStages * 8 + 1024;
 };
 static_assert(Bd<128>::kSmem <= 232448 && Bd<64>::kSmem <= 232448, "shared memory of a CTA");
@@ -134,6 +136,9 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
   float* const cols_of = reinterpret_cast<float*>(smem + L::kStatOff) + kBdWarps * L::kStat + team * WARPS * 24;  // max, sum, true max
   float* const joined = reinterpret_cast<float*>(smem + team * WARPS * L::kRing);  // a warp's outputs: in its ring's place
   constexpr int JOIN = L::kRing / 4;
+  static_assert(kBdWarps / WARPS <= 2, "places for queries");
+  const uint32_t q_at = smem_u32(smem) + L::kQOff + team * L::kQ;  // the segment's queries
+  float* const q_factor = reinterpret_cast<float*>(smem + L::kQOff + team * L::kQ + 2 * 8 * L::kQRow);
   if (lane == 0) {
 #pragma unroll
     for (int s = 0; s < S; ++s) mbar_init(bars + 8 * s, 1);
@@ -175,6 +180,16 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
     pos += count;
     const int cols = u.tokens * a.group;
 
+    // ---- queries, a warp to a row: asked for here, used behind the tiles' addresses ----
+    constexpr int QD = DH / 32;  // dims of a lane
+    float qv[QD];
+    const bool q_row = tw < cols;
+    if (q_row) {
+      const int tok = tw / a.group, h = head * a.group + tw - tok * a.group;
+      const int64_t at = (int64_t)(u.row0 + tok) * a.q_row_stride + (int64_t)h * a.q_head_stride + QD * lane;
+#pragma unroll
+      for (int i = 0; i < QD; ++i) qv[i] = load_as_float(a.q, a.q_dtype, at + i);
+    }
     // ---- where this warp's tiles lie: lane i holds tile 32 r + i of them ----
     const int mine = tw < count ? (count - tw + WARPS - 1) / WARPS : 0;
     const int32_t* table = a.c.block_table + (int64_t)u.b * a.c.max_blocks;
@@ -212,70 +227,45 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
     if (!lost)
       for (int k = 0; k < min(S, mine); ++k) issue(k, 0);
 
-    // ---- queries: lane 4g + j takes dims DH/4 j .. of row g ----
-    uint32_t qh[KS][2], ql[QLO ? KS : 1][2];
-    float f0, f1;      // logit factors of rows 2j, 2j + 1
-    int lim0, lim1;    // the keys that they see end here
-    int least = u.limit;
-    {
-      float v[DH / 4];
+    // ---- the rows in f16, scaled by powers of two; then lane 4g + j takes dims DH/4 j .. of row g ----
+    static_assert(WARPS >= 8, "a warp to a row");
+    if (tw < 8) {
       float top = 0.f;
-      const int tok = g / a.group, h = head * a.group + g - tok * a.group;
-      const bool there = g < cols;  // the others read row 0 of the unit, and are nothing
-      const int64_t at = (int64_t)(u.row0 + (there ? tok : 0)) * a.q_row_stride + (int64_t)(there ? h : head * a.group) * a.q_head_stride + (DH / 4) * j;
-      if (a.q_vec) {
-        constexpr int N = QLO ? DH / 16 : DH / 32;  // 16-byte loads, all on their way at once
-        uint4 raw[N];
-        const uint4* const from = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.q) + at * (QLO ? 4 : 2));
 #pragma unroll
-        for (int i = 0; i < N; ++i) raw[i] = from[i];
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if constexpr (QLO) {
-              v[4 * i + q] = __uint_as_float(w[q]);
-            } else if (a.q_dtype == SPHKV_BF16) {
-              v[8 * i + 2 * q] = __uint_as_float(w[q] << 16), v[8 * i + 2 * q + 1] = __uint_as_float(w[q] & 0xffff0000u);
-            } else {
-              const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[q]));
-              v[8 * i + 2 * q] = x.x, v[8 * i + 2 * q + 1] = x.y;
-            }
-          }
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < DH / 4; ++i) v[i] = load_as_float(a.q, a.q_dtype, at + i);
+      for (int i = 0; i < QD; ++i) {
+        if (!q_row) qv[i] = 0.f;
+        top = isnan(qv[i]) ? INFINITY : fmaxf(top, fabsf(qv[i]));
       }
-#pragma unroll
-      for (int i = 0; i < DH / 4; ++i) {
-        if (!there) v[i] = 0.f;
-        top = fmaxf(top, fabsf(v[i]));
-        if (isnan(v[i])) top = INFINITY;
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      int e = (int)(__float_as_uint(top) >> 23);
+      const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+      int e = (int)(bits >> 23);
       e = e == 255 ? 140 : max(e, 14);  // infinities and NaN go in as they are
-      const float up = __uint_as_float((uint32_t)(267 - e) << 23), down = __uint_as_float((uint32_t)(e - 13) << 23);
+      const float up = __uint_as_float((uint32_t)(267 - e) << 23);
+      if (lane == 0) q_factor[tw] = __uint_as_float((uint32_t)(e - 13) << 23) * a.scale_log2;
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const float x = v[4 * s + 2 * p] * up, y = v[4 * s + 2 * p + 1] * up;
-          if constexpr (QLO)
-            split_f16x2(x, y, qh[s][p], ql[s][p]);
-          else
-            qh[s][p] = pack_f16x2(x, y);
-        }
-      const float f = down * a.scale_log2;
-      f0 = __shfl_sync(0xffffffffu, f, 8 * j);
-      f1 = __shfl_sync(0xffffffffu, f, 8 * j + 4);
-      lim0 = 2 * j < cols ? u.pos0 + 2 * j / a.group + 1 : u.limit;
-      lim1 = 2 * j + 1 < cols ? u.pos0 + (2 * j + 1) / a.group + 1 : u.limit;
-      if (u.tokens > 1) least = u.pos0 + 1;
+      for (int i = 0; i < QD; i += 2) {
+        uint32_t hi, lo;
+        split_f16x2(qv[i] * up, qv[i + 1] * up, hi, lo);
+        const uint32_t to = q_at + tw * L::kQRow + 2 * (QD * lane + i);
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(to), "r"(hi) : "memory");
+        if constexpr (QLO) asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + 8 * L::kQRow), "r"(lo) : "memory");
+      }
     }
+    team_sync();
+    uint32_t qh[KS][2], ql[QLO ? KS : 1][2];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const uint32_t from = q_at + g * L::kQRow + 2 * ((DH / 4) * j + 4 * s);
+      const uint2 h = lds_u2(from);
+      qh[s][0] = h.x, qh[s][1] = h.y;
+      if constexpr (QLO) {
+        const uint2 l = lds_u2(from + 8 * L::kQRow);
+        ql[s][0] = l.x, ql[s][1] = l.y;
+      }
+    }
+    const float f0 = q_factor[2 * j], f1 = q_factor[2 * j + 1];  // logit factors of rows 2j, 2j + 1; where their keys end
+    const int lim0 = 2 * j < cols ? u.pos0 + 2 * j / a.group + 1 : u.limit;
+    const int lim1 = 2 * j + 1 < cols ? u.pos0 + (2 * j + 1) / a.group + 1 : u.limit;
+    const int least = u.tokens > 1 ? u.pos0 + 1 : u.limit;
 
     float acc[KS][4];  // [DH / 16 row tiles of dims]
 #pragma unroll
@@ -648,7 +638,6 @@ int few_queries(const sphkv_blocks& c, const BlockRows& r, const void* q, int q_
   a.group = Hq / c.Hkv;
   a.tshift = tshift;
   a.scale_log2 = sm_scale * kLog2e;
-  a.q_vec = ((uintptr_t)q & 15) == 0 && (((q_row_stride | q_head_stride) * (q_dtype == SPHKV_F32 ? 4 : 2)) & 15) == 0;
   return run_bd(a, scratch, scratch_bytes, what, st);
 }
 int64_t few_queries_scratch(int64_t rows, int B, int Hkv, int dh, int tshift, int sms) {
