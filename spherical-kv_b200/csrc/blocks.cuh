@@ -84,23 +84,29 @@ __device__ __forceinline__ BlockPiece find_piece_alone(const sphkv_blocks& c, co
 }
 
 // ---- work dealt evenly: tiles of all slots and heads in one line ------------------------------------------------
-// prefix[s] = tiles of the slots before s, prefix[slots] = all; by one block, of up to any number of slots.
-template <typename F>
-__device__ __forceinline__ void sum_tiles(int slots, int64_t* prefix, F item) {
-  __shared__ int64_t warp_sums[32];
+// prefix[s] = tiles of the slots before s, prefix[slots] = all; items[s]: the slot's item, which has its `tiles`.  The host has
+// checked that all tiles of all heads are fewer than 2^31.  By one block, of any number of slots.
+template <typename Item, typename F>
+__device__ __forceinline__ void plan_tiles(int slots, uint32_t* prefix, Item* items, F item) {
+  __shared__ uint32_t warp_sums[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int64_t before = 0;
+  uint32_t before = 0;
   for (int s0 = 0; s0 < slots; s0 += blockDim.x) {
     const int s = s0 + tid;
-    int64_t v = s < slots ? item(s).tiles : 0;
+    uint32_t v = 0;
+    if (s < slots) {
+      const Item u = item(s);
+      items[s] = u;
+      v = u.tiles;
+    }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, v, o);
+      const uint32_t up = __shfl_up_sync(0xffffffffu, v, o);
       if (lane >= o) v += up;
     }
     if (lane == 31) warp_sums[warp] = v;
     __syncthreads();
-    int64_t add = before;
+    uint32_t add = before;
     for (int w = 0; w < (int)blockDim.x / 32; ++w) {
       if (w < warp) add += warp_sums[w];
       before += warp_sums[w];
@@ -110,16 +116,17 @@ __device__ __forceinline__ void sum_tiles(int slots, int64_t* prefix, F item) {
   }
   if (tid == 0) prefix[0] = 0;
 }
-// The same for at most kDealt slots by the block's first warp, and the slots' items beside it: a block that shares in the work
-// begins with this, and one warp's shuffles take a third of what a block's barriers take.
+// The same for at most kDealt slots by the first warp of every block that shares in the work: its shuffles take a third of
+// what a block's barriers take, and no launch goes before.
 constexpr int kDealt = 128;
 template <typename Item, typename F>
-__device__ __forceinline__ void deal_tiles(int slots, int64_t* prefix, Item* items, F item) {
+__device__ __forceinline__ void deal_tiles(int slots, uint32_t* prefix, Item* items, F item) {
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
-    int64_t before = 0;
+    uint32_t before = 0;
+#pragma unroll 1
     for (int s0 = 0; s0 < slots; s0 += 32) {
-      int64_t v = 0;
+      uint32_t v = 0;
       if (s0 + lane < slots) {
         const Item u = item(s0 + lane);
         items[s0 + lane] = u;
@@ -127,7 +134,7 @@ __device__ __forceinline__ void deal_tiles(int slots, int64_t* prefix, Item* ite
       }
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, v, o);
+        const uint32_t up = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += up;
       }
       if (s0 + lane < slots) prefix[s0 + lane + 1] = before + v;
@@ -137,7 +144,21 @@ __device__ __forceinline__ void deal_tiles(int slots, int64_t* prefix, Item* ite
   }
   __syncthreads();
 }
-__device__ __forceinline__ int slot_at(const int64_t* prefix, int slots, int64_t tile) {  // prefix[s] <= tile < prefix[s + 1]
+// Tiles for each worker in turn, none without while there are tiles: a slot's segments are those of consecutive workers.
+struct Shares {
+  uint32_t n, per, more;  // workers with tiles; tiles of each; the first `more` have one more
+  __device__ __forceinline__ Shares(uint32_t total, uint32_t workers) {
+    n = min(workers, total);
+    per = n ? total / n : 0;
+    more = total - per * n;
+  }
+  __device__ __forceinline__ uint32_t start(uint32_t w) const { return w * per + min(w, more); }
+  __device__ __forceinline__ uint32_t owner(uint32_t tile) const {
+    const uint32_t large = more * (per + 1);
+    return tile < large ? tile / (per + 1) : more + (tile - large) / per;
+  }
+};
+__device__ __forceinline__ int slot_at(const uint32_t* prefix, int slots, uint32_t tile) {  // prefix[s] <= tile < prefix[s + 1]
   int lo = 0, hi = slots;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;

@@ -39,7 +39,8 @@ struct AtArgs {
   int64_t q_row_stride, q_head_stride;
   const int32_t* first;
   void* out;
-  const int64_t* prefix;
+  const uint32_t* prefix;
+  const struct AtItem* items;
   float* parts;  // [workers][2][dh + 2][256]: a worker's first, cut segment and its last
   int q_dtype, out_dtype, Hq, group, slots, workers;
   bool q_vec;
@@ -70,9 +71,9 @@ __device__ __forceinline__ AtItem item_of(const AtArgs& a, int slot) {
   u.tiles = u.first < limit ? (limit + kAtKeys - 1) / kAtKeys - u.kt0 : 0;
   return u;
 }
-__global__ void __launch_bounds__(1024) blocks_attend_plan_kernel(const __grid_constant__ AtArgs a, int64_t* prefix) {
+__global__ void __launch_bounds__(1024) blocks_attend_plan_kernel(const __grid_constant__ AtArgs a, uint32_t* prefix, AtItem* items) {
   griddep_wait();
-  sum_tiles(a.slots, prefix, [&](int s) { return item_of(a, s); });
+  plan_tiles(a.slots, prefix, items, [&](int s) { return item_of(a, s); });
 }
 
 // ---- shared memory ----------------------------------------------------------------------------------------
@@ -83,7 +84,7 @@ struct AtMeta {       // of a key tile, for the softmax
   uint32_t bad;       // groups without a page
   uint32_t pad;
 };
-constexpr int kAtWalkBytes = 96;
+constexpr int kAtWalkBytes = 112;
 template <int DH>
 struct At {
   static constexpr int kSlab = 128 * 128;             // 128 rows of 64 f16
@@ -91,7 +92,7 @@ struct At {
   static constexpr int kQ = 0, kK = 2 * kOperand, kV = kK + 2 * kOperand, kMeta = kV + 2 * kOperand;
   static constexpr int kBars = kMeta + 4 * (int)sizeof(AtMeta);
   static constexpr int kPrefix = kBars + 24 * 8;
-  static constexpr int kItems = kPrefix + (kDealt + 2) * 8;
+  static constexpr int kItems = kPrefix + (kDealt + 4) * 4;
   static constexpr int kWalks = kItems + kDealt * (int)sizeof(AtItem);
   static constexpr int kSmem = kWalks + kAtThreads / 32 * kAtWalkBytes + 1024;
 };
@@ -147,36 +148,36 @@ __device__ __forceinline__ uint32_t operand_at(int t, int c) { return (c >> 3) *
 // The segments of one worker; every warp walks them by itself, in a place of its own in shared memory: registers are what the
 // loops are short of, and local memory is L2 where shared memory takes all of L1.
 struct AtWalk {
-  int64_t left;  // tiles
+  const uint32_t* prefix;
+  const AtItem* items;
+  uint32_t left;  // tiles
   AtItem u;
   int slot, head, from, count, cnt[2];
   bool whole;
-  __device__ __forceinline__ void begin(const AtArgs& a, const int64_t* prefix, const AtItem* items, int64_t worker) {
-    const int64_t total = prefix[a.slots] * a.c.Hkv, workers = min((int64_t)a.workers, total);
+  __device__ __forceinline__ void begin(const AtArgs& a, uint32_t worker) {
+    const Shares shares(prefix[a.slots] * a.c.Hkv, a.workers);
     left = 0;
     count = 0;
-    if (worker >= workers) return;
-    const int64_t pos = worker * total / workers;
-    left = (worker + 1) * total / workers - pos;
+    if (worker >= shares.n) return;
+    const uint32_t pos = shares.start(worker);
+    left = shares.start(worker + 1) - pos;
     slot = slot_at(prefix, a.slots, pos / a.c.Hkv);
-    u = items ? items[slot] : item_of(a, slot);
-    const int64_t in_slot = pos - prefix[slot] * a.c.Hkv;
-    head = (int)(in_slot / u.tiles);
-    from = (int)(in_slot - (int64_t)head * u.tiles);
+    u = items[slot];
+    const uint32_t in_slot = pos - prefix[slot] * a.c.Hkv;
+    head = in_slot / (uint32_t)u.tiles;
+    from = in_slot - head * u.tiles;
   }
-  __device__ __forceinline__ bool next(const AtArgs& a, const AtItem* items) {
+  __device__ __forceinline__ bool next(const AtArgs& a) {
     if (left == 0) return false;
     if (count > 0) {  // behind a segment: the next head, or the next block with keys
       from = 0;
       if (++head == a.c.Hkv) {
         head = 0;
-        do {
-          ++slot;
-          u = items ? items[slot] : item_of(a, slot);
-        } while (u.tiles == 0);  // there is one: left > 0
+        do u = items[++slot];
+        while (u.tiles == 0);  // there is one: left > 0
       }
     }
-    count = (int)min((int64_t)(u.tiles - from), left);
+    count = min((uint32_t)(u.tiles - from), left);
     left -= count;
     whole = count == u.tiles;
 #pragma unroll
@@ -215,7 +216,6 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   const uint32_t base = smem_u32(smem), bars = base + L::kBars;
-  int64_t* const prefix_smem = reinterpret_cast<int64_t*>(smem + L::kPrefix);
   AtMeta* const metas = reinterpret_cast<AtMeta*>(smem + L::kMeta);
   __shared__ uint32_t tmem_at;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -237,15 +237,22 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
   const uint32_t tmem = tmem_at;
   griddep_launch();
   griddep_wait();
-  const int64_t* prefix = a.prefix;
-  const AtItem* const items = prefix == nullptr ? reinterpret_cast<const AtItem*>(smem + L::kItems) : nullptr;
+  const uint32_t* prefix = a.prefix;
+  const AtItem* items = a.items;
   if (prefix == nullptr) {
-    deal_tiles(a.slots, prefix_smem, reinterpret_cast<AtItem*>(smem + L::kItems), [&](int s) { return item_of(a, s); });
-    prefix = prefix_smem;
+    uint32_t* const at = reinterpret_cast<uint32_t*>(smem + L::kPrefix);
+    AtItem* const of = reinterpret_cast<AtItem*>(smem + L::kItems);
+    deal_tiles(a.slots, at, of, [&](int s) { return item_of(a, s); });
+    prefix = at;
+    items = of;
   }
   AtWalk& walk = *reinterpret_cast<AtWalk*>(smem + L::kWalks + warp * kAtWalkBytes);
   const AtItem& u = walk.u;
-  if (lane == 0) walk.begin(a, prefix, items, blockIdx.x);
+  if (lane == 0) {
+    walk.prefix = prefix;
+    walk.items = items;
+    walk.begin(a, blockIdx.x);
+  }
   bool lost = false;
   auto wait = [&](int bar, uint32_t n) {  // the n-th phase, from 0
     if (!lost && !mbar_wait(bars + 8 * bar, n & 1)) {
@@ -257,7 +264,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
   auto warp_wait = [&](int bar, uint32_t n) { return __all_sync(0xffffffffu, wait(bar, n)); };
   auto next_segment = [&] {
     __syncwarp();
-    const int more = lane == 0 ? walk.next(a, items) : 0;
+    const int more = lane == 0 ? walk.next(a) : 0;
     return __shfl_sync(0xffffffffu, more, 0) != 0;  // and what lane 0 wrote is there for all
   };
 
@@ -699,47 +706,49 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
 
 // CTA (w, y): the block that worker w begins and others go on with, dims 16 y .. of it; and rows of blocks without keys.
 __global__ void __launch_bounds__(256) blocks_attend_merge_kernel(const __grid_constant__ AtArgs a, int dh) {
-  __shared__ int64_t prefix_smem[kDealt + 1];
-  __shared__ AtItem items[kDealt];
+  __shared__ uint32_t prefix_smem[kDealt + 1];
+  __shared__ AtItem items_smem[kDealt];
   griddep_launch();
   griddep_wait();
-  const int64_t* prefix = a.prefix;
-  const bool dealt = prefix == nullptr;
-  if (dealt) {
-    deal_tiles(a.slots, prefix_smem, items, [&](int s) { return item_of(a, s); });
+  const uint32_t* prefix = a.prefix;
+  const AtItem* items = a.items;
+  if (prefix == nullptr) {
+    deal_tiles(a.slots, prefix_smem, items_smem, [&](int s) { return item_of(a, s); });
     prefix = prefix_smem;
+    items = items_smem;
   }
-  const int64_t total = prefix[a.slots] * a.c.Hkv, workers = min((int64_t)a.workers, total);
   const int flat = threadIdx.x, w = blockIdx.x, d0 = 16 * blockIdx.y;
   float o[16];
-  for (int s = w; s < a.slots; s += gridDim.x) {
-    if (prefix[s + 1] != prefix[s]) continue;
-    const AtItem u = dealt ? items[s] : item_of(a, s);
-    if (flat >= u.rows) continue;
-#pragma unroll
-    for (int c = 0; c < 16; ++c) o[c] = 0.f;
-    const int tok = (u.r0 + flat) / a.group, g = u.r0 + flat - tok * a.group;
-    for (int h = 0; h < a.c.Hkv; ++h) store_row16(a.out, a.out_dtype, ((int64_t)(u.row0 + tok) * a.Hq + h * a.group + g) * dh + d0, o);
-  }
-  if (w >= workers) return;
-  const int64_t start = w * total / workers, stop = (w + 1) * total / workers;
-  const int slot = slot_at(prefix, a.slots, (stop - 1) / a.c.Hkv);
-  const AtItem u = dealt ? items[slot] : item_of(a, slot);
-  const int64_t in_slot = stop - 1 - prefix[slot] * a.c.Hkv;
-  const int head = (int)(in_slot / u.tiles);
-  const int64_t p0 = prefix[slot] * a.c.Hkv + (int64_t)head * u.tiles, p1 = p0 + u.tiles - 1;
-  if (p0 < start || p1 < stop || flat >= u.rows) return;
-  const int64_t last = ((p1 + 1) * workers - 1) / total;
-  const int64_t size = (int64_t)(dh + 2) * kAtRows;
-  float top = -INFINITY, sum = 0.f;
-  auto part = [&](int64_t x) { return a.parts + (2 * x + (x == w ? 1 : 0)) * size + flat; };
-  for (int64_t x = w; x <= last; ++x) top = fmaxf(top, part(x)[0]);
 #pragma unroll
   for (int c = 0; c < 16; ++c) o[c] = 0.f;
-  for (int64_t x = w; x <= last; ++x) {
-    const float* p = part(x);
-    if (p[0] == -INFINITY) continue;  // nothing seen there
-    const float f = ex2(p[0] - top);
+#pragma unroll 1
+  for (int s = w; s < a.slots; s += gridDim.x) {
+    if (prefix[s + 1] != prefix[s]) continue;
+    const AtItem u = items[s];
+    if (flat >= u.rows) continue;
+    const int tok = (u.r0 + flat) / a.group, g = u.r0 + flat - tok * a.group;
+#pragma unroll 1
+    for (int h = 0; h < a.c.Hkv; ++h) store_row16(a.out, a.out_dtype, ((int64_t)(u.row0 + tok) * a.Hq + h * a.group + g) * dh + d0, o);
+  }
+  const Shares shares(prefix[a.slots] * a.c.Hkv, a.workers);
+  if (w >= (int)shares.n) return;
+  const uint32_t stop = shares.start(w + 1);
+  const int slot = slot_at(prefix, a.slots, (stop - 1) / a.c.Hkv);
+  const AtItem u = items[slot];
+  const int head = (stop - 1 - prefix[slot] * a.c.Hkv) / (uint32_t)u.tiles;
+  const uint32_t p0 = prefix[slot] * a.c.Hkv + head * u.tiles, end = p0 + u.tiles;
+  if (p0 < shares.start(w) || end <= stop || flat >= u.rows) return;
+  const int n = shares.owner(end - 1) - w + 1;
+  const int size = (dh + 2) * kAtRows;
+  float top = -INFINITY, sum = 0.f;
+  const float* const mine = a.parts + ((int64_t)2 * w + 1) * size + flat;  // the others' are their first places
+  auto part = [&](int x) { return x == 0 ? mine : mine + (int64_t)(2 * x - 1) * size; };
+#pragma unroll 4
+  for (int x = 0; x < n; ++x) top = fmaxf(top, part(x)[0]);
+#pragma unroll 2
+  for (int x = 0; x < n; ++x) {
+    const float* const p = part(x);
+    const float f = p[0] == -INFINITY ? 0.f : ex2(p[0] - top);  // nothing seen there: its outputs are zeros
     sum += p[kAtRows] * f;
 #pragma unroll
     for (int c = 0; c < 16; ++c) o[c] += p[(2 + d0 + c) * kAtRows] * f;
@@ -753,7 +762,7 @@ __global__ void __launch_bounds__(256) blocks_attend_merge_kernel(const __grid_c
 static int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 static int64_t at_slots(int64_t rows, int B, int group) { return (rows * group >> 8) + B; }  // at least block_slots()
 static int64_t at_scratch(int64_t rows, int B, int group, int dh, int sms) {
-  return align256((at_slots(rows, B, group) + 1) * 8) + (int64_t)sms * 2 * (dh + 2) * kAtRows * 4;
+  return align256((at_slots(rows, B, group) + 1) * 4) + align256(at_slots(rows, B, group) * (int64_t)sizeof(AtItem)) + (int64_t)sms * 2 * (dh + 2) * kAtRows * 4;
 }
 
 template <int DH, bool I8>
@@ -822,18 +831,23 @@ extern "C" int sphkv_blocks_attend(const sphkv_blocks* c, const void* q, int32_t
   a.scale_log2 = sm_scale * kLog2e;
   a.workers = sms;
   const int64_t slots = block_slots(a.r, c->B, 8, 1);
-  SPHKV_REQUIRE(slots * c->Hkv <= 0x7fffffff, SPHKV_E_LIMIT, "blocks_attend: too many queries for one launch");
+  // key tiles of all blocks of queries are counted in 32 bits
+  SPHKV_REQUIRE((double)slots * c->Hkv * ((int64_t)c->max_blocks * c->page_size / kAtKeys + 2) < 2147483648.0, SPHKV_E_LIMIT,
+                "blocks_attend: too many (query block, head, token)s for one launch");
   a.slots = (int)slots;
   const int64_t need = at_scratch(rows, c->B, group, c->dh, sms);
   SPHKV_REQUIRE(scratch != nullptr && scratch_bytes >= need, SPHKV_E_SCRATCH, "blocks_attend: scratch %lld B < %lld B",
                 (long long)scratch_bytes, (long long)need);
   SPHKV_REQUIRE(((uintptr_t)scratch & 255) == 0, SPHKV_E_ALIGN, "blocks_attend: scratch needs 256 B");
-  a.parts = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(scratch) + align256((at_slots(rows, c->B, group) + 1) * 8));
+  uint8_t* const items_at = reinterpret_cast<uint8_t*>(scratch) + align256((at_slots(rows, c->B, group) + 1) * 4);
+  a.parts = reinterpret_cast<float*>(items_at + align256(at_slots(rows, c->B, group) * (int64_t)sizeof(AtItem)));
   if (slots > kDealt) {
-    int64_t* prefix = reinterpret_cast<int64_t*>(scratch);
-    (void)launch_overlapped(blocks_attend_plan_kernel, dim3(1), dim3(1024), 0, st, a, prefix);
+    uint32_t* const prefix = reinterpret_cast<uint32_t*>(scratch);
+    AtItem* const items = reinterpret_cast<AtItem*>(items_at);
+    (void)launch_overlapped(blocks_attend_plan_kernel, dim3(1), dim3(1024), 0, st, a, prefix, items);
     if (int rc = check_launch("blocks_attend_plan_kernel")) return rc;
     a.prefix = prefix;
+    a.items = items;
   }
   const bool i8 = c->store == SPHKV_BLOCKS_I8;
   const int rc = c->dh == 128 ? (i8 ? launch_at<128, true>(a, st) : launch_at<128, false>(a, st))

@@ -32,7 +32,8 @@ struct BdArgs {
   const int32_t* first;
   void* out;
   float* out_partial;
-  const int64_t* prefix;  // tiles of the slots before each, where a launch has summed them; else NULL
+  const uint32_t* prefix;  // tiles of the slots before each, where a launch has summed them; else NULL
+  const struct BdUnit* items;
   float* parts;           // [workers + units][8][dh + 2]
   int q_dtype, out_dtype, Hq, group, slots, tshift, workers;
   float scale_log2;       // sm_scale * log2 e
@@ -46,7 +47,7 @@ struct Bd {
   static constexpr int kGroupDims = DH / 8;                        // output dims of a lane
   static constexpr int kCol = 8 * (kGroupDims + 2) + 4;            // floats of an output row in shared memory: no bank twice
   static constexpr int kPrefixOff = kBdWarps * kRing;
-  static constexpr int kItemsOff = kPrefixOff + (kDealt + 2) * 8;
+  static constexpr int kItemsOff = kPrefixOff + (kDealt + 4) * 4;
   static constexpr int kStatOff = kItemsOff + kDealt * 32;
   static constexpr int kStat = 5 * 8;                              // floats of a warp: maxima, sums, true maxima, S (8 times), factors
   static constexpr int kQOff = kStatOff + kBdWarps * (kStat + 8 * 3) * 4;
@@ -81,12 +82,10 @@ __device__ __forceinline__ BdUnit unit_of(const BdArgs& a, const BlockPiece& p) 
 
 static_assert(sizeof(BdUnit) == 32, "a slot's place");
 __device__ __forceinline__ BdUnit unit_of_slot(const BdArgs& a, int s) { return unit_of(a, find_piece_alone(a.c, a.r, s, a.tshift, 1)); }
-__global__ void __launch_bounds__(1024) blocks_plan_kernel(const __grid_constant__ BdArgs a, int64_t* prefix) {
+__global__ void __launch_bounds__(1024) blocks_plan_kernel(const __grid_constant__ BdArgs a, uint32_t* prefix, BdUnit* items) {
   griddep_wait();
-  sum_tiles(a.slots, prefix, [&](int s) { return unit_of_slot(a, s); });
+  plan_tiles(a.slots, prefix, items, [&](int s) { return unit_of_slot(a, s); });
 }
-// the workers that share the tiles: none goes without, so that a unit's segments are those of consecutive workers
-__device__ __forceinline__ int64_t workers_of(const BdArgs& a, int64_t total) { return min((int64_t)a.workers, total); }
 __device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -131,7 +130,6 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
   const int team = warp / WARPS, tw = warp % WARPS;
   const uint32_t ring = smem_u32(smem) + warp * L::kRing;
   const uint32_t bars = smem_u32(smem) + L::kBarOff + warp * S * 8;
-  int64_t* const prefix_smem = reinterpret_cast<int64_t*>(smem + L::kPrefixOff);
   float* const stats = reinterpret_cast<float*>(smem + L::kStatOff) + team * WARPS * L::kStat;  // of the team
   float* const cols_of = reinterpret_cast<float*>(smem + L::kStatOff) + kBdWarps * L::kStat + team * WARPS * 24;  // max, sum, true max
   float* const joined = reinterpret_cast<float*>(smem + team * WARPS * L::kRing);  // a warp's outputs: in its ring's place
@@ -147,18 +145,19 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
   __syncthreads();
   griddep_launch();
   griddep_wait();
-  const int64_t* prefix = a.prefix;
-  BdUnit* const items = reinterpret_cast<BdUnit*>(smem + L::kItemsOff);
-  const bool dealt = prefix == nullptr;
-  if (dealt) {
-    deal_tiles(a.slots, prefix_smem, items, [&](int s) { return unit_of_slot(a, s); });
-    prefix = prefix_smem;
+  const uint32_t* prefix = a.prefix;
+  const BdUnit* items = a.items;
+  if (prefix == nullptr) {
+    uint32_t* const at = reinterpret_cast<uint32_t*>(smem + L::kPrefixOff);
+    BdUnit* const of = reinterpret_cast<BdUnit*>(smem + L::kItemsOff);
+    deal_tiles(a.slots, at, of, [&](int s) { return unit_of_slot(a, s); });
+    prefix = at;
+    items = of;
   }
-  const int64_t total = prefix[a.slots] * a.c.Hkv;
-  const int worker = blockIdx.x * (kBdWarps / WARPS) + team;
-  const int64_t workers = workers_of(a, total);
-  int64_t pos = worker < workers ? worker * total / workers : 0;
-  const int64_t stop = worker < workers ? (worker + 1) * total / workers : 0;
+  const Shares shares(prefix[a.slots] * a.c.Hkv, a.workers);
+  const uint32_t worker = blockIdx.x * (kBdWarps / WARPS) + team;
+  uint32_t pos = worker < shares.n ? shares.start(worker) : 0;
+  const uint32_t stop = worker < shares.n ? shares.start(worker + 1) : 0;
   const uint64_t policy = policy_evict_first();
   const int shift = 31 - __clz(a.c.page_size);
   uint32_t issued = 0, taken = 0;  // tiles since the kernel began: stage = n % S, the barrier's phase n / S
@@ -172,10 +171,10 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
   while (pos < stop) {
     // ---- the segment ----
     const int slot = slot_at(prefix, a.slots, pos / a.c.Hkv);
-    const BdUnit u = dealt ? items[slot] : unit_of_slot(a, slot);
-    const int64_t in_slot = pos - prefix[slot] * a.c.Hkv;
-    const int head = (int)(in_slot / u.tiles), from = (int)(in_slot - (int64_t)head * u.tiles);
-    const int count = (int)min((int64_t)(u.tiles - from), stop - pos);
+    const BdUnit u = items[slot];
+    const uint32_t in_slot = pos - prefix[slot] * a.c.Hkv;
+    const int head = in_slot / (uint32_t)u.tiles, from = in_slot - head * u.tiles;
+    const int count = min((uint32_t)(u.tiles - from), stop - pos);
     const int unit = slot * a.c.Hkv + head;
     pos += count;
     const int cols = u.tokens * a.group;
@@ -478,81 +477,75 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
   }
 }
 
-// A block per unit: joins the segments of units that more than one worker had, and writes the rows of units without keys.
-constexpr int kBdParts = 32;  // segments whose maxima and sums are in shared memory at a time
-__global__ void __launch_bounds__(256) blocks_merge_kernel(const __grid_constant__ BdArgs a, int dh) {
-  __shared__ int64_t prefix_smem[kDealt + 1];
-  __shared__ BdUnit items[kDealt];
-  __shared__ float factor[kBdParts][8], sums[8];
+// A block per query row, a thread per dim: joins the segments of units that more than one worker had, and writes the rows of
+// units without keys.
+constexpr int kBdParts = 128;  // segments whose factors are in shared memory at a time
+template <int DH>
+__global__ void __launch_bounds__(DH) blocks_merge_kernel(const __grid_constant__ BdArgs a) {
+  __shared__ uint32_t prefix_smem[kDealt + 1];
+  __shared__ BdUnit items_smem[kDealt];
+  __shared__ float factor[kBdParts], tops[DH / 32], adds[DH / 32];
   griddep_launch();
   griddep_wait();
-  const int64_t* prefix = a.prefix;
-  const bool dealt = prefix == nullptr;
-  if (dealt) {
-    deal_tiles(a.slots, prefix_smem, items, [&](int s) { return unit_of_slot(a, s); });
+  const uint32_t* prefix = a.prefix;
+  const BdUnit* items = a.items;
+  if (prefix == nullptr) {
+    deal_tiles(a.slots, prefix_smem, items_smem, [&](int s) { return unit_of_slot(a, s); });
     prefix = prefix_smem;
+    items = items_smem;
   }
-  const int unit = blockIdx.x, slot = unit / a.c.Hkv, head = unit - slot * a.c.Hkv;
-  const int64_t total = prefix[a.slots] * a.c.Hkv;
-  const BdUnit u = dealt ? items[slot] : unit_of_slot(a, slot);
-  if (u.tokens == 0) return;
-  int64_t w0 = 0, w1 = -1;
+  const int unit = blockIdx.x, col = blockIdx.y, slot = unit / a.c.Hkv, head = unit - slot * a.c.Hkv;
+  const BdUnit u = items[slot];
+  if (col >= u.tokens * a.group) return;
+  const Shares shares(prefix[a.slots] * a.c.Hkv, a.workers);
+  int n = 0;
+  uint32_t first = 0;
   if (u.tiles > 0) {
-    const int64_t p0 = prefix[slot] * a.c.Hkv + (int64_t)head * u.tiles, p1 = p0 + u.tiles - 1;
-    const int64_t workers = workers_of(a, total);
-    w0 = ((p0 + 1) * workers - 1) / total;
-    w1 = ((p1 + 1) * workers - 1) / total;
-    if (w0 == w1) return;
+    const uint32_t p0 = prefix[slot] * a.c.Hkv + head * u.tiles;
+    first = shares.owner(p0);
+    n = shares.owner(p0 + u.tiles - 1) - first + 1;
+    if (n == 1) return;  // its worker has written it
   }
-  const int n = (int)(w1 - w0 + 1), cols = u.tokens * a.group, step = 8 * (dh + 2);
-  const float* const rows = a.parts + (w0 + unit) * step;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // a warp to a query row: the largest maximum, every segment's factor, the sum
+  const int d = threadIdx.x, warp = d >> 5, lane = d & 31;
+  constexpr int STEP = 8 * (DH + 2);
+  const float* const rows = a.parts + (int64_t)(first + unit) * STEP + col * (DH + 2);
   float top = -INFINITY;
-  if (warp < cols) {
-    for (int w = lane; w < n; w += 32) top = fmaxf(top, rows[w * step + warp * (dh + 2)]);
+  for (int p = d; p < n; p += DH) top = fmaxf(top, rows[p * STEP]);
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  }
-  constexpr int kOut = 4;  // outputs of a thread: 8 rows of 128 by 256 threads
-  float v[kOut] = {};
-  float sum = 0.f;
+  for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) tops[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < DH / 32; ++w) top = fmaxf(top, tops[w]);
+  float sum = 0.f, v = 0.f;
   for (int p0 = 0; p0 < n; p0 += kBdParts) {
-    __syncthreads();
-    if (warp < cols && p0 + lane < n) {
-      const float* const row = rows + (p0 + lane) * step + warp * (dh + 2);
+    const int here = min(kBdParts, n - p0);
+    if (p0 > 0) __syncthreads();
+    for (int p = d; p < here; p += DH) {
+      const float* const row = rows + (p0 + p) * STEP;
       const float f = row[0] == -INFINITY ? 0.f : ex2(row[0] - top);
-      factor[lane][warp] = f;
+      factor[p] = f;
       sum += row[1] * f;
     }
     __syncthreads();
-#pragma unroll
-    for (int q = 0; q < kOut; ++q) {
-      const int i = threadIdx.x + 256 * q, col = i / dh, d = i - col * dh;
-      if (i >= cols * dh) break;
+    const float* const from = rows + p0 * STEP + 2 + d;
 #pragma unroll 8
-      for (int p = 0; p < min(kBdParts, n - p0); ++p) v[q] += rows[(p0 + p) * step + col * (dh + 2) + 2 + d] * factor[p][col];
-    }
+    for (int p = 0; p < here; ++p) v += from[p * STEP] * factor[p];
   }
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (warp < cols && lane == 0) {
-    sums[warp] = sum;
-    if (a.out_partial) {
-      const int tok = warp / a.group, h = head * a.group + warp - tok * a.group;
-      float* const o = a.out_partial + ((int64_t)(u.row0 + tok) * a.Hq + h) * (dh + 2);
-      o[0] = top == -INFINITY ? -INFINITY : top * kLn2, o[1] = sum;
-    }
-  }
+  if (lane == 0) adds[warp] = sum;
   __syncthreads();
+  sum = 0.f;
 #pragma unroll
-  for (int q = 0; q < kOut; ++q) {
-    const int i = threadIdx.x + 256 * q, col = i / dh, d = i - col * dh;
-    if (i >= cols * dh) break;
-    const int tok = col / a.group, h = head * a.group + col - tok * a.group;
-    const int64_t at = (int64_t)(u.row0 + tok) * a.Hq + h;
-    if (a.out) store_from_float(a.out, a.out_dtype, at * dh + d, sums[col] == 0.f ? 0.f : v[q] / sums[col]);
-    if (a.out_partial) a.out_partial[at * (dh + 2) + 2 + d] = v[q];
+  for (int w = 0; w < DH / 32; ++w) sum += adds[w];
+  const int tok = col / a.group, h = head * a.group + col - tok * a.group;
+  const int64_t at = (int64_t)(u.row0 + tok) * a.Hq + h;
+  if (a.out) store_from_float(a.out, a.out_dtype, at * DH + d, sum == 0.f ? 0.f : v / sum);
+  if (a.out_partial) {
+    float* const o = a.out_partial + at * (DH + 2);
+    o[2 + d] = v;
+    if (d == 0) o[0] = top == -INFINITY ? -INFINITY : top * kLn2, o[1] = sum;
   }
 }
 
@@ -560,7 +553,7 @@ int tokens_shift(int group) { return group == 1 ? 3 : group == 2 ? 2 : group <= 
 static int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
 static int64_t bd_scratch(int64_t slots, int Hkv, int dh, int workers) {
-  return align256((slots + 1) * 8) + (workers + slots * Hkv) * 8 * (dh + 2) * 4;
+  return align256((slots + 1) * 4) + align256(slots * (int64_t)sizeof(BdUnit)) + (workers + slots * Hkv) * 8 * (dh + 2) * 4;
 }
 
 template <int DH, bool I8, bool QLO>
@@ -584,25 +577,35 @@ static int run_bd(BdArgs& a, void* scratch, int64_t scratch_bytes, const char* w
   if (sms <= 0) return sms;
   const int64_t slots = block_slots(a.r, a.c.B, a.tshift, 1);
   if (slots == 0) return 0;
-  SPHKV_REQUIRE(slots * a.c.Hkv <= 0x7fffffff, SPHKV_E_LIMIT, "%s: too many queries for one launch", what);
+  // tiles of all units are counted in 32 bits
+  SPHKV_REQUIRE((double)slots * a.c.Hkv * ((int64_t)a.c.max_blocks * (a.c.page_size / 16) + 1) < 2147483648.0, SPHKV_E_LIMIT,
+                "%s: too many (sequence, head, token)s for one launch", what);
   a.slots = (int)slots;
   a.workers = sms;
   const int64_t need = bd_scratch(slots, a.c.Hkv, a.c.dh, a.workers);
   SPHKV_REQUIRE(scratch != nullptr && scratch_bytes >= need, SPHKV_E_SCRATCH, "%s: scratch %lld B < %lld B", what,
                 (long long)scratch_bytes, (long long)need);
   SPHKV_REQUIRE(((uintptr_t)scratch & 255) == 0, SPHKV_E_ALIGN, "%s: scratch needs 256 B", what);
-  a.parts = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(scratch) + align256((slots + 1) * 8));
+  uint8_t* const items_at = reinterpret_cast<uint8_t*>(scratch) + align256((slots + 1) * 4);
+  a.parts = reinterpret_cast<float*>(items_at + align256(slots * (int64_t)sizeof(BdUnit)));
   a.prefix = nullptr;
+  a.items = nullptr;
   if (int rc = make_codes_map(&a.k_map, a.c, a.c.k_codes, 16, what)) return rc;
   if (int rc = make_codes_map(&a.v_map, a.c, a.c.v_codes, 16, what)) return rc;
   if (slots > kDealt) {
-    int64_t* prefix = reinterpret_cast<int64_t*>(scratch);
-    (void)launch_overlapped(blocks_plan_kernel, dim3(1), dim3(1024), 0, st, a, prefix);
+    uint32_t* const prefix = reinterpret_cast<uint32_t*>(scratch);
+    BdUnit* const items = reinterpret_cast<BdUnit*>(items_at);
+    (void)launch_overlapped(blocks_plan_kernel, dim3(1), dim3(1024), 0, st, a, prefix, items);
     if (int rc = check_launch("blocks_plan_kernel")) return rc;
     a.prefix = prefix;
+    a.items = items;
   }
   if (int rc = a.c.dh == 128 ? launch_bd_types<128>(a, sms, st) : launch_bd_types<64>(a, sms, st)) return rc;
-  (void)launch_overlapped(blocks_merge_kernel, dim3((unsigned)(slots * a.c.Hkv)), dim3(256), 0, st, a, (int)a.c.dh);
+  const dim3 grid((unsigned)(slots * a.c.Hkv), (unsigned)(a.group << a.tshift));
+  if (a.c.dh == 128)
+    (void)launch_overlapped(blocks_merge_kernel<128>, grid, dim3(128), 0, st, a);
+  else
+    (void)launch_overlapped(blocks_merge_kernel<64>, grid, dim3(64), 0, st, a);
   return check_launch("blocks_merge_kernel");
 }
 
