@@ -235,7 +235,6 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_at;
-  griddep_launch();
   griddep_wait();
   const uint32_t* prefix = a.prefix;
   const AtItem* items = a.items;
@@ -709,7 +708,6 @@ __global__ void __launch_bounds__(256) blocks_attend_merge_kernel(const __grid_c
   __shared__ uint32_t prefix_smem[kDealt + 1];
   __shared__ AtItem items_smem[kDealt];
   griddep_launch();
-  griddep_wait();
   const uint32_t* prefix = a.prefix;
   const AtItem* items = a.items;
   if (prefix == nullptr) {
@@ -853,6 +851,6 @@ extern "C" int sphkv_blocks_attend(const sphkv_blocks* c, const void* q, int32_t
   const int rc = c->dh == 128 ? (i8 ? launch_at<128, true>(a, st) : launch_at<128, false>(a, st))
                               : (i8 ? launch_at<64, true>(a, st) : launch_at<64, false>(a, st));
   if (rc) return rc;
-  (void)launch_overlapped(blocks_attend_merge_kernel, dim3(a.workers, c->dh / 16), dim3(256), 0, st, a, (int)c->dh);
+  blocks_attend_merge_kernel<<<dim3(a.workers, c->dh / 16), 256, 0, st>>>(a, c->dh);
   return check_launch("blocks_attend_merge_kernel");
 }

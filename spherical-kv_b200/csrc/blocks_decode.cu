@@ -34,6 +34,7 @@ struct BdArgs {
   float* out_partial;
   const uint32_t* prefix;  // tiles of the slots before each, where a launch has summed them; else NULL
   const struct BdUnit* items;
+  int4* spans;            // of each unit: first worker, workers, its queries' first row, tokens
   float* parts;           // [workers + units][8][dh + 2]
   int q_dtype, out_dtype, Hq, group, slots, tshift, workers;
   float scale_log2;       // sm_scale * log2 e
@@ -143,7 +144,6 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
     fence_async_smem();
   }
   __syncthreads();
-  griddep_launch();
   griddep_wait();
   const uint32_t* prefix = a.prefix;
   const BdUnit* items = a.items;
@@ -155,6 +155,9 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
     items = of;
   }
   const Shares shares(prefix[a.slots] * a.c.Hkv, a.workers);
+  for (int s = blockIdx.x; s < a.slots; s += gridDim.x)  // units without keys: zeros, by the second launch
+    if (items[s].tiles == 0 && tid < a.c.Hkv)
+      for (int h = tid; h < a.c.Hkv; h += kBdThreads) a.spans[s * a.c.Hkv + h] = make_int4(0, 0, items[s].row0, items[s].tokens);
   const uint32_t worker = blockIdx.x * (kBdWarps / WARPS) + team;
   uint32_t pos = worker < shares.n ? shares.start(worker) : 0;
   const uint32_t stop = worker < shares.n ? shares.start(worker + 1) : 0;
@@ -176,6 +179,8 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
     const int head = in_slot / (uint32_t)u.tiles, from = in_slot - head * u.tiles;
     const int count = min((uint32_t)(u.tiles - from), stop - pos);
     const int unit = slot * a.c.Hkv + head;
+    if (from == 0 && tw == 0 && lane == 0)
+      a.spans[unit] = make_int4(worker, shares.owner(pos + u.tiles - 1) - worker + 1, u.row0, u.tokens);
     pos += count;
     const int cols = u.tokens * a.group;
 
@@ -482,30 +487,13 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
 constexpr int kBdParts = 128;  // segments whose factors are in shared memory at a time
 template <int DH>
 __global__ void __launch_bounds__(DH) blocks_merge_kernel(const __grid_constant__ BdArgs a) {
-  __shared__ uint32_t prefix_smem[kDealt + 1];
-  __shared__ BdUnit items_smem[kDealt];
   __shared__ float factor[kBdParts], tops[DH / 32], adds[DH / 32];
   griddep_launch();
-  griddep_wait();
-  const uint32_t* prefix = a.prefix;
-  const BdUnit* items = a.items;
-  if (prefix == nullptr) {
-    deal_tiles(a.slots, prefix_smem, items_smem, [&](int s) { return unit_of_slot(a, s); });
-    prefix = prefix_smem;
-    items = items_smem;
-  }
-  const int unit = blockIdx.x, col = blockIdx.y, slot = unit / a.c.Hkv, head = unit - slot * a.c.Hkv;
-  const BdUnit u = items[slot];
-  if (col >= u.tokens * a.group) return;
-  const Shares shares(prefix[a.slots] * a.c.Hkv, a.workers);
-  int n = 0;
-  uint32_t first = 0;
-  if (u.tiles > 0) {
-    const uint32_t p0 = prefix[slot] * a.c.Hkv + head * u.tiles;
-    first = shares.owner(p0);
-    n = shares.owner(p0 + u.tiles - 1) - first + 1;
-    if (n == 1) return;  // its worker has written it
-  }
+  const int unit = blockIdx.x, col = blockIdx.y;
+  const int4 span = a.spans[unit];
+  const int first = span.x, n = span.y, row0 = span.z;
+  if (n == 1 || col >= span.w * a.group) return;  // one worker: it has written its unit
+  const int head = unit % a.c.Hkv;
   const int d = threadIdx.x, warp = d >> 5, lane = d & 31;
   constexpr int STEP = 8 * (DH + 2);
   const float* const rows = a.parts + (int64_t)(first + unit) * STEP + col * (DH + 2);
@@ -540,7 +528,7 @@ __global__ void __launch_bounds__(DH) blocks_merge_kernel(const __grid_constant_
 #pragma unroll
   for (int w = 0; w < DH / 32; ++w) sum += adds[w];
   const int tok = col / a.group, h = head * a.group + col - tok * a.group;
-  const int64_t at = (int64_t)(u.row0 + tok) * a.Hq + h;
+  const int64_t at = (int64_t)(row0 + tok) * a.Hq + h;
   if (a.out) store_from_float(a.out, a.out_dtype, at * DH + d, sum == 0.f ? 0.f : v / sum);
   if (a.out_partial) {
     float* const o = a.out_partial + at * (DH + 2);
@@ -553,7 +541,7 @@ int tokens_shift(int group) { return group == 1 ? 3 : group == 2 ? 2 : group <= 
 static int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
 static int64_t bd_scratch(int64_t slots, int Hkv, int dh, int workers) {
-  return align256((slots + 1) * 4) + align256(slots * (int64_t)sizeof(BdUnit)) + (workers + slots * Hkv) * 8 * (dh + 2) * 4;
+  return align256((slots + 1) * 4) + align256(slots * (int64_t)sizeof(BdUnit)) + align256(slots * Hkv * 16) + (workers + slots * Hkv) * 8 * (dh + 2) * 4;
 }
 
 template <int DH, bool I8, bool QLO>
@@ -587,7 +575,8 @@ static int run_bd(BdArgs& a, void* scratch, int64_t scratch_bytes, const char* w
                 (long long)scratch_bytes, (long long)need);
   SPHKV_REQUIRE(((uintptr_t)scratch & 255) == 0, SPHKV_E_ALIGN, "%s: scratch needs 256 B", what);
   uint8_t* const items_at = reinterpret_cast<uint8_t*>(scratch) + align256((slots + 1) * 4);
-  a.parts = reinterpret_cast<float*>(items_at + align256(slots * (int64_t)sizeof(BdUnit)));
+  a.spans = reinterpret_cast<int4*>(items_at + align256(slots * (int64_t)sizeof(BdUnit)));
+  a.parts = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.spans) + align256(slots * a.c.Hkv * 16));
   a.prefix = nullptr;
   a.items = nullptr;
   if (int rc = make_codes_map(&a.k_map, a.c, a.c.k_codes, 16, what)) return rc;
@@ -602,10 +591,11 @@ static int run_bd(BdArgs& a, void* scratch, int64_t scratch_bytes, const char* w
   }
   if (int rc = a.c.dh == 128 ? launch_bd_types<128>(a, sms, st) : launch_bd_types<64>(a, sms, st)) return rc;
   const dim3 grid((unsigned)(slots * a.c.Hkv), (unsigned)(a.group << a.tshift));
+  // a plain launch: one that may come in early is 2.5 us slower (its blocks wait where the next call's would begin)
   if (a.c.dh == 128)
-    (void)launch_overlapped(blocks_merge_kernel<128>, grid, dim3(128), 0, st, a);
+    blocks_merge_kernel<128><<<grid, 128, 0, st>>>(a);
   else
-    (void)launch_overlapped(blocks_merge_kernel<64>, grid, dim3(64), 0, st, a);
+    blocks_merge_kernel<64><<<grid, 64, 0, st>>>(a);
   return check_launch("blocks_merge_kernel");
 }
 
