@@ -20,57 +20,55 @@ constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds |q| < 2^22
 // q approximates the quotient to 1.5 ulp (a rounded reciprocal or ratio, one product).  Only where that leaves the nearest code
 // open, within 2^-15 of a whole number's border or 4 ulp of an e4m3 border, is the quotient itself formed in 64 bits,
 // whose error (2^-53) no quotient of two fp32 numbers is closer to a border than, unless it is a tie.
-template <typename Exact>
-__device__ __forceinline__ uint32_t nearest4_i8(const float (&q)[4], Exact exact) {
-  float t[4], off = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    t[i] = q[i] + kMagic;
-    off = fmaxf(off, fabsf(q[i] - (t[i] - kMagic)));
-  }
-  uint32_t r = __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040),
-                           __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
-  if (off > 0.5f - 0x1p-15f) {
-    r = 0;
-#pragma unroll 1
-    for (int i = 0; i < 4; ++i) r |= ((uint32_t)(int)rint(exact(i)) & 0xffu) << (8 * i);
-  }
-  return r;
-}
-__device__ __forceinline__ bool e4m3_border(float q) {
-  const uint32_t a = __float_as_uint(q) & 0x7fffffffu;
-  if (a < 0x3c800000u)  // below 2^-6 the codes are multiples of 2^-9; zero is one of them
-    return a != 0u && fabsf(fmodf(fabsf(q), 0x1p-9f) - 0x1p-10f) < 0x1p-27f;
-  return ((a - 0x7fffcu) & 0xfffffu) <= 8u;
-}
-static __device__ __noinline__ uint32_t e4m3_of_double(double q) {
+template <bool I8>
+__device__ uint32_t code_of_double(double q) {
+  if constexpr (I8) return (uint32_t)(int)rint(q) & 0xffu;
   const double a = fabs(q);
   const int e = a < 0x1p-6 ? -6 : ilogb(a);
   const double step = scalbn(1.0, e - 3);
-  const float v = (float)copysign(rint(a / step) * step, q);  // an e4m3 value, or 480 -> saturates
+  const float v = (float)copysign(rint(a / step) * step, q);  // an e4m3 value, or 480, which becomes 448
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(v));
   return r & 0xffu;
 }
-template <typename Exact>
-__device__ __forceinline__ uint32_t nearest4_e4m3(const float (&q)[4], Exact exact) {
-  uint16_t lo, hi;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(q[1]), "f"(q[0]));
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(q[3]), "f"(q[2]));
-  uint32_t r = (uint32_t)lo | ((uint32_t)hi << 16);
-  if (e4m3_border(q[0]) | e4m3_border(q[1]) | e4m3_border(q[2]) | e4m3_border(q[3])) {
-    r = 0;
-#pragma unroll 1
-    for (int i = 0; i < 4; ++i) r |= e4m3_of_double(exact(i)) << (8 * i);
-  }
-  return r;
+// codes of x * mul / s.  A function of its own: one in some thousands of its callers' elements comes here, and 64-bit
+// division in line, for every four elements of a lane, took their registers.
+template <bool I8>
+static __device__ __noinline__ uint32_t exact4(float x0, float x1, float x2, float x3, float mul, float s) {
+  return code_of_double<I8>((double)x0 * (double)mul / (double)s) | (code_of_double<I8>((double)x1 * (double)mul / (double)s) << 8) |
+         (code_of_double<I8>((double)x2 * (double)mul / (double)s) << 16) | (code_of_double<I8>((double)x3 * (double)mul / (double)s) << 24);
 }
-template <bool I8, typename Exact>
-__device__ __forceinline__ uint32_t nearest4(const float (&q)[4], Exact exact) {
-  if constexpr (I8)
-    return nearest4_i8(q, exact);
-  else
-    return nearest4_e4m3(q, exact);
+__device__ __forceinline__ bool e4m3_border(float q) {
+  const uint32_t a = __float_as_uint(q) & 0x7fffffffu;
+  if (a < 0x3c800000u)  // below 2^-6 the codes are multiples of 2^-9; zero is one of them
+    return a != 0u && fabsf(fabsf(q) * 0x1p9f - floorf(fabsf(q) * 0x1p9f) - 0.5f) < 0x1p-18f;
+  return ((a - 0x7fffcu) & 0xfffffu) <= 8u;
+}
+// codes of x * mul / s, by = mul / s rounded (or 1 / s where mul is 1)
+template <bool I8>
+__device__ __forceinline__ uint32_t nearest4(const float* x, float by, float mul, float s) {
+  const float q[4] = {x[0] * by, x[1] * by, x[2] * by, x[3] * by};
+  uint32_t r;
+  bool open;
+  if constexpr (I8) {
+    float t[4], off = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      t[i] = q[i] + kMagic;
+      off = fmaxf(off, fabsf(q[i] - (t[i] - kMagic)));
+    }
+    r = __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040),
+                    __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
+    open = off > 0.5f - 0x1p-15f;
+  } else {
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(q[1]), "f"(q[0]));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(q[3]), "f"(q[2]));
+    r = (uint32_t)lo | ((uint32_t)hi << 16);
+    open = e4m3_border(q[0]) | e4m3_border(q[1]) | e4m3_border(q[2]) | e4m3_border(q[3]);
+  }
+  if (open) r = exact4<I8>(x[0], x[1], x[2], x[3], mul, s);
+  return r;
 }
 
 // ---- 16 bytes of a dense row ---------------------------------------------------------------------------------
@@ -125,9 +123,12 @@ struct Chunk<__half> {
     return make_uint4(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]), pack_f16x2(f[4], f[5]), pack_f16x2(f[6], f[7]));
   }
 };
-template <typename T>
-__device__ __forceinline__ uint4 load_chunk(const T* p, bool vec) {
-  if (vec) return *reinterpret_cast<const uint4*>(p);
+template <typename T, bool VEC>
+__device__ __forceinline__ uint4 load_chunk(const T* p) {
+  if constexpr (VEC) {
+    const float4 v = ldg_stream_f4(p);
+    return make_uint4(__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w));
+  }
   constexpr int E = 16 / sizeof(T);
   union {
     uint4 v;
@@ -178,8 +179,11 @@ __device__ __forceinline__ IoTile io_tile(const BlocksIo& a, int64_t team, int p
 // A (page, side, head) belongs to page_size / 16 warps of one CTA; a warp holds its 16 rows as raw 16-byte chunks between the
 // search for the largest magnitude and the rounding, so keys and values are read once.  Consecutive teams are heads of one
 // page: their rows lie side by side in the dense tensors.
-template <typename T, int DH, bool I8>
-__global__ void __launch_bounds__(kIoThreads) blocks_append_kernel(const BlocksIo a) {
+//
+// Loads are made whether or not their row is wanted, from the nearest row that is (twice the same row leaves the largest magnitude as
+// it is): a load that may be skipped ends in a copy that waits for it, and 16 of them one after the other are what a tile takes.
+template <typename T, int DH, bool I8, bool VEC>
+__global__ void __launch_bounds__(kIoThreads, sizeof(T) * DH == 512 ? 2 : 4) blocks_append_kernel(const BlocksIo a) {
   constexpr int E = 16 / sizeof(T), LPR = DH / E, RPL = 32 / LPR, L = 16 / RPL;  // lanes a row, rows a load, loads
   __shared__ uint32_t tops[kIoThreads / 32];
   griddep_wait();
@@ -198,12 +202,16 @@ __global__ void __launch_bounds__(kIoThreads) blocks_append_kernel(const BlocksI
   uint4 raw[L];
   uint32_t m = 0;
   const T* src = reinterpret_cast<const T*>(a.src[t.side]) + (int64_t)t.head * a.head_stride[t.side] + (lane % LPR) * E;
+  const int lowest = max(first_new, 0);
+  if (lowest < end) {
 #pragma unroll
-  for (int i = 0; i < L; ++i) {
-    const int row = i * RPL + lane / LPR;
-    raw[i] = make_uint4(0, 0, 0, 0);
-    if (row >= first_new && row < end)
-      raw[i] = load_chunk(src + (int64_t)(t.p.row0 + row - first_new) * a.row_stride[t.side], a.vec);
+    for (int i = 0; i < L; ++i) {
+      const int row = min(max(i * RPL + lane / LPR, lowest), end - 1);
+      raw[i] = load_chunk<T, VEC>(src + (int64_t)(t.p.row0 + row - first_new) * a.row_stride[t.side]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < L; ++i) raw[i] = make_uint4(0, 0, 0, 0);
   }
   constexpr int OL = DH / 32, OLPR = DH / 16;  // held codes: 16 of a row per lane
   uint4 held[OL];
@@ -211,8 +219,8 @@ __global__ void __launch_bounds__(kIoThreads) blocks_append_kernel(const BlocksI
   if (holds) {
 #pragma unroll
     for (int i = 0; i < OL; ++i) {
-      const int row = i * (32 / OLPR) + lane / OLPR;
-      held[i] = row < first_new ? *reinterpret_cast<const uint4*>(codes + row * DH + (lane % OLPR) * 16) : make_uint4(0, 0, 0, 0);
+      const int row = min(i * (32 / OLPR) + lane / OLPR, first_new - 1);
+      held[i] = *reinterpret_cast<const uint4*>(codes + row * DH + (lane % OLPR) * 16);
     }
   }
 #pragma unroll
@@ -253,13 +261,7 @@ __global__ void __launch_bounds__(kIoThreads) blocks_append_kernel(const BlocksI
 #pragma unroll
     for (int k = 0; k < E / 4; ++k) {
       w[k] = 0;
-      if (finite) {
-        const float q[4] = {f[4 * k] * inv, f[4 * k + 1] * inv, f[4 * k + 2] * inv, f[4 * k + 3] * inv};
-        w[k] = nearest4<I8>(q, [&](int j) {
-          const float x = j < 2 ? (j ? f[4 * k + 1] : f[4 * k]) : (j == 2 ? f[4 * k + 2] : f[4 * k + 3]);
-          return (double)x / (double)s;
-        });
-      }
+      if (finite) w[k] = nearest4<I8>(f + 4 * k, inv, 1.f, s);
     }
     uint8_t* to = codes + row * DH + (lane % LPR) * E;
     if constexpr (E == 8)
@@ -279,12 +281,7 @@ __global__ void __launch_bounds__(kIoThreads) blocks_append_kernel(const BlocksI
         float f[4];
         codes_to_f32<I8>(w[k], f);
         w[k] = 0;
-        if (finite) {
-          const float q[4] = {f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio};
-          w[k] = nearest4<I8>(q, [&](int j) {
-            return (double)(j < 2 ? (j ? f[1] : f[0]) : (j == 2 ? f[2] : f[3])) * (double)s_old / (double)s;
-          });
-        }
+        if (finite) w[k] = nearest4<I8>(f, ratio, s_old, s);
       }
       *reinterpret_cast<uint4*>(codes + row * DH + (lane % OLPR) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
     }
@@ -308,17 +305,12 @@ __global__ void __launch_bounds__(kIoThreads) blocks_read_kernel(const BlocksIo 
   uint32_t w[L][E / 4];
 #pragma unroll
   for (int i = 0; i < L; ++i) {
-    const int row = i * RPL + lane / LPR;
-    const uint8_t* from = codes + row * DH + (lane % LPR) * E;
-#pragma unroll
-    for (int k = 0; k < E / 4; ++k) w[i][k] = 0;
-    if (live && row >= first && row < end) {
-      if constexpr (E == 8) {
-        const uint2 v = *reinterpret_cast<const uint2*>(from);
-        w[i][0] = v.x, w[i][1] = v.y;
-      } else {
-        w[i][0] = *reinterpret_cast<const uint32_t*>(from);
-      }
+    const uint8_t* from = codes + (i * RPL + lane / LPR) * DH + (lane % LPR) * E;  // all 16 rows are a page's, wanted or not
+    if constexpr (E == 8) {
+      const uint2 v = *reinterpret_cast<const uint2*>(from);
+      w[i][0] = v.x, w[i][1] = v.y;
+    } else {
+      w[i][0] = *reinterpret_cast<const uint32_t*>(from);
     }
   }
 #pragma unroll
@@ -331,7 +323,7 @@ __global__ void __launch_bounds__(kIoThreads) blocks_read_kernel(const BlocksIo 
       float g[4];
       codes_to_f32<I8>(w[i][k], g);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) f[4 * k + j] = g[j] * s;
+      for (int j = 0; j < 4; ++j) f[4 * k + j] = live ? g[j] * s : 0.f;
     }
     T* to = reinterpret_cast<T*>(a.dst[t.side]) + ((int64_t)(t.p.row0 + row - first) * a.c.Hkv + t.head) * DH + (lane % LPR) * E;
     *reinterpret_cast<uint4*>(to) = Chunk<T>::pack(f);
@@ -410,7 +402,8 @@ static int launch_io(const BlocksIo& a, int64_t blocks, cudaStream_t st) {
     (void)launch_overlapped(k, dim3((unsigned)blocks), dim3(kIoThreads), 0, st, a);
     return check_launch("blocks_read_kernel");
   } else {
-    auto k = a.c.store == SPHKV_BLOCKS_I8 ? blocks_append_kernel<T, DH, true> : blocks_append_kernel<T, DH, false>;
+    auto k = a.c.store == SPHKV_BLOCKS_I8 ? (a.vec ? blocks_append_kernel<T, DH, true, true> : blocks_append_kernel<T, DH, true, false>)
+                                          : (a.vec ? blocks_append_kernel<T, DH, false, true> : blocks_append_kernel<T, DH, false, false>);
     (void)launch_overlapped(k, dim3((unsigned)blocks), dim3(kIoThreads), 0, st, a);
     return check_launch("blocks_append_kernel");
   }
