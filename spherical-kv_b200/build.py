@@ -48,12 +48,12 @@ def _host_module(force: bool) -> "subprocess.Popen | None":
     import torch
     src = os.path.join(CSRC, "host_tables.cpp")
     target = _host_path()
-    if not (force or _stale(target, [src, os.path.abspath(__file__)])):
+    if not (force or _stale(target, [src, os.path.join(INCLUDE, "sphkv.h"), os.path.abspath(__file__)])):
         return None
     root = os.path.dirname(torch.__file__)
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-isystem", os.path.join(root, "include"), "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
-           "-isystem", sysconfig.get_paths()["include"], src, "-o", target,
+           "-isystem", sysconfig.get_paths()["include"], "-I", INCLUDE, src, "-o", target,
            "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
     return subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
 
