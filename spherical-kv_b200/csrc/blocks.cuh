@@ -31,56 +31,65 @@ struct BlockPiece {
 __device__ __forceinline__ void bad_status(const sphkv_blocks& c, int bit) {
   if (c.status) atomicOr(c.status, bit);
 }
-__device__ __forceinline__ BlockPiece checked_piece(const sphkv_blocks& c, const BlockRows& r, int b, int j, int lo, int hi) {
-  BlockPiece p = {b, j, lo, hi - lo, 0};
+__device__ __forceinline__ BlockPiece checked_piece(const sphkv_blocks& c, const BlockRows& r, int b, int j, int lo, int hi, int end) {
+  BlockPiece p = {b, j, lo, hi - lo, end};
   if (b < 0 || lo < 0 || hi < lo || hi > r.rows) {
     if (b >= 0) bad_status(c, SPHKV_ST_BAD_LENGTH);
     p.b = -1;
     p.n = 0;
     return p;
   }
-  p.end = c.ends[b];
   if (p.end < 0 || p.end > (int64_t)c.max_blocks * c.page_size || (p.n > p.end && !r.lone)) {
     bad_status(c, SPHKV_ST_BAD_LENGTH);
     p.end = -1;
   }
   return p;
 }
-__device__ __forceinline__ int slot_base(const BlockRows& r, int b, int shift, int extra) {
-  return (min(max(r.cu[b], 0), r.rows) * r.mul >> shift) + extra * b;
+__device__ __forceinline__ BlockPiece even_piece(const sphkv_blocks& c, const BlockRows& r, int slot, int shift, int extra) {
+  const int per = block_slots_even(r.even * r.mul, shift, extra), b = slot / per;
+  return checked_piece(c, r, b, slot - b * per, b * r.even, (b + 1) * r.even, c.ends[b]);
+}
+__device__ __forceinline__ int slot_base(const BlockRows& r, int cu, int b, int shift, int extra) {
+  return (min(max(cu, 0), r.rows) * r.mul >> shift) + extra * b;
 }
 
-// Called by whole warps; every lane gets the answer.
+// Called by whole warps; every lane gets the answer.  Everything that may be the answer is read before it is known which is.
 __device__ __forceinline__ BlockPiece find_piece(const sphkv_blocks& c, const BlockRows& r, int slot, int shift, int extra) {
-  if (r.cu == nullptr) {
-    const int per = block_slots_even(r.even * r.mul, shift, extra), b = slot / per;
-    return checked_piece(c, r, b, slot - b * per, b * r.even, (b + 1) * r.even);
-  }
-  int b = -1, base = 0;
+  if (r.cu == nullptr) return even_piece(c, r, slot, shift, extra);
+  int b = -1, base = 0, lo = 0, hi = 0, end = 0;
   for (int b0 = 0; b0 < c.B; b0 += 32) {
-    const int i = b0 + (threadIdx.x & 31);
-    const int mine = i < c.B ? slot_base(r, i, shift, extra) : 0x7fffffff;
+    const int i = min(b0 + (int)(threadIdx.x & 31), c.B - 1);
+    const bool there = b0 + (int)(threadIdx.x & 31) < c.B;
+    const int from = r.cu[i], to = r.cu[i + 1], e = c.ends[i];
+    const int mine = there ? slot_base(r, from, i, shift, extra) : 0x7fffffff;
     const unsigned below = __ballot_sync(0xffffffffu, mine <= slot);
     if (below == 0) break;
     const int last = 31 - __clz(below);
     b = b0 + last;
     base = __shfl_sync(0xffffffffu, mine, last);
+    lo = __shfl_sync(0xffffffffu, from, last);
+    hi = __shfl_sync(0xffffffffu, to, last);
+    end = __shfl_sync(0xffffffffu, e, last);
     if (last < 31) break;
   }
-  return checked_piece(c, r, b, slot - base, b < 0 ? 0 : r.cu[b], b < 0 ? 0 : r.cu[b + 1]);
+  return checked_piece(c, r, b, slot - base, lo, hi, end);
 }
 // The same by one thread.
 __device__ __forceinline__ BlockPiece find_piece_alone(const sphkv_blocks& c, const BlockRows& r, int slot, int shift, int extra) {
-  if (r.cu == nullptr) {
-    const int per = block_slots_even(r.even * r.mul, shift, extra), b = slot / per;
-    return checked_piece(c, r, b, slot - b * per, b * r.even, (b + 1) * r.even);
+  if (r.cu == nullptr) return even_piece(c, r, slot, shift, extra);
+  int lo = 0;  // the last sequence whose slots begin at or before this one
+  if (c.B <= 32) {  // loads that do not wait for one another
+#pragma unroll 8
+    for (int i = 1; i < c.B; ++i) lo = slot_base(r, r.cu[i], i, shift, extra) <= slot ? i : lo;
+  } else {
+    int hi = c.B;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      (slot_base(r, r.cu[mid], mid, shift, extra) <= slot ? lo : hi) = mid;
+    }
   }
-  int lo = 0, hi = c.B;  // the last sequence whose slots begin at or before this one
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    (slot_base(r, mid, shift, extra) <= slot ? lo : hi) = mid;
-  }
-  return checked_piece(c, r, lo, slot - slot_base(r, lo, shift, extra), r.cu[lo], r.cu[lo + 1]);
+  const int from = r.cu[lo], to = r.cu[lo + 1], end = c.ends[lo];
+  return checked_piece(c, r, lo, slot - slot_base(r, from, lo, shift, extra), from, to, end);
 }
 
 // ---- work dealt evenly: tiles of all slots and heads in one line ------------------------------------------------

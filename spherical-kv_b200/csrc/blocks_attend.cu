@@ -41,6 +41,7 @@ struct AtArgs {
   void* out;
   const uint32_t* prefix;
   const struct AtItem* items;
+  struct AtSpan* spans;  // [workers]: the block that a worker begins and others go on with
   float* parts;  // [workers][2][dh + 2][256]: a worker's first, cut segment and its last
   int q_dtype, out_dtype, Hq, group, slots, workers;
   bool q_vec;
@@ -71,6 +72,11 @@ __device__ __forceinline__ AtItem item_of(const AtArgs& a, int slot) {
   u.tiles = u.first < limit ? (limit + kAtKeys - 1) / kAtKeys - u.kt0 : 0;
   return u;
 }
+struct AtSpan {
+  int n;                      // workers; 0: no such block
+  int row0, r0, rows, head;   // of AtItem
+  int pad[3];
+};
 __global__ void __launch_bounds__(1024) blocks_attend_plan_kernel(const __grid_constant__ AtArgs a, uint32_t* prefix, AtItem* items) {
   griddep_wait();
   plan_tiles(a.slots, prefix, items, [&](int s) { return item_of(a, s); });
@@ -252,6 +258,30 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
     walk.items = items;
     walk.begin(a, blockIdx.x);
   }
+  if (tid == 0) {  // what the second launch joins
+    const Shares shares(prefix[a.slots] * a.c.Hkv, a.workers);
+    AtSpan span = {};
+    if (blockIdx.x < shares.n) {
+      const uint32_t stop = shares.start(blockIdx.x + 1);
+      const int slot = slot_at(prefix, a.slots, (stop - 1) / a.c.Hkv);
+      const AtItem it = items[slot];
+      span.head = (stop - 1 - prefix[slot] * a.c.Hkv) / (uint32_t)it.tiles;
+      const uint32_t p0 = prefix[slot] * a.c.Hkv + span.head * it.tiles, end = p0 + it.tiles;
+      if (p0 >= shares.start(blockIdx.x) && end > stop) span.n = shares.owner(end - 1) - blockIdx.x + 1;
+      span.row0 = it.row0, span.r0 = it.r0, span.rows = it.rows;
+    }
+    a.spans[blockIdx.x] = span;
+  }
+  if (warp < 8) {  // queries that see nothing
+    for (int s = blockIdx.x; s < a.slots; s += gridDim.x) {
+      if (prefix[s + 1] != prefix[s] || tid >= items[s].rows) continue;
+      const AtItem& it = items[s];
+      const float none[16] = {};
+      const int tok = (it.r0 + tid) / a.group, g = it.r0 + tid - tok * a.group;
+      for (int h = 0; h < a.c.Hkv; ++h)
+        for (int d = 0; d < DH; d += 16) store_row16(a.out, a.out_dtype, ((int64_t)(it.row0 + tok) * a.Hq + h * a.group + g) * DH + d, none);
+    }
+  }
   bool lost = false;
   auto wait = [&](int bar, uint32_t n) {  // the n-th phase, from 0
     if (!lost && !mbar_wait(bars + 8 * bar, n & 1)) {
@@ -280,53 +310,63 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
       float m = kNone, l = 0.f, big = 0.f;
       if (cnt > 0) {
         const bool live = flat < u.rows;
-        const int tok = (u.r0 + flat) / a.group, hd = walk.head * a.group + (u.r0 + flat) - tok * a.group;
-        const int64_t dense = (int64_t)u.row0 + tok;
-        const int lim = live ? u.pos0 + tok + 1 : u.lim[t], first = u.first;
+        const int lim = live ? u.pos0 + (u.r0 + flat) / a.group + 1 : u.lim[t], first = u.first;
         const int least = u.pos0 + (u.r0 + 128 * t) / a.group + 1;  // of the tile's rows
         const int seg_key0 = (u.kt0 + walk.from) * kAtKeys;
-        // the row of queries: scaled by a power of two into f16
-        uint4 raw[DH / 8];
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (live ? dense * a.q_row_stride + (int64_t)hd * a.q_head_stride : 0);
-        uint32_t top2 = 0;
+        // The warp's 32 rows of queries, scaled by powers of two into f16: DH / 8 lanes to a row.
+        constexpr int LPR = DH / 8, RPL = 32 / LPR, NQ = 32 / RPL;
+        const bool bf = a.q_dtype == SPHKV_BF16;
+        const uint32_t q_at = base + L::kQ + t * L::kOperand;
+        uint32_t mine = 0;  // the largest magnitude of this thread's row, as bits
+#pragma unroll 1
+        for (int part = 0; part < 2; ++part) {
+          uint4 raw[NQ / 2];
 #pragma unroll
-        for (int i = 0; i < DH / 8; ++i) {
-          raw[i] = make_uint4(0, 0, 0, 0);
-          if (live) {
+          for (int i = 0; i < NQ / 2; ++i) {
+            const int r = 128 * t + 32 * (warp & 3) + RPL * (i + part * (NQ / 2)) + lane / LPR;
+            const int of = u.r0 + min(r, u.rows - 1), tk = of / a.group;  // rows behind the last are its like, and are not written
+            const uint16_t* const src = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(u.row0 + tk) * a.q_row_stride +
+                                        (int64_t)(walk.head * a.group + of - tk * a.group) * a.q_head_stride + 8 * (lane % LPR);
             if (a.q_vec) {
-              raw[i] = *reinterpret_cast<const uint4*>(src + 8 * i);
+              raw[i] = *reinterpret_cast<const uint4*>(src);
             } else {
               uint32_t w[4];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) w[k] = (uint32_t)src[8 * i + 2 * k] | ((uint32_t)src[8 * i + 2 * k + 1] << 16);
+              for (int k = 0; k < 4; ++k) w[k] = (uint32_t)src[2 * k] | ((uint32_t)src[2 * k + 1] << 16);
               raw[i] = make_uint4(w[0], w[1], w[2], w[3]);
             }
           }
-          top2 = __vmaxu2(__vmaxu2(top2, raw[i].x & 0x7fff7fffu), __vmaxu2(raw[i].y & 0x7fff7fffu, __vmaxu2(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu)));
-        }
-        const uint32_t th = max(top2 >> 16, top2 & 0xffffu);
-        const bool bf = a.q_dtype == SPHKV_BF16;
-        const uint16_t th16 = (uint16_t)th;
-        const uint32_t tb = bf ? th << 16 : __float_as_uint(__half2float(*reinterpret_cast<const __half*>(&th16)));
-        int e = (int)(tb >> 23);
-        e = e == 255 ? 140 : max(e, 14);
-        const float sc = __uint_as_float((uint32_t)(267 - e) << 23), f = __uint_as_float((uint32_t)(e - 13) << 23) * a.scale_log2;
-        const uint32_t q_at = base + L::kQ + t * L::kOperand;
 #pragma unroll
-        for (int i = 0; i < DH / 8; ++i) {
-          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-          uint32_t h[4];
+          for (int i = 0; i < NQ / 2; ++i) {
+            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+            uint32_t top = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            float2 x;
-            if (bf)
-              x = make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
-            else
-              x = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-            h[k] = pack_f16x2(x.x * sc, x.y * sc);
+            for (int x = 1; x < LPR; x <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, x));
+            const uint32_t th = max(top >> 16, top & 0xffffu);
+            const uint16_t th16 = (uint16_t)th;
+            const uint32_t tb = bf ? th << 16 : __float_as_uint(__half2float(*reinterpret_cast<const __half*>(&th16)));
+            const int r = RPL * (i + part * (NQ / 2));  // of the warp's
+            const uint32_t theirs = __shfl_sync(0xffffffffu, tb, (lane % RPL) * LPR);
+            if (lane / RPL == r / RPL) mine = theirs;
+            int e = (int)(tb >> 23);
+            e = e == 255 ? 140 : max(e, 14);
+            const float sc = __uint_as_float((uint32_t)(267 - e) << 23);
+            uint32_t h[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float2 x;
+              if (bf)
+                x = make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
+              else
+                x = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+              h[k] = pack_f16x2(x.x * sc, x.y * sc);
+            }
+            sts_u4(q_at + operand_at(32 * (warp & 3) + r + lane / LPR, lane % LPR), h[0], h[1], h[2], h[3]);
           }
-          sts_u4(q_at + operand_at(row, i), h[0], h[1], h[2], h[3]);
         }
+        int e = (int)(mine >> 23);
+        e = e == 255 ? 140 : max(e, 14);
+        const float f = __uint_as_float((uint32_t)(e - 13) << 23) * a.scale_log2;
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + 8 * (kQFull + t));
@@ -703,41 +743,17 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
   if (warp == kAtProducts) tmem_dealloc(tmem, 512);
 }
 
-// CTA (w, y): the block that worker w begins and others go on with, dims 16 y .. of it; and rows of blocks without keys.
+// CTA (w, y): the block that worker w begins and others go on with, dims 16 y .. of it.
 __global__ void __launch_bounds__(256) blocks_attend_merge_kernel(const __grid_constant__ AtArgs a, int dh) {
-  __shared__ uint32_t prefix_smem[kDealt + 1];
-  __shared__ AtItem items_smem[kDealt];
   griddep_launch();
-  const uint32_t* prefix = a.prefix;
-  const AtItem* items = a.items;
-  if (prefix == nullptr) {
-    deal_tiles(a.slots, prefix_smem, items_smem, [&](int s) { return item_of(a, s); });
-    prefix = prefix_smem;
-    items = items_smem;
-  }
   const int flat = threadIdx.x, w = blockIdx.x, d0 = 16 * blockIdx.y;
+  const AtSpan u = a.spans[w];
+  if (u.n == 0 || flat >= u.rows) return;
+  const int n = u.n, head = u.head;
+  const int size = (dh + 2) * kAtRows;
   float o[16];
 #pragma unroll
   for (int c = 0; c < 16; ++c) o[c] = 0.f;
-#pragma unroll 1
-  for (int s = w; s < a.slots; s += gridDim.x) {
-    if (prefix[s + 1] != prefix[s]) continue;
-    const AtItem u = items[s];
-    if (flat >= u.rows) continue;
-    const int tok = (u.r0 + flat) / a.group, g = u.r0 + flat - tok * a.group;
-#pragma unroll 1
-    for (int h = 0; h < a.c.Hkv; ++h) store_row16(a.out, a.out_dtype, ((int64_t)(u.row0 + tok) * a.Hq + h * a.group + g) * dh + d0, o);
-  }
-  const Shares shares(prefix[a.slots] * a.c.Hkv, a.workers);
-  if (w >= (int)shares.n) return;
-  const uint32_t stop = shares.start(w + 1);
-  const int slot = slot_at(prefix, a.slots, (stop - 1) / a.c.Hkv);
-  const AtItem u = items[slot];
-  const int head = (stop - 1 - prefix[slot] * a.c.Hkv) / (uint32_t)u.tiles;
-  const uint32_t p0 = prefix[slot] * a.c.Hkv + head * u.tiles, end = p0 + u.tiles;
-  if (p0 < shares.start(w) || end <= stop || flat >= u.rows) return;
-  const int n = shares.owner(end - 1) - w + 1;
-  const int size = (dh + 2) * kAtRows;
   float top = -INFINITY, sum = 0.f;
   const float* const mine = a.parts + ((int64_t)2 * w + 1) * size + flat;  // the others' are their first places
   auto part = [&](int x) { return x == 0 ? mine : mine + (int64_t)(2 * x - 1) * size; };
@@ -760,7 +776,7 @@ __global__ void __launch_bounds__(256) blocks_attend_merge_kernel(const __grid_c
 static int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 static int64_t at_slots(int64_t rows, int B, int group) { return (rows * group >> 8) + B; }  // at least block_slots()
 static int64_t at_scratch(int64_t rows, int B, int group, int dh, int sms) {
-  return align256((at_slots(rows, B, group) + 1) * 4) + align256(at_slots(rows, B, group) * (int64_t)sizeof(AtItem)) + (int64_t)sms * 2 * (dh + 2) * kAtRows * 4;
+  return align256((at_slots(rows, B, group) + 1) * 4) + align256(at_slots(rows, B, group) * (int64_t)sizeof(AtItem)) + align256(sms * (int64_t)sizeof(AtSpan)) + (int64_t)sms * 2 * (dh + 2) * kAtRows * 4;
 }
 
 template <int DH, bool I8>
@@ -838,7 +854,8 @@ extern "C" int sphkv_blocks_attend(const sphkv_blocks* c, const void* q, int32_t
                 (long long)scratch_bytes, (long long)need);
   SPHKV_REQUIRE(((uintptr_t)scratch & 255) == 0, SPHKV_E_ALIGN, "blocks_attend: scratch needs 256 B");
   uint8_t* const items_at = reinterpret_cast<uint8_t*>(scratch) + align256((at_slots(rows, c->B, group) + 1) * 4);
-  a.parts = reinterpret_cast<float*>(items_at + align256(at_slots(rows, c->B, group) * (int64_t)sizeof(AtItem)));
+  a.spans = reinterpret_cast<AtSpan*>(items_at + align256(at_slots(rows, c->B, group) * (int64_t)sizeof(AtItem)));
+  a.parts = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.spans) + align256(sms * (int64_t)sizeof(AtSpan)));
   if (slots > kDealt) {
     uint32_t* const prefix = reinterpret_cast<uint32_t*>(scratch);
     AtItem* const items = reinterpret_cast<AtItem*>(items_at);
