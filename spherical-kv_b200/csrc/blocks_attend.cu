@@ -23,7 +23,7 @@ namespace sphkv {
 
 constexpr int kAtRows = 256, kAtKeys = 128;
 constexpr int kAtThreads = 640;  // warps 0-3, 4-7: softmax of tile 0, 1; 8-11, 12-15: keys, values to operands; 16: products;
-// 17: scales; 18, 19 have no work
+// 17: scales; 18: what is left over; 19 has no work
 constexpr int kAtProducts = 16;
 // Registers of a thread: at launch; after the softmax has taken what the others gave up.  The file is four quarters, with
 // five warps each (two of softmax, two of codes, one of 16 .. 19), so what goes up has to come down quarter by quarter.
@@ -258,30 +258,6 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
     walk.items = items;
     walk.begin(a, blockIdx.x);
   }
-  if (tid == 0) {  // what the second launch joins
-    const Shares shares(prefix[a.slots] * a.c.Hkv, a.workers);
-    AtSpan span = {};
-    if (blockIdx.x < shares.n) {
-      const uint32_t stop = shares.start(blockIdx.x + 1);
-      const int slot = slot_at(prefix, a.slots, (stop - 1) / a.c.Hkv);
-      const AtItem it = items[slot];
-      span.head = (stop - 1 - prefix[slot] * a.c.Hkv) / (uint32_t)it.tiles;
-      const uint32_t p0 = prefix[slot] * a.c.Hkv + span.head * it.tiles, end = p0 + it.tiles;
-      if (p0 >= shares.start(blockIdx.x) && end > stop) span.n = shares.owner(end - 1) - blockIdx.x + 1;
-      span.row0 = it.row0, span.r0 = it.r0, span.rows = it.rows;
-    }
-    a.spans[blockIdx.x] = span;
-  }
-  if (warp < 8) {  // queries that see nothing
-    for (int s = blockIdx.x; s < a.slots; s += gridDim.x) {
-      if (prefix[s + 1] != prefix[s] || tid >= items[s].rows) continue;
-      const AtItem& it = items[s];
-      const float none[16] = {};
-      const int tok = (it.r0 + tid) / a.group, g = it.r0 + tid - tok * a.group;
-      for (int h = 0; h < a.c.Hkv; ++h)
-        for (int d = 0; d < DH; d += 16) store_row16(a.out, a.out_dtype, ((int64_t)(it.row0 + tok) * a.Hq + h * a.group + g) * DH + d, none);
-    }
-  }
   bool lost = false;
   auto wait = [&](int bar, uint32_t n) {  // the n-th phase, from 0
     if (!lost && !mbar_wait(bars + 8 * bar, n & 1)) {
@@ -315,6 +291,8 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
         const int seg_key0 = (u.kt0 + walk.from) * kAtKeys;
         // The warp's 32 rows of queries, scaled by powers of two into f16: DH / 8 lanes to a row.
         constexpr int LPR = DH / 8, RPL = 32 / LPR, NQ = 32 / RPL;
+        const int tok0 = u.r0 / a.group, rem0 = u.r0 - tok0 * a.group;
+        const uint32_t per_group = 65535u / a.group + 1u;  // x / group = x * per_group >> 16 for x below 2^13
         const bool bf = a.q_dtype == SPHKV_BF16;
         const uint32_t q_at = base + L::kQ + t * L::kOperand;
         uint32_t mine = 0;  // the largest magnitude of this thread's row, as bits
@@ -324,9 +302,9 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
 #pragma unroll
           for (int i = 0; i < NQ / 2; ++i) {
             const int r = 128 * t + 32 * (warp & 3) + RPL * (i + part * (NQ / 2)) + lane / LPR;
-            const int of = u.r0 + min(r, u.rows - 1), tk = of / a.group;  // rows behind the last are its like, and are not written
-            const uint16_t* const src = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(u.row0 + tk) * a.q_row_stride +
-                                        (int64_t)(walk.head * a.group + of - tk * a.group) * a.q_head_stride + 8 * (lane % LPR);
+            const uint32_t of = rem0 + min(r, u.rows - 1), tk = of * per_group >> 16;  // rows behind the last are its like, and are not written
+            const uint16_t* const src = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(u.row0 + tok0 + (int)tk) * a.q_row_stride +
+                                        (int64_t)(walk.head * a.group + (int)(of - tk * a.group)) * a.q_head_stride + 8 * (lane % LPR);
             if (a.q_vec) {
               raw[i] = *reinterpret_cast<const uint4*>(src);
             } else {
@@ -734,6 +712,35 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
           if (lane == 0) mbar_arrive(bars + 8 * (kMFull + (n & 3)));
         }
         lost = __any_sync(0xffffffffu, lost);
+      }
+    } else if (warp == kAtProducts + 2) {
+      // -------------------------------------------------------------- what the second launch joins; queries that see nothing
+      if (lane == 0) {
+        const Shares shares(prefix[a.slots] * a.c.Hkv, a.workers);
+        AtSpan span = {};
+        if (blockIdx.x < shares.n) {
+          const uint32_t stop = shares.start(blockIdx.x + 1);
+          const int slot = slot_at(prefix, a.slots, (stop - 1) / a.c.Hkv);
+          const AtItem it = items[slot];
+          span.head = (stop - 1 - prefix[slot] * a.c.Hkv) / (uint32_t)it.tiles;
+          const uint32_t p0 = prefix[slot] * a.c.Hkv + span.head * it.tiles, end = p0 + it.tiles;
+          if (p0 >= shares.start(blockIdx.x) && end > stop) span.n = shares.owner(end - 1) - blockIdx.x + 1;
+          span.row0 = it.row0, span.r0 = it.r0, span.rows = it.rows;
+        }
+        a.spans[blockIdx.x] = span;
+      }
+#pragma unroll 1
+      for (int s = blockIdx.x; s < a.slots; s += gridDim.x) {
+        if (prefix[s + 1] != prefix[s]) continue;
+        const AtItem it = items[s];
+        const float none[16] = {};
+#pragma unroll 1
+        for (int r = lane; r < it.rows; r += 32) {
+          const int tok = (it.r0 + r) / a.group, g = it.r0 + r - tok * a.group;
+#pragma unroll 1
+          for (int i = 0; i < a.c.Hkv * (DH / 16); ++i)
+            store_row16(a.out, a.out_dtype, ((int64_t)(it.row0 + tok) * a.Hq + i / (DH / 16) * a.group + g) * DH + 16 * (i % (DH / 16)), none);
+        }
       }
     }
   }
