@@ -17,9 +17,11 @@ constexpr int kIoThreads = 256;  // eight warps, each with 16 tokens of one (pag
 constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds |q| < 2^22 to a whole number, ties to even
 
 // ---- nearest 8-bit codes -----------------------------------------------------------------------------------
-// q approximates the quotient to 1.5 ulp (a rounded reciprocal or ratio, one product).  Only where that leaves the nearest code
-// open, within 2^-15 of a whole number's border or 4 ulp of an e4m3 border, is the quotient itself formed in 64 bits,
-// whose error (2^-53) no quotient of two fp32 numbers is closer to a border than, unless it is a tie.
+// q approximates the quotient to 1.5 ulp (a rounded reciprocal or ratio, one product).  Where that leaves the nearest code
+// open, within 2^-15 of a whole number's border or 4 ulp of an e4m3 border, the sign of x - border * s decides, which one fma gives
+// exactly: a border has 8 bits at most, the product 32, and a rounding keeps the sign.  bf16 tokens lie exactly on borders
+// often, since scale and token are quotients of 8-bit numbers: some word of most rows is open, and 64-bit division there was half of
+// the kernel's instructions.
 template <bool I8>
 __device__ uint32_t code_of_double(double q) {
   if constexpr (I8) return (uint32_t)(int)rint(q) & 0xffu;
@@ -31,12 +33,35 @@ __device__ uint32_t code_of_double(double q) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(v));
   return r & 0xffu;
 }
-// codes of x * mul / s.  A function of its own: one in some thousands of its callers' elements comes here, and 64-bit
-// division in line, for every four elements of a lane, took their registers.
+// Codes of x * mul / s for a re-quantised page, where two products would have to be compared: the quotient in 64 bits, whose error
+// (2^-53) no quotient of such numbers is closer to a border than, unless it is a tie.  Not in line: it would take its callers'
+// registers.
 template <bool I8>
 static __device__ __noinline__ uint32_t exact4(float x0, float x1, float x2, float x3, float mul, float s) {
   return code_of_double<I8>((double)x0 * (double)mul / (double)s) | (code_of_double<I8>((double)x1 * (double)mul / (double)s) << 8) |
          (code_of_double<I8>((double)x2 * (double)mul / (double)s) << 16) | (code_of_double<I8>((double)x3 * (double)mul / (double)s) << 24);
+}
+__device__ __forceinline__ uint32_t settled_i8(float q, float x, float s) {
+  const float r = (q + kMagic) - kMagic, e = q - r;
+  if (fabsf(e) <= 0.5f - 0x1p-15f) return (uint32_t)(int)r & 0xffu;
+  const float border = r + copysignf(0.5f, e), d = fmaf(-border, s, x);
+  const int low = (int)(border - 0.5f);
+  return (uint32_t)(low + (d > 0.f || (d == 0.f && (low & 1)))) & 0xffu;
+}
+__device__ __forceinline__ uint32_t settled_e4m3(float q, float x, float s) {
+  const uint32_t sign = (__float_as_uint(x) >> 24) & 0x80u, bits = __float_as_uint(fabsf(q));
+  float border;
+  uint32_t low;  // the code below it
+  if (bits < 0x3c800000u) {
+    const float k = floorf(fabsf(q) * 0x1p9f);
+    border = (k + 0.5f) * 0x1p-9f;
+    low = (uint32_t)(int)k;
+  } else {
+    border = __uint_as_float((bits & 0xfff00000u) | 0x80000u);
+    low = (bits >> 20) - 960u;
+  }
+  const float d = fmaf(-border, s, fabsf(x));
+  return min(low + (d > 0.f || (d == 0.f && (low & 1u))), 126u) | sign;
 }
 __device__ __forceinline__ bool e4m3_border(float q) {
   const uint32_t a = __float_as_uint(q) & 0x7fffffffu;
@@ -44,8 +69,8 @@ __device__ __forceinline__ bool e4m3_border(float q) {
     return a != 0u && fabsf(fabsf(q) * 0x1p9f - floorf(fabsf(q) * 0x1p9f) - 0.5f) < 0x1p-18f;
   return ((a - 0x7fffcu) & 0xfffffu) <= 8u;
 }
-// codes of x * mul / s, by = mul / s rounded (or 1 / s where mul is 1)
-template <bool I8>
+// codes of x / s (NEW: by = 1 / s rounded), or of x * mul / s (by = mul / s rounded)
+template <bool I8, bool NEW>
 __device__ __forceinline__ uint32_t nearest4(const float* x, float by, float mul, float s) {
   const float q[4] = {x[0] * by, x[1] * by, x[2] * by, x[3] * by};
   uint32_t r;
@@ -67,7 +92,14 @@ __device__ __forceinline__ uint32_t nearest4(const float* x, float by, float mul
     r = (uint32_t)lo | ((uint32_t)hi << 16);
     open = e4m3_border(q[0]) | e4m3_border(q[1]) | e4m3_border(q[2]) | e4m3_border(q[3]);
   }
-  if (open) r = exact4<I8>(x[0], x[1], x[2], x[3], mul, s);
+  if (open) {
+    if constexpr (!NEW)
+      r = exact4<I8>(x[0], x[1], x[2], x[3], mul, s);
+    else if constexpr (I8)
+      r = settled_i8(q[0], x[0], s) | (settled_i8(q[1], x[1], s) << 8) | (settled_i8(q[2], x[2], s) << 16) | (settled_i8(q[3], x[3], s) << 24);
+    else
+      r = settled_e4m3(q[0], x[0], s) | (settled_e4m3(q[1], x[1], s) << 8) | (settled_e4m3(q[2], x[2], s) << 16) | (settled_e4m3(q[3], x[3], s) << 24);
+  }
   return r;
 }
 
@@ -261,7 +293,7 @@ __global__ void __launch_bounds__(kIoThreads, sizeof(T) * DH == 512 ? 2 : 4) blo
 #pragma unroll
     for (int k = 0; k < E / 4; ++k) {
       w[k] = 0;
-      if (finite) w[k] = nearest4<I8>(f + 4 * k, inv, 1.f, s);
+      if (finite) w[k] = nearest4<I8, true>(f + 4 * k, inv, 1.f, s);
     }
     uint8_t* to = codes + row * DH + (lane % LPR) * E;
     if constexpr (E == 8)
@@ -281,7 +313,7 @@ __global__ void __launch_bounds__(kIoThreads, sizeof(T) * DH == 512 ? 2 : 4) blo
         float f[4];
         codes_to_f32<I8>(w[k], f);
         w[k] = 0;
-        if (finite) w[k] = nearest4<I8>(f, ratio, s_old, s);
+        if (finite) w[k] = nearest4<I8, false>(f, ratio, s_old, s);
       }
       *reinterpret_cast<uint4*>(codes + row * DH + (lane % OLPR) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
     }
