@@ -12,9 +12,15 @@
 // exact in f16 then, fp32 rows go in as hi + lo (22 bits); weights are hi + lo as well; sums are fp32.  A page's key scale
 // multiplies its logits, its value scale its weights, relative to the largest value scale seen (a power of two, S).
 //
-// Work: 16-token tiles of all (unit, tile) pairs in one line, cut evenly over the workers (a team of warps each); a worker's
-// share of a unit is a segment.  A segment's tiles go round the team's warps; each warp keeps maxima, sums and outputs of
-// its own, with its own ring of tiles that TMA fills, so nothing is shared until the segment's end.
+// Work: 16-token tiles of all (unit, tile) pairs in one line, cut evenly over the CTAs; a CTA's share of a unit is a segment.
+// A segment's tiles go round the CTA's warps; each warp keeps maxima, sums and outputs of its own, with its own ring of
+// tiles that TMA fills (three of 4 KB: 192 KB on their way per SM), so nothing is shared until the segment's end.
+//
+// Measured (graph replay; codes and outputs at the copy rate of 6563 GB/s in brackets): 8 x 32768 tokens x 8 heads of 128 dims 96 us
+// in int8, 101 in e4m3 (82); 1 x 131072 64 (41); 16 x 8192 57 (41: of 128 units on 148 CTAs most CTAs have two segments, and
+// a segment's beginning and end take 3 us each); 1 x 2048 of 64 dims 13, all of it latency: work dealt 1.2 us, addresses and
+// first tiles 1, tiles 0.8, warps joined 0.8, then the second launch.  DRAM 56 % at 8 x 16384 under cold caches, issue slots 56 %
+// (268 instructions a tile), tensor pipe 24 %: with 16 warps neither bandwidth nor issue is full, the warps' own chains are long.
 #include "blocks.cuh"
 
 namespace sphkv {
@@ -51,10 +57,10 @@ struct Bd {
   static constexpr int kItemsOff = kPrefixOff + (kDealt + 4) * 4;
   static constexpr int kStatOff = kItemsOff + kDealt * 32;
   static constexpr int kStat = 5 * 8;                              // floats of a warp: maxima, sums, true maxima, S (8 times), factors
-  static constexpr int kQOff = kStatOff + kBdWarps * (kStat + 8 * 3) * 4;
+  static constexpr int kQOff = kStatOff + (kBdWarps * kStat + 8 * 3) * 4;
   static constexpr int kQRow = 2 * (DH + 8);                       // bytes of a row of queries in f16
-  static constexpr int kQ = 2 * 8 * kQRow + 32;                    // of a team: hi, lo, factors
-  static constexpr int kBarOff = kQOff + 2 * kQ;
+  static constexpr int kQ = 2 * 8 * kQRow + 32;                    // hi, lo, factors
+  static constexpr int kBarOff = kQOff + kQ;
   static constexpr int kSmem = kBarOff + kBdWarps * kStages * 8 + 1024;
 };
 static_assert(Bd<128>::kSmem <= 232448 && Bd<64>::kSmem <= 232448, "shared memory of a CTA");
@@ -120,24 +126,22 @@ __device__ __forceinline__ void pair_codes(uint32_t k0, uint32_t k1, uint32_t (&
   codes_to_f16<I8>(hi, d[2], d[3]);
 }
 
-// WARPS: warps of a team
-template <int DH, bool I8, bool QLO, int WARPS>
+template <int DH, bool I8, bool QLO>
 __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __grid_constant__ BdArgs a) {
   using L = Bd<DH>;
   constexpr int S = L::kStages, KS = DH / 16, GD = L::kGroupDims, W4 = GD / 4;  // words of a value row per lane
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j = lane & 3;
-  const int team = warp / WARPS, tw = warp % WARPS;
+  constexpr int WARPS = kBdWarps;
   const uint32_t ring = smem_u32(smem) + warp * L::kRing;
   const uint32_t bars = smem_u32(smem) + L::kBarOff + warp * S * 8;
-  float* const stats = reinterpret_cast<float*>(smem + L::kStatOff) + team * WARPS * L::kStat;  // of the team
-  float* const cols_of = reinterpret_cast<float*>(smem + L::kStatOff) + kBdWarps * L::kStat + team * WARPS * 24;  // max, sum, true max
-  float* const joined = reinterpret_cast<float*>(smem + team * WARPS * L::kRing);  // a warp's outputs: in its ring's place
+  float* const stats = reinterpret_cast<float*>(smem + L::kStatOff);
+  float* const cols_of = stats + WARPS * L::kStat;  // of a query row: maximum, sum, true maximum
+  float* const joined = reinterpret_cast<float*>(smem);  // a warp's outputs: in its ring's place
   constexpr int JOIN = L::kRing / 4;
-  static_assert(kBdWarps / WARPS <= 2, "places for queries");
-  const uint32_t q_at = smem_u32(smem) + L::kQOff + team * L::kQ;  // the segment's queries
-  float* const q_factor = reinterpret_cast<float*>(smem + L::kQOff + team * L::kQ + 2 * 8 * L::kQRow);
+  const uint32_t q_at = smem_u32(smem) + L::kQOff;  // the segment's queries
+  float* const q_factor = reinterpret_cast<float*>(smem + L::kQOff + 2 * 8 * L::kQRow);
   if (lane == 0) {
 #pragma unroll
     for (int s = 0; s < S; ++s) mbar_init(bars + 8 * s, 1);
@@ -158,18 +162,13 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
   for (int s = blockIdx.x; s < a.slots; s += gridDim.x)  // units without keys: zeros, by the second launch
     if (items[s].tiles == 0 && tid < a.c.Hkv)
       for (int h = tid; h < a.c.Hkv; h += kBdThreads) a.spans[s * a.c.Hkv + h] = make_int4(0, 0, items[s].row0, items[s].tokens);
-  const uint32_t worker = blockIdx.x * (kBdWarps / WARPS) + team;
+  const uint32_t worker = blockIdx.x;
   uint32_t pos = worker < shares.n ? shares.start(worker) : 0;
   const uint32_t stop = worker < shares.n ? shares.start(worker + 1) : 0;
   const uint64_t policy = policy_evict_first();
   const int shift = 31 - __clz(a.c.page_size);
   uint32_t issued = 0, taken = 0;  // tiles since the kernel began: stage = n % S, the barrier's phase n / S
   bool lost = false;
-
-  auto team_sync = [&] {
-    if constexpr (WARPS > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(32 * WARPS) : "memory");
-    else __syncwarp();
-  };
 
   while (pos < stop) {
     // ---- the segment ----
@@ -179,7 +178,7 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
     const int head = in_slot / (uint32_t)u.tiles, from = in_slot - head * u.tiles;
     const int count = min((uint32_t)(u.tiles - from), stop - pos);
     const int unit = slot * a.c.Hkv + head;
-    if (from == 0 && tw == 0 && lane == 0)
+    if (from == 0 && tid == 0)
       a.spans[unit] = make_int4(worker, shares.owner(pos + u.tiles - 1) - worker + 1, u.row0, u.tokens);
     pos += count;
     const int cols = u.tokens * a.group;
@@ -187,15 +186,15 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
     // ---- queries, a warp to a row: asked for here, used behind the tiles' addresses ----
     constexpr int QD = DH / 32;  // dims of a lane
     float qv[QD];
-    const bool q_row = tw < cols;
+    const bool q_row = warp < cols;
     if (q_row) {
-      const int tok = tw / a.group, h = head * a.group + tw - tok * a.group;
+      const int tok = warp / a.group, h = head * a.group + warp - tok * a.group;
       const int64_t at = (int64_t)(u.row0 + tok) * a.q_row_stride + (int64_t)h * a.q_head_stride + QD * lane;
 #pragma unroll
       for (int i = 0; i < QD; ++i) qv[i] = load_as_float(a.q, a.q_dtype, at + i);
     }
     // ---- where this warp's tiles lie: lane i holds tile 32 r + i of them ----
-    const int mine = tw < count ? (count - tw + WARPS - 1) / WARPS : 0;
+    const int mine = warp < count ? (count - warp + WARPS - 1) / WARPS : 0;
     const int32_t* table = a.c.block_table + (int64_t)u.b * a.c.max_blocks;
     struct Meta {
       int row;  // of the pools; negative: a bad table entry
@@ -204,7 +203,7 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
     auto lookup = [&](int k) {
       Meta m = {0, 0.f, 0.f};
       if (k >= mine) return m;
-      const int tok = (u.tile0 + from + tw + k * WARPS) << 4;
+      const int tok = (u.tile0 + from + warp + k * WARPS) << 4;
       const int page = table[tok >> shift];
       if (page < 0 || page >= a.c.n_pages) {
         bad_status(a.c, SPHKV_ST_BAD_BLOCK);
@@ -232,8 +231,7 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
       for (int k = 0; k < min(S, mine); ++k) issue(k, 0);
 
     // ---- the rows in f16, scaled by powers of two; then lane 4g + j takes dims DH/4 j .. of row g ----
-    static_assert(WARPS >= 8, "a warp to a row");
-    if (tw < 8) {
+    if (warp < 8) {
       float top = 0.f;
 #pragma unroll
       for (int i = 0; i < QD; ++i) {
@@ -244,17 +242,17 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
       int e = (int)(bits >> 23);
       e = e == 255 ? 140 : max(e, 14);  // infinities and NaN go in as they are
       const float up = __uint_as_float((uint32_t)(267 - e) << 23);
-      if (lane == 0) q_factor[tw] = __uint_as_float((uint32_t)(e - 13) << 23) * a.scale_log2;
+      if (lane == 0) q_factor[warp] = __uint_as_float((uint32_t)(e - 13) << 23) * a.scale_log2;
 #pragma unroll
       for (int i = 0; i < QD; i += 2) {
         uint32_t hi, lo;
         split_f16x2(qv[i] * up, qv[i + 1] * up, hi, lo);
-        const uint32_t to = q_at + tw * L::kQRow + 2 * (QD * lane + i);
+        const uint32_t to = q_at + warp * L::kQRow + 2 * (QD * lane + i);
         asm volatile("st.shared.u32 [%0], %1;" ::"r"(to), "r"(hi) : "memory");
         if constexpr (QLO) asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + 8 * L::kQRow), "r"(lo) : "memory");
       }
     }
-    team_sync();
+    __syncthreads();
     uint32_t qh[KS][2], ql[QLO ? KS : 1][2];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -329,7 +327,7 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
 
       const float e0 = f0 * ks, e1 = f1 * ks;
       float x[4] = {(c[0][0] + c[1][0]) * e0, (c[0][1] + c[1][1]) * e1, (c[0][2] + c[1][2]) * e0, (c[0][3] + c[1][3]) * e1};
-      const int tok = (u.tile0 + from + tw + k * WARPS) << 4;
+      const int tok = (u.tile0 + from + warp + k * WARPS) << 4;
       const bool edge = row < 0 || tok < u.first || tok + 16 > least;
       bool seen[4] = {true, true, true, true};
       if (edge) {  // some keys of the tile are not seen by every row, or by none
@@ -406,7 +404,7 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
       }
     }
 
-    // ---- the team's warps are joined ----
+    // ---- the warps are joined ----
     {
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) {
@@ -415,22 +413,22 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
         t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
         t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
       }
-      float* const st = stats + tw * L::kStat;
+      float* const st = stats + warp * L::kStat;
       if (g == 0) {
         st[2 * j] = m0, st[2 * j + 1] = m1;
         st[8 + 2 * j] = l0, st[9 + 2 * j] = l1;
         st[16 + 2 * j] = t0, st[17 + 2 * j] = t1;
         st[24 + 2 * j] = st[25 + 2 * j] = big;
       }
-      float* const mine_at = joined + tw * JOIN + g * (GD + 2);  // this warp has taken every tile of its own
+      float* const mine_at = joined + warp * JOIN + g * (GD + 2);  // this warp has taken every tile of its own
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
         *reinterpret_cast<float2*>(mine_at + 2 * j * L::kCol + 2 * i) = make_float2(acc[i][0], acc[i][2]);
         *reinterpret_cast<float2*>(mine_at + (2 * j + 1) * L::kCol + 2 * i) = make_float2(acc[i][1], acc[i][3]);
       }
-      team_sync();
+      __syncthreads();
       const int n_warps = min(count, WARPS);
-      for (int col = tw; col < cols; col += WARPS) {  // a warp to a query row: lane w looks after warp w
+      for (int col = warp; col < cols; col += WARPS) {  // a warp to a query row: lane w looks after warp w
         const float* const of = stats + (lane % WARPS) * L::kStat + col;
         const bool have = lane < n_warps;
         float top = have ? of[0] : kNone, true_top = have ? of[16] : -INFINITY;
@@ -446,10 +444,10 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
         if (have) stats[lane * L::kStat + 32 + col] = f * (of[24] * (1.f / kWeight));
         if (lane == 0) cols_of[3 * col] = top, cols_of[3 * col + 1] = sum, cols_of[3 * col + 2] = true_top;
       }
-      team_sync();
+      __syncthreads();
       const bool whole = count == u.tiles;
       float* const part = a.parts + (int64_t)(worker + unit) * 8 * (DH + 2);
-      for (int i = tw * 32 + lane; i < cols * DH; i += WARPS * 32) {
+      for (int i = tid; i < cols * DH; i += kBdThreads) {
         const int col = i / DH, d = i - col * DH;
         const float* const from = joined + col * L::kCol + (d / GD) * (GD + 2) + d % GD;
         float v = 0.f;
@@ -472,9 +470,9 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
           if (d == 0) part[col * (DH + 2)] = true_top, part[col * (DH + 2) + 1] = sum * to_true;
         }
       }
-      team_sync();
+      __syncthreads();
       fence_async_smem();  // the next segment's copies come in through the other proxy
-      team_sync();
+      __syncthreads();
     }
   }
   if (lost) {  // copies that are still on their way
@@ -547,7 +545,7 @@ static int64_t bd_scratch(int64_t slots, int Hkv, int dh, int workers) {
 template <int DH, bool I8, bool QLO>
 static int launch_bd(const BdArgs& a, int ctas, cudaStream_t st) {
   static SmemOptIn opt_in;
-  auto kern = blocks_decode_kernel<DH, I8, QLO, kBdWarps>;
+  auto kern = blocks_decode_kernel<DH, I8, QLO>;
   if (int rc = ensure_dynamic_smem(opt_in, (const void*)kern, Bd<DH>::kSmem, "blocks_decode")) return rc;
   (void)launch_overlapped(kern, dim3(ctas), dim3(kBdThreads), Bd<DH>::kSmem, st, a);
   return check_launch("blocks_decode_kernel");

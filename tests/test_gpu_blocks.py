@@ -258,6 +258,77 @@ def test_attend(pkg, store, N, dh, Hq, H, dtype):
     pkg.check_status(cache)
 
 
+@pytest.mark.parametrize("store,N,dh,Hq,H", [(I8, 16, 128, 16, 4), (E4M3, 64, 64, 8, 2)])
+def test_references_move(pkg, store, N, dh, Hq, H):
+    """Many key tiles a worker, logits that grow along the sequence and values over twenty powers of two: maxima and the value scales'
+    reference move all the time, in front of every part of a tile."""
+    ctx, n = 9001, 150
+    cache = _cache(pkg, [ctx], H, N, dh, store, 61)
+    ramp = torch.linspace(0.05, 3.0, ctx)[:, None, None]
+    k, v = _random((ctx, H, dh), 5, torch.float32) * ramp, _random((ctx, H, dh), 6, torch.float32) * torch.exp2(20 * torch.linspace(-1, 0, ctx))[:, None, None]
+    pkg.append_blocks(cache, k.to(DEV), v.to(DEV), cu_new=_cu([ctx]))
+    sides, table = _sides(cache), cache.block_table.cpu()
+    kk, vv = (s.rows(table[0], 0, ctx) for s in sides)
+    q = _random((n, Hq, dh), 3, torch.float16)
+    want, _, _, off, size, _ = orc.attend(q, kk, vv, 0, list(range(ctx - n, ctx)), 1 / math.sqrt(dh))
+    # a weight below 2^-14 is off by up to 2^-25 in f16, of weights up to 2^14 (the reference's slack 2^8, times 2^6) and as low as 2^6: the sum
+    # of 2^-31 |v| over keys, relative to the largest scale
+    tiny = ctx * 2.0 ** -31 * float(vv.abs().max())
+    got = pkg.attend_blocks(q.to(DEV), cache, cu_new=_cu([n]), out_dtype=torch.float32)
+    _check(got, want, off + torch.finfo(torch.float16).eps / 2 * size + tiny, torch.float32)
+    got = pkg.decode_blocks(q[-1:].to(DEV), cache, out_dtype=torch.float32)
+    _check(got, want[-1:], off[-1:] + tiny, torch.float32)
+    # the other way round: the largest come first
+    cache = _cache(pkg, [ctx], H, N, dh, store, 61)
+    pkg.append_blocks(cache, k.flip(0).to(DEV), v.flip(0).to(DEV), cu_new=_cu([ctx]))
+    sides = _sides(cache)
+    kk, vv = (s.rows(table[0], 0, ctx) for s in sides)
+    want, _, _, off, size, _ = orc.attend(q, kk, vv, 0, list(range(ctx - n, ctx)), 1 / math.sqrt(dh))
+    got = pkg.attend_blocks(q.to(DEV), cache, cu_new=_cu([n]), out_dtype=torch.float32)
+    _check(got, want, off + torch.finfo(torch.float16).eps / 2 * size + tiny, torch.float32)
+    pkg.check_status(cache)
+
+
+def test_attend_shapes(pkg):
+    """The even form, one token and the decode kernel's few, strided queries, outputs of other types, more blocks of queries than a CTA
+    deals by itself, and a recorded call."""
+    H, N, dh, Hq = 2, 32, 128, 8
+    lens = [90, 200, 33]
+    cache = _filled(pkg, lens, H, N, dh, I8, 71)
+    sides, table = _sides(cache), cache.block_table.cpu()
+    for n in (1, 2, 3, 20):
+        base = _random((3, n, Hq + 2, dh + 8), 3, torch.bfloat16).to(DEV)
+        for q in (base[:, :, :Hq, :dh], base[:, :, 1:Hq + 1, 3:dh + 3]):
+            for out_dtype in (torch.bfloat16, torch.float32):
+                out = pkg.attend_blocks(q, cache, out_dtype=out_dtype)
+                assert out.shape == (3, n, Hq, dh) and out.dtype == out_dtype
+                for b in range(3):
+                    kk, vv = (s.rows(table[b], 0, lens[b]) for s in sides)
+                    want, _, _, off, size, _ = orc.attend(q[b].cpu(), kk, vv, 0, list(range(lens[b] - n, lens[b])), 1 / math.sqrt(dh))
+                    _check(out[b], want, off + torch.finfo(torch.float16).eps / 2 * size, out_dtype)
+    q = _random((3, 20, Hq, dh), 3, torch.bfloat16).to(DEV)
+    want = pkg.attend_blocks(q, cache)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = pkg.attend_blocks(q, cache)
+    for _ in range(2):
+        out.zero_()
+        gr.replay()
+        assert torch.equal(out, want)
+    many = [40 + b % 3 for b in range(150)]
+    cache = _filled(pkg, many, 1, 16, 64, E4M3, 81)
+    sides, table = _sides(cache), cache.block_table.cpu()
+    q = _random((sum(many), 4, 64), 3, torch.float16)
+    out = pkg.attend_blocks(q.to(DEV), cache, cu_new=_cu(many))
+    for b in range(0, 150, 13):
+        kk, vv = (s.rows(table[b], 0, many[b]) for s in sides)
+        at = sum(many[:b])
+        want, _, _, off, size, _ = orc.attend(q[at:at + many[b]], kk, vv, 0, list(range(many[b])), 0.125)
+        _check(out[at:at + many[b]], want, off + torch.finfo(torch.float16).eps / 2 * size, torch.float16)
+    pkg.check_status(cache)
+
+
 def test_padding_bad_tables_and_lengths(pkg):
     H, N, dh = 2, 16, 128
     cache = _filled(pkg, [40, 40, 40, 40], H, N, dh, I8, 61)
