@@ -433,7 +433,8 @@ typedef struct sphkv_blocks {
  * max(scale, scale') and its codes are re-quantised where that is larger.  Codes are the nearest
  * to x / scale' (the exact quotient, ties to even).  A scale below 2^-126 becomes 0 with codes 0.
  * Where a new x is not finite, its page, head and side get an infinite or NaN scale and codes 0:
- * they read back as NaN.  Pages that receive tokens must not be shared by two sequences. */
+ * they read back as NaN.  A page that receives tokens belongs to one sequence, and stands once in its
+ * row of the table. */
 int sphkv_blocks_append(const sphkv_blocks* c, const void* k, const void* v, int32_t dtype, int64_t k_row_stride,
                         int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride, const int32_t* cu,
                         int64_t rows, void* stream);
@@ -448,8 +449,9 @@ int sphkv_blocks_read(const sphkv_blocks* c, void* k_out, void* v_out, int32_t d
  * of out_dtype and out_partial f32 [B][Hq][dh + 2] = (max, sum, acc) as sphkv_decode_paged writes it
  * (optional; sphkv_merge_partials takes both together).  A sequence without keys gets zeros and
  * (-inf, 0, 0).  Hq / Hkv <= SPHKV_MAX_GQA.  scratch: sphkv_blocks_decode_scratch_bytes() bytes, 256-aligned, free
- * for other use when the call's kernels are done.  Two launches; the first may become resident while the
- * kernel before it in the stream still runs, and waits for it before it reads or writes memory. */
+ * for other use when the call's kernels are done.  Two launches (three for more than 128 sequences); the first may
+ * become resident while the kernel before it in the stream still runs, and waits for it before it reads
+ * or writes memory. */
 int64_t sphkv_blocks_decode_scratch_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t dh);
 int sphkv_blocks_decode(const sphkv_blocks* c, const void* q, int32_t q_dtype, int64_t q_row_stride,
                         int64_t q_head_stride, const int32_t* first, void* out, int32_t out_dtype,

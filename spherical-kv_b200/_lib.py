@@ -94,7 +94,6 @@ class Blocks(C.Structure):
         ("n_pages", C.c_int32), ("Hkv", C.c_int32), ("page_size", C.c_int32), ("dh", C.c_int32), ("B", C.c_int32),
         ("max_blocks", C.c_int32), ("store", C.c_int32),
     ]
-    packer = struct.Struct("@7P7i4x")
 
 
 # name -> (restype, argtypes); every symbol include/sphkv.h declares
@@ -135,15 +134,14 @@ SIGNATURES = {
                                          C.c_int32] + [C.c_void_p] * 4 + [C.c_int32] * 3 + [C.c_void_p]),
     "sphkv_kmeans_assign": (C.c_int, [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_int32] + [C.c_void_p] * 5),
     "sphkv_pool_append_step": (C.c_int, [C.c_void_p] * 12 + [C.c_int32] * 10 + [C.c_void_p]),
-    # the cache struct of the block functions goes in as its packed bytes
-    "sphkv_blocks_append": (C.c_int, [C.c_char_p, C.c_void_p, C.c_void_p, C.c_int32] + [C.c_int64] * 4 +
+    "sphkv_blocks_append": (C.c_int, [C.POINTER(Blocks), C.c_void_p, C.c_void_p, C.c_int32] + [C.c_int64] * 4 +
                             [C.c_void_p, C.c_int64, C.c_void_p]),
-    "sphkv_blocks_read": (C.c_int, [C.c_char_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p]),
+    "sphkv_blocks_read": (C.c_int, [C.POINTER(Blocks), C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p]),
     "sphkv_blocks_decode_scratch_bytes": (C.c_int64, [C.c_int32] * 4),
-    "sphkv_blocks_decode": (C.c_int, [C.c_char_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p,
+    "sphkv_blocks_decode": (C.c_int, [C.POINTER(Blocks), C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p,
                                       C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_float, C.c_void_p]),
     "sphkv_blocks_attend_scratch_bytes": (C.c_int64, [C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_int32]),
-    "sphkv_blocks_attend": (C.c_int, [C.c_char_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_void_p, C.c_int64,
+    "sphkv_blocks_attend": (C.c_int, [C.POINTER(Blocks), C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_void_p, C.c_int64,
                                       C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_int32, C.c_float,
                                       C.c_void_p]),
 }

@@ -18,7 +18,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-from dataclasses import dataclass, field
+from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
@@ -44,7 +44,6 @@ class BlockCache:
     block_table: torch.Tensor  # i32 [B, max_blocks]: page of tokens page_size * i ..; entries past a sequence's end: anything
     seq_lens: torch.Tensor     # i32 [B]: tokens held, those of the present step among them
     status: Optional[torch.Tensor] = None
-    extra: dict = field(default_factory=dict)
 
     def __post_init__(self):
         if self.status is None and self.k_codes.is_cuda:
@@ -128,7 +127,7 @@ def append_blocks(cache: BlockCache, k: torch.Tensor, v: torch.Tensor, cu_new: O
     they come (slices of a fused projection).  seq_lens counts the new tokens already.  A page keeps one scale per head and
     side, max |x| / 127 (e4m3: / 448) of all it was given: where new tokens raise it, the page's earlier tokens of the sequence are
     re-quantised.  Codes are the nearest to x / scale, ties to even.  An infinity or NaN makes its page, head and side read
-    back as NaN.  Two sequences must not append to the same page."""
+    back as NaN.  A page that is appended to belongs to one sequence, and stands once in its row of the table."""
     _call("append", cache, cache.seq_lens, k, v, cu_new)
 
 

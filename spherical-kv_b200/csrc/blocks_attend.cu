@@ -1,22 +1,32 @@
 // Causal attention of many queries a sequence over the 8-bit block cache (a prompt's chunk, drafted tokens).
 //
 // The query rows of one KV head (tokens x group heads, flat) are cut into blocks of 256, two tensor-core tiles of 128; the
-// keys into tiles of 128.  A CTA walks a block's key tiles with four kinds of warps:
-//   4 warps  fetch codes a tile ahead into registers and turn them into f16 operands in shared memory (codes are exact in
-//            f16; scales stay apart), keys and values double buffered;
-//   1 warp   issues the products: logits S_t = Q_t K^T and outputs O_t += P_t V, for the two tiles t in turn, so that the tensor
-//            cores work on one tile while the other's softmax runs;
-//   8 warps  softmax, a thread to a query row: S from tensor memory, a page's key scale times the row's factor as one
-//            multiplier for its 16 keys and up, weights 2^6 p v / S_v in f16 back over S as the next product's operand.
-//            The page's value scale is part of the exponent, so it costs nothing per element; the sum of p takes it out
-//            again once for 16 keys.  A row's reference maximum moves only when a logit passes it by 2^8; O is then
-//            rescaled in place (every earlier product is complete: S_t(k) is issued behind P_t V(k - 1)).
+// keys into tiles of 128.  A CTA walks a block's key tiles with five kinds of warps:
+//   4 + 4 warps  fetch a tile's key or value codes into registers, a tile ahead, and turn them into f16 operands in shared memory
+//            (codes are exact in f16; scales stay apart), double buffered;
+//   1 warp   fetches the tile's scales;
+//   1 warp   issues the products: logits S_t = Q_t K^T and outputs O_t += P_t V (tcgen05, P from tensor memory), for the two
+//            row tiles t in turn, so that the tensor cores work on one while the other's softmax runs;
+//   8 warps  softmax, a thread to a query row, 32 keys at a time: S from tensor memory, a page's key scale times the row's
+//            factor as one multiplier for its 16 keys and up, weights 2^6 p v / S_v in f16 back over S as the next product's
+//            operand.  The page's value scale is part of the exponent, so it costs nothing per element; the sum of p takes
+//            it out again once for 16 keys.  A row's reference maximum moves only when a logit passes it by 2^8; O and the
+//            tile's weights so far are then rescaled in place (every earlier product is complete: S_t(k) is issued behind
+//            P_t V(k - 1)).
 // Q rows are scaled by a power of two as in the decode kernel: bf16 and f16 queries are exact in f16.  Weights have f16's 11
-// bits, sums are fp32.
+// bits, sums are fp32.  A quarter of the exponentials goes through a polynomial on the fma pipe.
 //
 // Work: (block, head, key tile) in one line, cut evenly over the CTAs; a block that two or more CTAs share is joined by a
-// second launch.  What bounds it: the exponentials (16 a cycle and SM, 2048 cycles for 256 rows x 128 keys) and, as much, the
-// products (2048 cycles at the nominal rate).
+// second launch.
+//
+// Measured: 2048 queries x 32 heads on 32768 tokens 1.29 ms in a graph, 0.83 PFLOP/s, half of what cuBLAS reaches in a burst; five
+// pieces of 301 .. 61 queries on up to 6001 tokens 109 us.  A pair of tiles (256 x 128) takes 5900 cycles.  The floor is 2048 for
+// the products (their operands ask for 96 of shared memory's 128 bytes a cycle, the conversion for another 32) and 2048 for the
+// exponentials; what is missing is in the chain S -> softmax -> P V -> S of each tile: a warp needs 620 cycles for 64 weights where
+// the exponential unit is busy for 550, and in the kernel, with two more warps on each scheduler and tensor memory shared
+// with the products, 1100 to 1500; a wait for a barrier costs 70 to 130 cycles even where there is nothing to wait for.
+// Tensor pipe 35 %, issue slots 54 %, no local memory.  Local memory is what the arrangement of the roles avoids: with all of L1
+// taken by shared memory a spilled word comes from L2 (1.96 ms with 512 threads and the tile's 128 logits in registers).
 #include "blocks.cuh"
 
 namespace sphkv {
@@ -827,11 +837,11 @@ extern "C" int sphkv_blocks_attend(const sphkv_blocks* c, const void* q, int32_t
   a.c = *c;
   if (int rc = block_rows(a.r, c, cu, rows, "blocks_attend")) return rc;
   SPHKV_REQUIRE(rows <= 0x7ffffff, SPHKV_E_LIMIT, "blocks_attend: rows=%lld (max 2^27 - 1)", (long long)rows);
-  SPHKV_REQUIRE(rows == 0 || q != nullptr, SPHKV_E_ARG, "blocks_attend: q is NULL");
+  if (rows == 0) return 0;  // tensors without elements have no address
+  SPHKV_REQUIRE(q != nullptr, SPHKV_E_ARG, "blocks_attend: q is NULL");
   if (int rc = check_queries(*c, q, q_dtype, out, nullptr, out_dtype, Hq, "blocks_attend")) return rc;
   SPHKV_REQUIRE(q_dtype != SPHKV_F32, SPHKV_E_DTYPE, "blocks_attend: q_dtype=%d (16-bit types)", q_dtype);
   SPHKV_REQUIRE(((uintptr_t)out & 15) == 0, SPHKV_E_ALIGN, "blocks_attend: out needs 16 B");
-  if (rows == 0) return 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int group = Hq / c->Hkv, sms = sm_count_current_device();
   if (sms <= 0) return sms;

@@ -115,11 +115,15 @@ struct Args {  // in the order of the Python side
   double real() { return PyFloat_AsDouble(next()); }
   template <typename F>
   F function() { return reinterpret_cast<F>(static_cast<intptr_t>(integer())); }
-  const at::Tensor* tensor() {  // NULL: None, or no tensor
+  bool wrong = false;          // something that is neither a tensor nor None stood for a tensor
+  const at::Tensor* tensor() {  // NULL: None
     PyObject* o = next();
-    return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr;
+    if (THPVariable_Check(o)) return &THPVariable_Unpack(o);
+    wrong |= o != Py_None;
+    return nullptr;
   }
 };
+const char* const kNoTensor = "an argument that is to be a tensor is something else";
 
 int type_of(at::ScalarType t) {
   return t == at::kFloat ? SPHKV_F32 : t == at::kBFloat16 ? SPHKV_BF16 : t == at::kHalf ? SPHKV_F16 : -1;
@@ -218,6 +222,7 @@ PyObject* blocks_append(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   if (!v.read(args)) return refused(v.why);
   const at::Tensor *k = args.tensor(), *val = args.tensor(), *cu = args.tensor();
   const int32_t* at;
+  if (args.wrong) return refused(kNoTensor);
   if (!v.dense(k, cu == nullptr, v.c.Hkv, "k", rows, kr, kh)) return refused(v.why);
   if (val == nullptr || val->sizes() != k->sizes() || val->scalar_type() != k->scalar_type()) return refused("v: expected k's shape and type");
   if (!v.dense(val, cu == nullptr, v.c.Hkv, "v", rows, vr, vh) || !v.i32(cu, (int64_t)v.c.B + 1, "cu_new", at)) return refused(v.why);
@@ -247,6 +252,7 @@ PyObject* blocks_read(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   const int type = (int)args.integer();
   const at::Tensor *ko = args.tensor(), *vo = args.tensor();
   if (PyErr_Occurred()) return nullptr;
+  if (args.wrong) return refused(kNoTensor);
   const int32_t* at;
   if (!v.i32(cu, (int64_t)v.c.B + 1, "cu_rows", at)) return refused(v.why);
   std::array<int64_t, 4> even = {v.c.B, each, v.c.Hkv, v.c.dh};
@@ -289,6 +295,7 @@ PyObject* blocks_decode(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   const at::Tensor *given = args.tensor(), *partial = args.tensor();
   const bool want = args.integer() != 0;
   if (PyErr_Occurred()) return nullptr;
+  if (args.wrong) return refused(kNoTensor);
   if (q == nullptr || q->device() != v.dev || type_of(q->scalar_type()) < 0 || q->dim() != 3 || q->size(0) != v.c.B || q->size(2) != v.c.dh ||
       q->stride(2) != 1)
     return refused("q: expected [B, Hq, dh] of float32, bfloat16 or float16 on the cache's device, elements of a head contiguous");
@@ -337,6 +344,7 @@ PyObject* blocks_attend(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   int type = (int)args.integer();
   const at::Tensor* given = args.tensor();
   if (PyErr_Occurred()) return nullptr;
+  if (args.wrong) return refused(kNoTensor);
   int64_t rows, row, head;
   if (!v.dense(q, cu == nullptr, 0, "q", rows, row, head)) return refused(v.why);
   if (q->scalar_type() == at::kFloat) return refused("attend_blocks: q is bfloat16 or float16");

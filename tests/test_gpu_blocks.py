@@ -372,6 +372,41 @@ def test_padding_bad_tables_and_lengths(pkg):
     assert out.isfinite().all()
 
 
+def test_refusals(pkg):
+    H, N, dh = 2, 16, 128
+    cache = _filled(pkg, [40, 20], H, N, dh, I8, 61)
+    q, k = _random((2, 4, dh), 3, torch.bfloat16).to(DEV), _random((2, 1, H, dh), 3, torch.bfloat16).to(DEV)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    bad = [lambda: pkg.decode_blocks(q, cache, first=[0, 0]), lambda: pkg.decode_blocks(q, cache, first=torch.zeros(2, device=DEV)),
+           lambda: pkg.decode_blocks(q, cache, first=torch.zeros(3, **i32)), lambda: pkg.decode_blocks(q, cache, first=torch.zeros(2, dtype=torch.int32)),
+           lambda: pkg.decode_blocks(q[:1], cache), lambda: pkg.decode_blocks(q[..., :64], cache), lambda: pkg.decode_blocks(q.double(), cache),
+           lambda: pkg.decode_blocks(q.transpose(1, 2).contiguous().transpose(1, 2), cache), lambda: pkg.decode_blocks(q[:, :3], cache),
+           lambda: pkg.decode_blocks(torch.cat([q] * 5, 1), cache), lambda: pkg.decode_blocks(q, cache, out=q[:, :2]),
+           lambda: pkg.decode_blocks(q, cache, out_dtype=torch.int8), lambda: pkg.decode_blocks(q, cache, out_partial=torch.zeros(2, 4, dh, device=DEV)),
+           lambda: pkg.decode_blocks(q, cache, want_out=False), lambda: pkg.decode_blocks(q.cpu(), cache),
+           lambda: pkg.append_blocks(cache, k, k.float()), lambda: pkg.append_blocks(cache, k[:, 0], k[:, 0]), lambda: pkg.append_blocks(cache, k[:, :, :1], k[:, :, :1]),
+           lambda: pkg.append_blocks(cache, k[:, 0], k[:, 0], cu_new=torch.zeros(2, **i32)), lambda: pkg.append_blocks(cache, k, [1, 2]),
+           lambda: pkg.append_blocks(cache, k.expand(2, 3, H, dh)[:, ::2].contiguous()[:, :1].expand(2, 2, H, dh), k.expand(2, 2, H, dh)),
+           lambda: pkg.read_blocks(cache), lambda: pkg.read_blocks(cache, n=2, cu_rows=torch.zeros(3, **i32)), lambda: pkg.read_blocks(cache, n=-1),
+           lambda: pkg.read_blocks(cache, cu_rows=torch.zeros(3, **i32)), lambda: pkg.read_blocks(cache, n=2, out=(q, q)),
+           lambda: pkg.read_blocks(cache, n=2, out_dtype=torch.float64), lambda: pkg.attend_blocks(q[:, None].float(), cache),
+           lambda: pkg.attend_blocks(q, cache), lambda: pkg.attend_blocks(q, cache, cu_new=torch.zeros(2, **i32))]
+    for n, call in enumerate(bad):
+        with pytest.raises(pkg.SphKVError):
+            call()
+            print("call", n, "was taken")
+    for field, wrong in (("k_scale", cache.k_scale.half()), ("v_codes", cache.v_codes[:, :, :, :64].contiguous()), ("block_table", cache.block_table.long()),
+                         ("k_codes", cache.k_codes.transpose(0, 1)), ("seq_lens", cache.seq_lens.long()), ("status", torch.zeros(1, device=DEV))):
+        other = pkg.BlockCache(**{**cache.__dict__, field: wrong})
+        with pytest.raises(pkg.SphKVError):
+            pkg.decode_blocks(q, other)
+    # nothing to do is no error
+    assert pkg.read_blocks(cache, n=0)[0].shape == (2, 0, H, dh)
+    pkg.append_blocks(cache, k[:, :0], k[:, :0])
+    assert pkg.attend_blocks(q[:, None][:, :0], cache).shape == (2, 0, 4, dh)
+    pkg.check_status(cache)
+
+
 def test_nan_pages_stay_where_they_are_seen(pkg):
     """A page that reads back as NaN reaches the rows that see it, and no others."""
     H, N, dh = 1, 16, 64
