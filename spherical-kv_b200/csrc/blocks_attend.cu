@@ -19,13 +19,13 @@
 // Work: (block, head, key tile) in one line, cut evenly over the CTAs; a block that two or more CTAs share is joined by a
 // second launch.
 //
-// Measured: 2048 queries x 32 heads on 32768 tokens 1.29 ms in a graph, 0.83 PFLOP/s, half of what cuBLAS reaches in a burst; five
-// pieces of 301 .. 61 queries on up to 6001 tokens 109 us.  A pair of tiles (256 x 128) takes 5900 cycles.  The floor is 2048 for
+// Measured: 2048 queries x 32 heads on 32768 tokens 1.14 ms in a graph, 0.94 PFLOP/s, 57 % of what cuBLAS reaches in a burst; five
+// pieces of 301 .. 61 queries on up to 6001 tokens 102 us.  A pair of tiles (256 x 128) takes 5200 cycles.  The floor is 2048 for
 // the products (their operands ask for 96 of shared memory's 128 bytes a cycle, the conversion for another 32) and 2048 for the
 // exponentials; what is missing is in the chain S -> softmax -> P V -> S of each tile: a warp needs 620 cycles for 64 weights where
 // the exponential unit is busy for 550, and in the kernel, with two more warps on each scheduler and tensor memory shared
-// with the products, 1100 to 1500; a wait for a barrier costs 70 to 130 cycles even where there is nothing to wait for.
-// Tensor pipe 35 %, issue slots 54 %, no local memory.  Local memory is what the arrangement of the roles avoids: with all of L1
+// with the products, twice that (1.29 ms while the next logits came in behind all of a step's weights); a wait for a barrier costs 70 to 130 cycles even where there is nothing to wait for.
+// Tensor pipe 40 %, issue slots 52 %, no local memory.  Local memory is what the arrangement of the roles avoids: with all of L1
 // taken by shared memory a spilled word comes from L2 (1.96 ms with 512 threads and the tile's 128 logits in registers).
 #include "blocks.cuh"
 
@@ -439,49 +439,59 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
             }
           } else {
             // 32 keys at a time, in a loop that stays one: with all 128 in sight the compiler starts more than it has registers
-            // for.  The next 32 travel while the exponentials are taken.
-            float x[32];
-            tmem_ld_x32(s_at, x);
-#pragma unroll 1
-            for (int h = 0; h < 4; ++h) {
-              float2 e[16], part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-              uint32_t p[16];
-              const float4 of[2] = {lds_f4(meta_at + 32 * h), lds_f4(meta_at + 32 * h + 16)};
-              const float c[2] = {of[0].x * f, of[1].x * f};
-              tmem_wait_ld();
+            // for.  The next 32 travel while the first half of the exponentials is taken, and their largest is found beside the
+            // second half (behind the last 32 the first are read again, to no purpose: a branch would part the two).
+            float x[32], mx;
+            float4 of[2];
+            auto highest = [&] {
               float top[2];
 #pragma unroll
               for (int gg = 0; gg < 2; ++gg) {
                 const float* const v = x + 16 * gg;
-                top[gg] = fmaxf(fmaxf(v[0], v[1]), v[2]);
-                float odd = fmaxf(fmaxf(v[3], v[4]), v[5]);
+                float even = fmaxf(fmaxf(v[0], v[1]), v[2]), odd = fmaxf(fmaxf(v[3], v[4]), v[5]);
 #pragma unroll
-                for (int i = 6; i < 14; i += 4) top[gg] = fmaxf(fmaxf(top[gg], v[i]), v[i + 1]), odd = fmaxf(fmaxf(odd, v[i + 2]), v[i + 3]);
-                top[gg] = fmaxf(fmaxf(fmaxf(top[gg], v[14]), v[15]), odd) * c[gg];
+                for (int i = 6; i < 14; i += 4) even = fmaxf(fmaxf(even, v[i]), v[i + 1]), odd = fmaxf(fmaxf(odd, v[i + 2]), v[i + 3]);
+                top[gg] = fmaxf(fmaxf(fmaxf(even, v[14]), v[15]), odd) * (of[gg].x * f);
               }
-              const float mx = fmaxf(top[0], top[1]);
+              mx = fmaxf(top[0], top[1]);
+            };
+            of[0] = lds_f4(meta_at), of[1] = lds_f4(meta_at + 16);
+            tmem_ld_x32(s_at, x);
+            tmem_wait_ld();
+            highest();
+#pragma unroll 1
+            for (int h = 0; h < 4; ++h) {
               const bool up = mx > m + kAtLazy;
               if (__any_sync(0xffffffffu, up)) move(up ? mx : m, 1.f, h);
+              float2 e[16], part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+              uint32_t p[16];
 #pragma unroll
               for (int gg = 0; gg < 2; ++gg) {
-                const float add = of[gg].y - m;
+                const float c = of[gg].x * f, add = of[gg].y - m;
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                  e[8 * gg + i] = __ffma2_rn(make_float2(x[16 * gg + 2 * i], x[16 * gg + 2 * i + 1]), make_float2(c[gg], c[gg]), make_float2(add, add));
+                  e[8 * gg + i] = __ffma2_rn(make_float2(x[16 * gg + 2 * i], x[16 * gg + 2 * i + 1]), make_float2(c, c), make_float2(add, add));
               }
-              if (h < 3) tmem_ld_x32(s_at + 32 * (h + 1), x);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
+              const float up0 = of[0].z, up1 = of[1].z;
+              const int next = (h + 1) & 3;
+              of[0] = lds_f4(meta_at + 32 * next), of[1] = lds_f4(meta_at + 32 * next + 16);
+              tmem_ld_x32(s_at + 32 * next, x);
+              auto weigh = [&](int i) {
                 if ((i & 3) == 1)  // a quarter: 64 keys take a warp 535 cycles instead of 622, three or four of eight no less
                   e[i] = ex2_poly(e[i]);
                 else
                   e[i].x = ex2(e[i].x), e[i].y = ex2(e[i].y);
                 part[i >> 3] = __fadd2_rn(part[i >> 3], e[i]);
                 p[i] = pack_f16x2(e[i].x, e[i].y);
-              }
-              l += (part[0].x + part[0].y) * of[0].z;
-              l += (part[1].x + part[1].y) * of[1].z;
+              };
+#pragma unroll
+              for (int i = 0; i < 8; ++i) weigh(i);
               tmem_wait_ld();
+#pragma unroll
+              for (int i = 8; i < 16; ++i) weigh(i);
+              highest();
+              l += (part[0].x + part[0].y) * up0;
+              l += (part[1].x + part[1].y) * up1;
               tmem_st_x16u(s_at + 16 * h, p);  // over logits that have been read
             }
           }
