@@ -8,11 +8,12 @@
 //   1 warp   issues the products: logits S_t = Q_t K^T and outputs O_t += P_t V (tcgen05, P from tensor memory), for the two
 //            row tiles t in turn, so that the tensor cores work on one while the other's softmax runs;
 //   8 warps  softmax, a thread to a query row, 32 keys at a time: S from tensor memory, a page's key scale times the row's
-//            factor as one multiplier for its 16 keys and up, weights 2^6 p v / S_v in f16 back over S as the next product's
+//            factor as one multiplier for its 16 keys and up, weights p v / S_v in f16 back over S as the next product's
 //            operand.  The page's value scale is part of the exponent, so it costs nothing per element; the sum of p takes
-//            it out again once for 16 keys.  A row's reference maximum moves only when a logit passes it by 2^8; O and the
-//            tile's weights so far are then rescaled in place (every earlier product is complete: S_t(k) is issued behind
-//            P_t V(k - 1)).
+//            it out again once for 16 keys.  The row's reference is of logit and value scale together, so that f16 has the bits
+//            of what weighs most in the row, whatever scales it does not see; it puts the largest at 2^6 and moves only
+//            when one passes 2^14.  O and the tile's weights so far are then rescaled in place (every earlier product is complete:
+//            S_t(k) is issued behind P_t V(k - 1)).
 // Q rows are scaled by a power of two as in the decode kernel: bf16 and f16 queries are exact in f16.  Weights have f16's 11
 // bits, sums are fp32.  A quarter of the exponentials goes through a polynomial on the fma pipe.
 //
@@ -39,8 +40,7 @@ constexpr int kAtProducts = 16;
 // five warps each (two of softmax, two of codes, one of 16 .. 19), so what goes up has to come down quarter by quarter.
 constexpr int kAtRegs = 96, kAtRegsSoftmax = 128, kAtRegsCodes = 80, kAtRegsRest = 64;
 static_assert(2 * kAtRegsSoftmax + 2 * kAtRegsCodes + kAtRegsRest <= 5 * kAtRegs && 20 * 32 * kAtRegs <= 65536, "registers");
-constexpr float kAtLazy = 8.f;
-constexpr float kAtWeight = 6.f;  // log2: weights stay below 2^15 with the lazy maximum
+constexpr float kAtWeight = 6.f, kAtLazy = 14.f;  // log2 of the largest weight where the reference moves, and where it does not yet
 
 struct AtArgs {
   sphkv_blocks c;
@@ -94,10 +94,10 @@ __global__ void __launch_bounds__(1024) blocks_attend_plan_kernel(const __grid_c
 
 // ---- shared memory ----------------------------------------------------------------------------------------
 struct AtMeta {       // of a key tile, for the softmax
-  float4 of[8];       // of 16 keys: key scale; log2(value scale / S) + 6; 1 / (that, not as a logarithm), which takes the value
-                      // scale out of the sum of weights; unused
+  float4 of[8];       // of 16 keys: key scale; log2(value scale / S); S / value scale, which takes the value scale out of the sum of
+                      // weights; unused
   float down, big;    // S before / S; S
-  uint32_t bad;       // groups without a page
+  uint32_t bad;       // groups without a page; << 8: whose values count as zeros
   uint32_t pad;
 };
 constexpr int kAtWalkBytes = 112;
@@ -406,7 +406,18 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
               tmem_st_x16(s_at + 16 * h, w);
             }
           };
-          if (down != 1.f) move(m, down, 0);
+          if (down != 1.f) {
+            // S has grown.  The row's reference goes the other way, so that O stays as it is; where the sum would grow past
+            // 32 bits (or all scales were 0) O shrinks instead.
+            const int e = (int)(__float_as_uint(down) >> 23) - 127;  // a power of two
+            const float grown = l * __uint_as_float((uint32_t)(127 - max(e, -80)) << 23);
+            if (e >= -80 && !__any_sync(0xffffffffu, grown > 0x1p110f)) {
+              m += (float)e;
+              l = grown;
+            } else {
+              move(m, down, 0);
+            }
+          }
           if (edge) {
 #pragma unroll 1
             for (int g = 0; g < 8; ++g) {
@@ -420,10 +431,10 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
                 if (key0 + 16 * g + c < first || key0 + 16 * g + c >= lim || ((bad >> g) & 1)) v[c] = -INFINITY;
                 top = fmaxf(top, v[c]);
               }
-              top *= of.x * f;
+              top = fmaf(top, of.x * f, of.y);
               const bool up = top > m + kAtLazy;
               // 16 keys are half of what move() counts in: an odd group's first half has not been stored yet
-              if (__any_sync(0xffffffffu, up)) move(up ? top : m, 1.f, (g + 1) >> 1);
+              if (__any_sync(0xffffffffu, up)) move(up ? top - kAtWeight : m, 1.f, (g + 1) >> 1);
               float all = 0.f;
               uint32_t p[8];
 #pragma unroll
@@ -431,7 +442,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
                 const float y = v[2 * i], z = v[2 * i + 1];
                 const float e = y == -INFINITY ? 0.f : ex2(fmaf(y, of.x * f, of.y - m)), h = z == -INFINITY ? 0.f : ex2(fmaf(z, of.x * f, of.y - m));
                 all += e + h;
-                p[i] = pack_f16x2(e, h);
+                p[i] = (bad >> (8 + g)) & 1 ? 0u : pack_f16x2(e, h);  // their values count as zeros
               }
               l += all == 0.f ? 0.f : all * of.z;
               tmem_st_x8u(s_at + 8 * g, p);  // over logits that have been read
@@ -451,7 +462,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
                 float even = fmaxf(fmaxf(v[0], v[1]), v[2]), odd = fmaxf(fmaxf(v[3], v[4]), v[5]);
 #pragma unroll
                 for (int i = 6; i < 14; i += 4) even = fmaxf(fmaxf(even, v[i]), v[i + 1]), odd = fmaxf(fmaxf(odd, v[i + 2]), v[i + 3]);
-                top[gg] = fmaxf(fmaxf(fmaxf(even, v[14]), v[15]), odd) * (of[gg].x * f);
+                top[gg] = fmaf(fmaxf(fmaxf(fmaxf(even, v[14]), v[15]), odd), of[gg].x * f, of[gg].y);
               }
               mx = fmaxf(top[0], top[1]);
             };
@@ -462,7 +473,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
 #pragma unroll 1
             for (int h = 0; h < 4; ++h) {
               const bool up = mx > m + kAtLazy;
-              if (__any_sync(0xffffffffu, up)) move(up ? mx : m, 1.f, h);
+              if (__any_sync(0xffffffffu, up)) move(up ? mx - kAtWeight : m, 1.f, h);
               float2 e[16], part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
               uint32_t p[16];
 #pragma unroll
@@ -511,9 +522,9 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
         const bool live = flat < u.rows;
         const int tok = (u.r0 + flat) / a.group, hd = walk.head * a.group + (u.r0 + flat) - tok * a.group;
         const int64_t dense = (int64_t)u.row0 + tok;
-        const float scale = big * 0x1p-6f;
+        const float scale = big * 0x1p-6f;  // of outputs and sums of a part
         float* const part = a.parts + ((int64_t)blockIdx.x * 2 + (walk.from > 0 ? 0 : 1)) * (DH + 2) * kAtRows + flat;
-        const float per = l == 0.f ? 0.f : scale / l;
+        const float per = l == 0.f ? 0.f : big / l;
         tc_fence_after();
 #pragma unroll 1
         for (int i = 0; i < DH / 16; ++i) {
@@ -535,7 +546,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
             for (int c = 0; c < 16; ++c) part[(2 + 16 * i + c) * kAtRows] = o[c] * scale;
           }
         }
-        if (live && !walk.whole) part[0] = l == 0.f ? -INFINITY : m, part[kAtRows] = l;
+        if (live && !walk.whole) part[0] = l == 0.f ? -INFINITY : m, part[kAtRows] = l * 0x1p-6f;
         tc_fence_before();
       }
     }
@@ -695,7 +706,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
       const int shift = 31 - __clz(a.c.page_size);
       uint32_t n = 0;
       while (!lost && next_segment()) {
-          const int limit = max(u.lim[0], u.lim[1]), key_begin = (u.kt0 + walk.from) * kAtKeys + 16 * (lane & 7);
+        const int limit = max(u.lim[0], u.lim[1]), key_begin = (u.kt0 + walk.from) * kAtKeys + 16 * (lane & 7);
         const int32_t* table = a.c.block_table + (int64_t)u.b * a.c.max_blocks;
         auto page_of = [&](int k) {
           const int t0 = key_begin + k * kAtKeys;
@@ -707,8 +718,9 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
         int page = page_of(0), next_page = page_of(1);
         float big = 0.f, ks = scale_of(a.c.k_scale, page), vs = scale_of(a.c.v_scale, page);
         for (int k = 0; k < walk.count; ++k, ++n) {
-          const unsigned bad = __ballot_sync(0xffffffffu, page != -2 && (page < 0 || page >= a.c.n_pages)) & 0xffu;
+          const bool there = page >= 0 && page < a.c.n_pages;
           const float ks_now = ks, vs_now = vs;
+          unsigned bad = __ballot_sync(0xffffffffu, page != -2 && !there) & 0xffu;
           page = next_page;
           next_page = page_of(k + 2);
           ks = scale_of(a.c.k_scale, page), vs = scale_of(a.c.v_scale, page);
@@ -717,16 +729,21 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
           for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
           float down = 1.f;
           if (top > big) {
-            const float b = __uint_as_float((__float_as_uint(top) + 0x7fffffu) & 0x7f800000u);
+            const float b = __uint_as_float(min((__float_as_uint(top) + 0x7fffffu) & 0x7f800000u, 0x7e800000u));
             down = big > 0.f ? big / b : 0.f;
             big = b;
           }
-          // pages of zeros have scale 0: any other value serves
-          const float ref = big > 0.f ? big : 1.f, v = vs_now == 0.f ? 1.f : vs_now * (1.f / ref);
+          const float ref = big > 0.f ? big : 1.f;
+          // The sum of weights takes v out again, which 32 bits allow down to 2^-80: values that are smaller still count as zeros,
+          // like those of scale 0, and v is what serves.
+          float v = vs_now * (1.f / ref);
+          const bool zeros = v < 0x1p-80f;
+          if (zeros) v = 1.f;
+          bad |= (__ballot_sync(0xffffffffu, there && zeros) & 0xffu) << 8;
           // as far ahead as keys may be: the softmax has left tile n - 3 behind, and this place held n - 4
           if (n >= 2 && !warp_wait(kKFree + (n & 1), (n >> 1) - 1)) break;
           AtMeta& mt = metas[n & 3];
-          if (lane < 8) mt.of[lane] = make_float4(ks_now, log2f(v) + kAtWeight, 0x1p-6f / v, 0.f);
+          if (lane < 8) mt.of[lane] = make_float4(ks_now, log2f(v), 1.f / v, 0.f);
           if (lane == 0) mt.down = k == 0 ? 1.f : down, mt.big = ref, mt.bad = bad;
           __syncwarp();
           if (lane == 0) mbar_arrive(bars + 8 * (kMFull + (n & 3)));

@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
         n1 = fmaxf(n1, m1);
         float down = 1.f;
         if (larger) {
-          const float b = __uint_as_float((__float_as_uint(vs) + 0x7fffffu) & 0x7f800000u);
+          const float b = __uint_as_float(min((__float_as_uint(vs) + 0x7fffffu) & 0x7f800000u, 0x7e800000u));
           per_big = __uint_as_float(0x7f000000u - __float_as_uint(b));
           down = big * per_big;
           big = b;

@@ -427,6 +427,52 @@ def test_nan_pages_stay_where_they_are_seen(pkg):
         scales.copy_(clean)
 
 
+@pytest.mark.parametrize("big", [2.0 ** 30, 2.0 ** 70, 1e36])
+def test_scales_that_are_not_seen(pkg, big):
+    """Rows do not lose bits to a larger value that only later rows see (down to 2^-80 of it), and pages whose value scale is smaller still
+    keep their part in the sums of weights."""
+    H, N, dh, Hq, ctx, n = 1, 16, 128, 8, 700, 150
+    cache = _cache(pkg, [ctx], H, N, dh, I8, 91)
+    k, v = _random((ctx, H, dh), 5, torch.float32), _random((ctx, H, dh), 6, torch.float32)
+    v[ctx - 30] *= big
+    v[:600] *= 2.0 ** -60 if big == 1e36 else 1.0
+    pkg.append_blocks(cache, k.to(DEV), v.to(DEV), cu_new=_cu([ctx]))
+    sides, table = _sides(cache), cache.block_table.cpu()
+    kk, vv = (s.rows(table[0], 0, ctx) for s in sides)
+    q = _random((n, Hq, dh), 3, torch.float16)
+    got = pkg.attend_blocks(q.to(DEV), cache, cu_new=_cu([n]), out_dtype=torch.float32)
+    # the page's 16 tokens share the large scale
+    see = (ctx - 30) // N * N - (ctx - n)
+    for lo, hi in ((0, see), (see, n))[big == 1e36:]:
+        want, _, _, off, size, _ = orc.attend(q[lo:hi], kk, vv, 0, list(range(ctx - n + lo, ctx - n + hi)), 1 / math.sqrt(dh))
+        last = ctx - n + hi
+        # weights below 2^-14 are off by 2^-25 where the row's largest weight times scale is 2^6 at least, and that is no more than what
+        # the row's values, scale by scale, weigh: keys * 2^-31 * the largest scale * 127 that the row sees
+        tiny = last * 2.0 ** -31 * float(vv[:last].abs().max())
+        _check(got[lo:hi], want, off + torch.finfo(torch.float16).eps / 2 * size + tiny, torch.float32)
+    pkg.check_status(cache)
+
+
+def test_value_scales_of_zero(pkg):
+    """A value is code * scale: pages of scale 0 are zeros whatever their codes, and count in the sum of weights."""
+    H, N, dh, Hq, ctx = 2, 16, 64, 8, 400
+    cache = _filled(pkg, [ctx], H, N, dh, I8, 95)
+    table = cache.block_table.cpu()
+    for zero in ([3, 4, 20], list(range(25)), list(range(0, 16))):
+        cache.v_scale[table[0, zero].long().to(DEV)] = 0
+        sides = _sides(cache)
+        kk, vv = (s.rows(table[0], 0, ctx) for s in sides)
+        for n in (1, 200):
+            q = _random((n, Hq, dh), 3, torch.bfloat16)
+            want, _, _, off, size, _ = orc.attend(q, kk, vv, 0, list(range(ctx - n, ctx)), 0.125)
+            got = pkg.attend_blocks(q.to(DEV), cache, cu_new=_cu([n]), out_dtype=torch.float32)
+            _check(got, want, off + torch.finfo(torch.float16).eps / 2 * size, torch.float32)
+            got = pkg.decode_blocks(q[-1:].to(DEV), cache, out_dtype=torch.float32)
+            _check(got, want[-1:], off[-1:], torch.float32)
+        cache.v_scale[:] = 0.01
+    pkg.check_status(cache)
+
+
 def test_streams_and_graphs(pkg):
     """A decode step recorded into two graphs that replay over growing lengths, and the same on another stream."""
     H, N, dh, Hq = 2, 16, 128, 8
