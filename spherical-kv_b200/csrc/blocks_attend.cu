@@ -20,12 +20,13 @@
 // Work: (block, head, key tile) in one line, cut evenly over the CTAs; a block that two or more CTAs share is joined by a
 // second launch.
 //
-// Measured: 2048 queries x 32 heads on 32768 tokens 1.14 ms in a graph, 0.94 PFLOP/s, 57 % of what cuBLAS reaches in a burst; five
-// pieces of 301 .. 61 queries on up to 6001 tokens 102 us.  A pair of tiles (256 x 128) takes 5200 cycles.  The floor is 2048 for
+// Measured: 2048 queries x 32 heads on 32768 tokens 1.10 ms in a graph, 0.97 PFLOP/s, 59 % of what cuBLAS reaches in a burst; five
+// pieces of 301 .. 61 queries on up to 6001 tokens 102 us.  A pair of tiles (256 x 128) takes 5000 cycles.  The floor is 2048 for
 // the products (their operands ask for 96 of shared memory's 128 bytes a cycle, the conversion for another 32) and 2048 for the
-// exponentials; what is missing is in the chain S -> softmax -> P V -> S of each tile: a warp needs 620 cycles for 64 weights where
-// the exponential unit is busy for 550, and in the kernel, with two more warps on each scheduler and tensor memory shared
-// with the products, twice that (1.29 ms while the next logits came in behind all of a step's weights); a wait for a barrier costs 70 to 130 cycles even where there is nothing to wait for.
+// exponentials; what is missing is in the chain of each row tile: softmax 2950 cycles (a warp alone needs 1100 for the tile, but
+// there are five on each scheduler), weights seen by the products' warp 400, P V 460, S 570, logits seen 340 (1.29 ms while the next
+// logits came in behind all of a step's weights).  Logits of 64 keys at a time ahead of P V, in the columns that the weights leave
+// free: 1.40 ms, since a product of 64 columns takes as long as one of 128.
 // Tensor pipe 40 %, issue slots 52 %, no local memory.  Local memory is what the arrangement of the roles avoids: with all of L1
 // taken by shared memory a spilled word comes from L2 (1.96 ms with 512 threads and the tile's 128 logits in registers).
 #include "blocks.cuh"
@@ -38,7 +39,7 @@ constexpr int kAtThreads = 640;  // warps 0-3, 4-7: softmax of tile 0, 1; 8-11, 
 constexpr int kAtProducts = 16;
 // Registers of a thread: at launch; after the softmax has taken what the others gave up.  The file is four quarters, with
 // five warps each (two of softmax, two of codes, one of 16 .. 19), so what goes up has to come down quarter by quarter.
-constexpr int kAtRegs = 96, kAtRegsSoftmax = 128, kAtRegsCodes = 80, kAtRegsRest = 64;
+constexpr int kAtRegs = 96, kAtRegsSoftmax = 136, kAtRegsCodes = 72, kAtRegsRest = 64;
 static_assert(2 * kAtRegsSoftmax + 2 * kAtRegsCodes + kAtRegsRest <= 5 * kAtRegs && 20 * 32 * kAtRegs <= 65536, "registers");
 constexpr float kAtWeight = 6.f, kAtLazy = 14.f;  // log2 of the largest weight where the reference moves, and where it does not yet
 
@@ -107,13 +108,15 @@ struct At {
   static constexpr int kOperand = kSlab * (DH / 64);  // keys or values of a tile, or a tile of queries
   static constexpr int kQ = 0, kK = 2 * kOperand, kV = kK + 2 * kOperand, kMeta = kV + 2 * kOperand;
   static constexpr int kBars = kMeta + 4 * (int)sizeof(AtMeta);
-  static constexpr int kPrefix = kBars + 24 * 8;
+  static constexpr int kPrefix = kBars + 18 * 8;
   static constexpr int kItems = kPrefix + (kDealt + 4) * 4;
   static constexpr int kWalks = kItems + kDealt * (int)sizeof(AtItem);
   static constexpr int kSmem = kWalks + kAtThreads / 32 * kAtWalkBytes + 1024;
 };
 static_assert(At<128>::kSmem <= 232448, "shared memory of a CTA");
-enum { kKFull = 0, kKFree = 2, kVFull = 4, kVFree = 6, kMFull = 8, kQFull = 12, kSFull = 14, kPFull = 16, kODone = 18, kLast = 20 };
+// kNext: for the n-th step of the products, keys and scales of tile n and values of tile n - 1 are there, in one barrier, since
+// every wait costs the products' warp 350 cycles of its chain (1.12 ms with three); kVFull: the values alone, behind a segment's last tile.
+enum { kNext = 0, kKFree = 2, kVFull = 4, kVFree = 6, kQFull = 8, kSFull = 10, kPFull = 12, kODone = 14, kLast = 16 };
 
 __device__ __forceinline__ void tmem_ld_x32(uint32_t addr, float* v) {
   asm volatile(
@@ -237,12 +240,11 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bars + 8 * (kKFull + i), 4), mbar_init(bars + 8 * (kKFree + i), 1);
+      mbar_init(bars + 8 * (kNext + i), 9), mbar_init(bars + 8 * (kKFree + i), 1);
       mbar_init(bars + 8 * (kVFull + i), 4), mbar_init(bars + 8 * (kVFree + i), 1);
       mbar_init(bars + 8 * (kQFull + i), 4), mbar_init(bars + 8 * (kSFull + i), 1);
       mbar_init(bars + 8 * (kPFull + i), 4), mbar_init(bars + 8 * (kODone + i), 1);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(bars + 8 * (kMFull + i), 1);
     mbar_init(bars + 8 * kLast, 1);
     fence_async_smem();
   }
@@ -561,9 +563,10 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
     const int ch = DH == 128 ? (lane & 3) + 4 * ((lane >> 3) & 1) : lane & 3;
     const int shift = 31 - __clz(a.c.page_size);
     const uint8_t* const codes = reinterpret_cast<const uint8_t*>(values ? a.c.v_codes : a.c.k_codes) + ts * DH + 16 * ch;
-    const int full = values ? kVFull : kKFull, free = values ? kVFree : kKFree;
+    const int full = values ? kVFull : kNext, free = values ? kVFree : kKFree;
     const uint32_t to = base + (values ? L::kV : L::kK);
     uint32_t n = 0;  // key tiles of the worker
+    if (values && lane == 0) mbar_arrive(bars + 8 * kNext);  // no values before the first tile
     while (!lost && next_segment()) {
       const int limit = max(u.lim[0], u.lim[1]), key_begin = (u.kt0 + walk.from) * kAtKeys;
       const int32_t* table = a.c.block_table + (int64_t)u.b * a.c.max_blocks;
@@ -619,7 +622,13 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
         }
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bars + 8 * (full + st));
+        // Behind a segment's last tile values are asked for ahead of the next step's keys: their second tile may not count for the
+        // step before it.
+        if (values && n >= 1 && !warp_wait(kNext + (st ^ 1), (n - 1) >> 1)) break;
+        if (lane == 0) {
+          mbar_arrive(bars + 8 * (full + st));
+          if (values) mbar_arrive(bars + 8 * (kNext + (st ^ 1)));
+        }
         // the next tile's codes are asked for as soon as their registers are free
         page = checked(next_page);
         next_page = page_of(k + 2);
@@ -652,8 +661,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
 #pragma unroll 1
         for (int k = 0; k <= count; ++k) {
           const uint32_t st = (n + k) & 1, before = st ^ 1;
-          if (k < count && !(warp_wait(kKFull + st, (n + k) >> 1) && warp_wait(kMFull + ((n + k) & 3), (n + k) >> 2))) break;
-          if (k > 0 && !warp_wait(kVFull + before, (n + k - 1) >> 1)) break;
+          if (!(k < count ? warp_wait(kNext + st, (n + k) >> 1) : warp_wait(kVFull + before, (n + k - 1) >> 1))) break;
           bool ok = true;
 #pragma unroll 1
           for (int t = 0; t < 2; ++t) {
@@ -746,7 +754,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
           if (lane < 8) mt.of[lane] = make_float4(ks_now, log2f(v), 1.f / v, 0.f);
           if (lane == 0) mt.down = k == 0 ? 1.f : down, mt.big = ref, mt.bad = bad;
           __syncwarp();
-          if (lane == 0) mbar_arrive(bars + 8 * (kMFull + (n & 3)));
+          if (lane == 0) mbar_arrive(bars + 8 * (kNext + (n & 1)));
         }
         lost = __any_sync(0xffffffffu, lost);
       }
