@@ -27,7 +27,7 @@
 // there are five on each scheduler), weights seen by the products' warp 400, P V 460, S 570, logits seen 340 (1.29 ms while the next
 // logits came in behind all of a step's weights).  Logits of 64 keys at a time ahead of P V, in the columns that the weights leave
 // free: 1.40 ms, since a product of 64 columns takes as long as one of 128.
-// Tensor pipe 40 %, issue slots 52 %, no local memory.  Local memory is what the arrangement of the roles avoids: with all of L1
+// Tensor pipe 41 %, issue slots 51 %, no local memory.  Local memory is what the arrangement of the roles avoids: with all of L1
 // taken by shared memory a spilled word comes from L2 (1.96 ms with 512 threads and the tile's 128 logits in registers).
 #include "blocks.cuh"
 
