@@ -280,9 +280,10 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
   };
   auto warp_wait = [&](int bar, uint32_t n) { return __all_sync(0xffffffffu, wait(bar, n)); };
   auto next_segment = [&] {
-    __syncwarp();
+    __syncwarp();  // the segment before has been read
     const int more = lane == 0 ? walk.next(a) : 0;
-    return __shfl_sync(0xffffffffu, more, 0) != 0;  // and what lane 0 wrote is there for all
+    __syncwarp();  // what lane 0 wrote is there for all: a shuffle alone orders no memory
+    return __shfl_sync(0xffffffffu, more, 0) != 0;
   };
 
   if (warp < 8) {
