@@ -408,6 +408,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
               }
               tmem_st_x16(s_at + 16 * h, w);
             }
+            tmem_wait_st();  // an odd group of 16 keys stores its weights into the last of these columns
           };
           if (down != 1.f) {
             // S has grown.  The row's reference goes the other way, so that O stays as it is; where the sum would grow past
