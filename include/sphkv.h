@@ -409,8 +409,8 @@ int sphkv_omega_ema(const float* ml, float* omega, int32_t n_units, int32_t kv_g
  * heads of its tokens.  Keys are stored as they come (post-RoPE for sphkv_blocks_decode / _attend).
  *
  * Every call is about the last n_b tokens of each sequence, positions ends[b] - n_b .. ends[b] - 1.
- * Their rows in the dense tensors are cu[b] .. cu[b + 1] - 1 (cu: device i32 [B + 1], ascending from
- * 0; rows from cu[B] on are left alone), or b * n .. b * n + n - 1 with n = rows / B where cu is NULL.
+ * Their rows in the dense tensors are cu[b] .. cu[b + 1] - 1 (cu: device i32 [B + 1], ascending;
+ * rows before cu[0] and from cu[B] on are left alone), or b * n .. b * n + n - 1 with n = rows / B where cu is NULL.
  * A sequence whose numbers do not fit (ends outside [0, max_blocks * page_size], cu not ascending
  * within [0, rows], n_b > ends[b]) is left out and raises SPHKV_ST_BAD_LENGTH in *status; a table
  * entry outside [0, n_pages) raises SPHKV_ST_BAD_BLOCK and its tokens count as absent. */

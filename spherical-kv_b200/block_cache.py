@@ -9,7 +9,7 @@ over a PagedCache merge by log-sum-exp: give both decodes an `out_partial` and j
 
 Every call is about the last n_b tokens of each sequence b, positions seq_lens[b] - n_b .. seq_lens[b] - 1: the same n for
 all (a dense [B, n, ...] tensor), or rows cu[b] .. cu[b + 1] - 1 of a [rows, ...] tensor (cu: int32 [B + 1] on the device;
-rows from cu[B] on are padding and left alone).  Lengths live on the device and no call reads them back, so all of them record
+rows before cu[0] and from cu[B] on are padding and left alone).  Lengths live on the device and no call reads them back, so all of them record
 into CUDA graphs.  Sequences whose numbers do not fit and bad table entries raise bits of `cache.status`
 (ops.check_status reads it).  Calls run on the current stream of the cache's device; their workspaces come from torch's
 allocator per call, so calls on several streams do not meet in them.

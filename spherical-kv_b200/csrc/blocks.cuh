@@ -33,8 +33,8 @@ __device__ __forceinline__ void bad_status(const sphkv_blocks& c, int bit) {
 }
 __device__ __forceinline__ BlockPiece checked_piece(const sphkv_blocks& c, const BlockRows& r, int b, int j, int lo, int hi, int end) {
   BlockPiece p = {b, j, lo, hi - lo, end};
-  if (b < 0 || lo < 0 || hi < lo || hi > r.rows) {
-    if (b >= 0) bad_status(c, SPHKV_ST_BAD_LENGTH);
+  if (b < 0 || j < 0 || lo < 0 || hi < lo || hi > r.rows) {  // j < 0: a slot of rows before cu[0], which are no sequence's
+    if (b >= 0 && j >= 0) bad_status(c, SPHKV_ST_BAD_LENGTH);
     p.b = -1;
     p.n = 0;
     return p;

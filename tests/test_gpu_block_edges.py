@@ -54,3 +54,40 @@ def test_references_move_inside_an_edge_tile(pkg, store, N, dh):
         tiny = 16 * ctx * 2.0 ** -31 * float(vv.abs().max())
         _check(got, want, off + HALF16 * size + tiny, torch.float32)
     pkg.check_status(cache)
+
+
+@pytest.mark.parametrize("group", [1, 3, 8])
+@pytest.mark.parametrize("lead", [1, 5, 700])
+def test_rows_before_the_first_sequence(pkg, group, lead):
+    """cu[0] above 0: the rows before it are no sequence's, in every operator and in both of attend's kernels."""
+    H, N, dh = 2, 16, 64
+    lens, Hq = [900, 40], 2 * group
+    cache = _filled(pkg, lens, H, N, dh, I8, 23)
+    other = _cache(pkg, lens, H, N, dh, I8, 23)
+    sides, table = _sides(cache), cache.block_table.cpu()
+    for news in ([1, 1], [500, 33]):
+        rows = lead + sum(news) + 2
+        cu = _cu(news) + lead
+        q = _random((rows, Hq, dh), 3, torch.bfloat16).to(DEV)
+        out = torch.full((rows, Hq, dh), 7.0, dtype=torch.bfloat16, device=DEV)
+        pkg.attend_blocks(q, cache, cu_new=cu, out=out)
+        assert (out[:lead] == 7.0).all() and (out[-2:] == 7.0).all()
+        at = lead
+        for b, n in enumerate(news):
+            kk, vv = (s.rows(table[b], 0, lens[b]) for s in sides)
+            want, _, _, off, size, _ = orc.attend(q[at:at + n].cpu(), kk, vv, 0, list(range(lens[b] - n, lens[b])), 1 / math.sqrt(dh))
+            _check(out[at:at + n], want, off + HALF16 * size, torch.bfloat16)
+            at += n
+        k, v = pkg.read_blocks(cache, cu_rows=_cu(news), rows=sum(news))
+        got = tuple(torch.full((rows, H, dh), 7.0, device=DEV) for _ in range(2))
+        pkg.read_blocks(cache, cu_rows=cu, out=got)
+        for a, b in zip(got, (k, v)):
+            assert (a[:lead] == 7.0).all() and torch.equal(a[lead:-2], b) and (a[-2:] == 7.0).all()
+    new = [torch.full((lead + sum(lens), H, dh), math.nan, device=DEV) for _ in range(2)]
+    for x, s in zip(new, (5, 6)):
+        x[lead:] = _random((sum(lens), H, dh), 23 + s, torch.bfloat16).to(DEV)
+    pkg.append_blocks(other, *new, cu_new=_cu(lens) + lead)
+    for a, b in zip(pkg.read_blocks(other, cu_rows=_cu(lens), rows=sum(lens)), pkg.read_blocks(cache, cu_rows=_cu(lens), rows=sum(lens))):
+        assert torch.equal(a, b)
+    pkg.check_status(cache)
+    pkg.check_status(other)
