@@ -132,7 +132,7 @@ def append_blocks(cache: BlockCache, k: torch.Tensor, v: torch.Tensor, cu_new: O
 
 
 def read_blocks(cache: BlockCache, n: Optional[int] = None, cu_rows: Optional[torch.Tensor] = None, rows: Optional[int] = None,
-                ends: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32,
+                ends: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = torch.float32,
                 out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Keys and values of a run of tokens of every sequence as dense rows: the last `n` (-> [B, n, Hkv, dh]), or cu_rows[b + 1]
     - cu_rows[b] of them (-> [rows, Hkv, dh], `rows` the host's bound of cu_rows[B]).  `ends` (int32 [B]) takes the tokens
@@ -145,7 +145,7 @@ def read_blocks(cache: BlockCache, n: Optional[int] = None, cu_rows: Optional[to
             raise _lib.SphKVError("read_blocks: cu_rows needs rows")
         rows = k.shape[0]
     return _call("read", cache, cache.seq_lens if ends is None else ends, -1 if n is None else n, cu_rows, 0 if rows is None else rows,
-                 _type(out_dtype), k, v)
+                 _type(torch.float32 if out_dtype is None else out_dtype), k, v)
 
 
 def _output(out: Optional[torch.Tensor], shape, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:

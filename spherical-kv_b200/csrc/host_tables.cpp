@@ -193,6 +193,7 @@ struct View {
   // `given`, or a new tensor
   bool output(const at::Tensor* given, at::IntArrayRef shape, int type, const char* name, at::Tensor& out) {
     if (given == nullptr) {
+      if (type < 0 || type > 2) return fail((Text(name) + ": no type for it").c_str());
       out = at::empty(shape, at::TensorOptions().dtype(kTypes[type]).device(dev));
       return true;
     }

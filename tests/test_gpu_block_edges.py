@@ -91,3 +91,16 @@ def test_rows_before_the_first_sequence(pkg, group, lead):
         assert torch.equal(a, b)
     pkg.check_status(cache)
     pkg.check_status(other)
+
+
+def test_read_without_a_type(pkg):
+    """out_dtype=None is read_blocks' default, and is not looked at where outputs are given."""
+    cache = _filled(pkg, [40, 20], 2, 16, 64, I8, 29)
+    want = pkg.read_blocks(cache, n=20)
+    for got in (pkg.read_blocks(cache, n=20, out_dtype=None), pkg.read_blocks(cache, cu_rows=_cu([20, 20]), rows=40, out_dtype=None)):
+        for a, b in zip(got, want):
+            assert a.dtype == torch.float32 and torch.equal(a.view_as(b), b)
+    out = tuple(torch.empty(2, 20, 2, 64, dtype=torch.float16, device=DEV) for _ in range(2))
+    got = pkg.read_blocks(cache, n=20, out=out, out_dtype=None)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b.half())
