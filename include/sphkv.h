@@ -420,7 +420,8 @@ int sphkv_omega_ema(const float* ml, float* omega, int32_t n_units, int32_t kv_g
 typedef struct sphkv_blocks {
   void *k_codes, *v_codes;    /* [n_pages][Hkv][page_size][dh], 16-byte aligned            */
   float *k_scale, *v_scale;   /* [n_pages][Hkv]                                          */
-  const int32_t* block_table; /* [B][max_blocks]; entries past a sequence's end are not read */
+  const int32_t* block_table; /* [B][max_blocks]; entries past a sequence's end, or before the page
+                                 of its `first`, are not read                          */
   const int32_t* ends;        /* [B] tokens held, the ones of this call among them       */
   int32_t* status;            /* optional device int, OR-ed with SPHKV_ST_* bits         */
   int32_t n_pages, Hkv, page_size, dh, B, max_blocks; /* page_size 16..128, dh 64 or 128  */

@@ -41,7 +41,8 @@ class BlockCache:
     v_codes: torch.Tensor      # the same
     k_scale: torch.Tensor      # f32 [n_pages, Hkv]
     v_scale: torch.Tensor      # f32 [n_pages, Hkv]
-    block_table: torch.Tensor  # i32 [B, max_blocks]: page of tokens page_size * i ..; entries past a sequence's end: anything
+    block_table: torch.Tensor  # i32 [B, max_blocks]: page of tokens page_size * i ..; entries past a sequence's end, or before the
+                               # page of the `first` that a call is given: anything
     seq_lens: torch.Tensor     # i32 [B]: tokens held, those of the present step among them
     status: Optional[torch.Tensor] = None
 

@@ -575,10 +575,10 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
       // lanes 0 .. 7 look after a tile's eight groups of 16 keys
       auto page_of = [&](int k) {
         const int t0 = key_begin + k * kAtKeys + 16 * (lane & 7);
-        return k < walk.count && t0 < limit ? table[t0 >> shift] : -2;
+        return k < walk.count && t0 < limit && t0 + 16 > u.first ? table[t0 >> shift] : -2;
       };
       auto checked = [&](int page) {
-        if (page == -2) return -2;  // behind the keys
+        if (page == -2) return -2;  // before the keys, or behind them: the table need not name a page
         if (page < 0 || page >= a.c.n_pages) {
           bad_status(a.c, SPHKV_ST_BAD_BLOCK);
           return -1;
@@ -603,12 +603,12 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
         const uint32_t st = n & 1;
         const int now = page;
         if (n >= 2 && !warp_wait(free + st, (n >> 1) - 1)) break;
-        const int there = limit - (key_begin + k * kAtKeys + 32 * w);
-        if (there < 32 || __any_sync(0xffffffffu, now < 0)) {  // rows behind the last key, or of no page, may be any bytes
+        const int warp_key0 = key_begin + k * kAtKeys + 32 * w, there = limit - warp_key0, before = u.first - warp_key0;
+        if (there < 32 || before > 0 || __any_sync(0xffffffffu, now < 0)) {  // rows that are no keys', or of no page, may be any bytes
 #pragma unroll
           for (int i = 0; i < NL; ++i) {
             const int its = __shfl_sync(0xffffffffu, now, 2 * w + (TPL * i) / 16);
-            if (TPL * i + ts >= there || its < 0) raw[i] = make_uint4(0, 0, 0, 0);
+            if (TPL * i + ts >= there || TPL * i + ts < before || its < 0) raw[i] = make_uint4(0, 0, 0, 0);
           }
         }
 #pragma unroll
@@ -720,7 +720,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
         const int32_t* table = a.c.block_table + (int64_t)u.b * a.c.max_blocks;
         auto page_of = [&](int k) {
           const int t0 = key_begin + k * kAtKeys;
-          return k < walk.count && t0 < limit ? table[t0 >> shift] : -2;
+          return k < walk.count && t0 < limit && t0 + 16 > u.first ? table[t0 >> shift] : -2;
         };
         auto scale_of = [&](const float* scales, int page) {
           return page >= 0 && page < a.c.n_pages ? scales[page * a.c.Hkv + walk.head] : 0.f;

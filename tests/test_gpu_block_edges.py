@@ -104,3 +104,36 @@ def test_read_without_a_type(pkg):
     got = pkg.read_blocks(cache, n=20, out=out, out_dtype=None)
     for a, b in zip(got, want):
         assert torch.equal(a, b.half())
+
+
+@pytest.mark.parametrize("store,N,dh", [(I8, 16, 128), (E4M3, 16, 64), (E4M3, 32, 128), (E4M3, 128, 64), (I8, 64, 64)])
+def test_nothing_before_first_is_looked_at(pkg, store, N, dh):
+    """Pages before first's have been given away (the table names none), and the slots before first hold any bytes."""
+    H, Hq = 2, 8
+    lens, first = [300, 140, 700], [100, 139, 517]
+    cache = _filled(pkg, lens, H, N, dh, store, 33)
+    sides, table = _sides(cache), cache.block_table.cpu()
+    for b, f in enumerate(first):
+        page = int(table[b, f // N])
+        for codes in (cache.k_codes, cache.v_codes):
+            codes.view(torch.uint8)[page, :, :f % N] = 0x7f  # NaN in e4m3
+        cache.block_table[b, :f // N] = -1
+    fs = torch.tensor(first, dtype=torch.int32, device=DEV)
+    for news in ([1, 1, 1], [2, 1, 0], [20, 1, 3], [250, 130, 300]):
+        q = _random((sum(news), Hq, dh), 3, torch.bfloat16)
+        got = pkg.attend_blocks(q.to(DEV), cache, cu_new=_cu(news), first=fs)
+        pkg.check_status(cache)
+        at = 0
+        for b, n in enumerate(news):
+            kk, vv = (s.rows(table[b], first[b], lens[b]) for s in sides)
+            want, _, _, off, size, _ = orc.attend(q[at:at + n], kk, vv, first[b], list(range(lens[b] - n, lens[b])), 1 / math.sqrt(dh))
+            if n:
+                _check(got[at:at + n], want, off + HALF16 * size, torch.bfloat16)
+            at += n
+    q = _random((3, Hq, dh), 3, torch.float32)
+    got = pkg.decode_blocks(q.to(DEV), cache, first=fs)
+    for b in range(3):
+        kk, vv = (s.rows(table[b], first[b], lens[b]) for s in sides)
+        want, _, _, off, _, _ = orc.attend(q[b:b + 1], kk, vv, first[b], [lens[b] - 1], 1 / math.sqrt(dh))
+        _check(got[b:b + 1], want, off, torch.float32)
+    pkg.check_status(cache)
