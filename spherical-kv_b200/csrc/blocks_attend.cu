@@ -393,7 +393,6 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
                 tmem_st_x16(o_at + 16 * i, o);
               }
             }
-            const uint32_t dd = pack_f16x2(d, d);
             tmem_wait_st();
 #pragma unroll 1
             for (int h = 0; h < done; ++h) {
@@ -403,8 +402,8 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
 #pragma unroll
               for (int c = 0; c < 16; ++c) {
                 const uint32_t v = __float_as_uint(w[c]);
-                const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&dd));
-                w[c] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&r));
+                const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&v));
+                w[c] = __uint_as_float(pack_f16x2(x.x * d, x.y * d));  // d in f16 would lose its bits below 2^-14
               }
               tmem_st_x16(s_at + 16 * h, w);
             }

@@ -137,3 +137,54 @@ def test_nothing_before_first_is_looked_at(pkg, store, N, dh):
         want, _, _, off, _, _ = orc.attend(q[b:b + 1], kk, vv, first[b], [lens[b] - 1], 1 / math.sqrt(dh))
         _check(got[b:b + 1], want, off, torch.float32)
     pkg.check_status(cache)
+
+
+def _scales(side, table, lo, hi):
+    """Of the pages of keys lo .. hi - 1: [keys, H]."""
+    return side.scale[table[torch.arange(lo, hi) // side.N].long()]
+
+
+def _least(q, k, scale, pos, scales, top, key0=0):
+    """What weights may be off that are below f16's normal numbers, per query row and head: 2^-25 of each where the row's largest weight (times
+    value scale) is put at 2^5 at least, that is 2^-30 of the largest, for every key; times the largest code.  scales: [keys, H], of the keys' pages."""
+    n, Hq, dh = q.shape
+    H = k.shape[1]
+    out = torch.zeros(n, Hq, 1, dtype=torch.float64)
+    if k.shape[0] == 0:
+        return out
+    for h in range(Hq):
+        x = q[:, h].double() @ k[:, h // (Hq // H)].T * scale
+        x = x.masked_fill(torch.arange(key0, key0 + k.shape[0])[None] > torch.as_tensor(pos)[:, None], -math.inf)
+        out[:, h, 0] = (torch.softmax(x, 1).nan_to_num(0.0) * scales[:, h // (Hq // H)].double()).amax(1) * (k.shape[0] * top * 2.0 ** -30)
+    return out
+
+
+@pytest.mark.parametrize("sm_scale", [0.4, 1.0])
+@pytest.mark.parametrize("store,N,dh,Hq,H,dtype", [(I8, 16, 128, 8, 2, torch.bfloat16), (E4M3, 64, 64, 6, 2, torch.float16)])
+def test_large_sm_scales(pkg, store, N, dh, Hq, H, dtype, sm_scale):
+    """Logits far apart: weights stand beside ones 2^20 times as large, and were scaled down where those came in behind them."""
+    lens = [5, 333, 200, 0]
+    cache = _filled(pkg, lens, H, N, dh, store, 51)
+    sides, table = _sides(cache), cache.block_table.cpu()
+    for news, first in (([1, 2, 1, 0], None), ([5, 150, 129, 0], None), ([5, 150, 129, 0], [3, 190, 130, 0])):
+        q = _random((sum(news), Hq, dh), 3, dtype)
+        f = None if first is None else torch.tensor(first, dtype=torch.int32, device=DEV)
+        out = pkg.attend_blocks(q.to(DEV), cache, cu_new=_cu(news), first=f, sm_scale=sm_scale, out_dtype=torch.float32)
+        at = 0
+        for b, n in enumerate(news):
+            lo = min(lens[b], 0 if first is None else first[b])
+            k, v = (s.rows(table[b], lo, lens[b]).reshape(-1, H, dh) for s in sides)
+            pos = list(range(lens[b] - n, lens[b]))
+            want, _, _, off, size, _ = orc.attend(q[at:at + n], k, v, lo, pos, sm_scale)
+            if n:
+                least = _least(q[at:at + n], k, sm_scale, pos, _scales(sides[1], table[b], lo, lens[b]), orc.TOP[store], lo)
+                _check(out[at:at + n], want, off + HALF16 * size + least, torch.float32)
+            at += n
+    q = _random((4, Hq, dh), 3, dtype)
+    out = pkg.decode_blocks(q.to(DEV), cache, sm_scale=sm_scale, out_dtype=torch.float32)
+    for b, n in enumerate(lens):
+        k, v = (s.rows(table[b], 0, n).reshape(-1, H, dh) for s in sides)
+        want, _, _, off, _, _ = orc.attend(q[b:b + 1], k, v, 0, [n - 1], sm_scale)
+        least = _least(q[b:b + 1], k, sm_scale, [n - 1], _scales(sides[1], table[b], 0, n), orc.TOP[store])
+        _check(out[b:b + 1], want, off + least, torch.float32)
+    pkg.check_status(cache)
