@@ -56,7 +56,8 @@ struct AtArgs {
   float* parts;  // [workers][2][dh + 2][256]: a worker's first, cut segment and its last
   int q_dtype, out_dtype, Hq, group, slots, workers;
   bool q_vec;
-  float scale_log2;
+  uint32_t q_sign;   // the sign of sm_scale, which the queries take: the softmax multiplies maxima, and needs a factor of 0 or more
+  float scale_log2;  // its magnitude, times log2 e
 };
 
 struct AtItem {
@@ -341,7 +342,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
             if (lane / RPL == r / RPL) mine = theirs;
             int e = (int)(tb >> 23);
             e = e == 255 ? 140 : max(e, 14);
-            const float sc = __uint_as_float((uint32_t)(267 - e) << 23);
+            const float sc = __uint_as_float(((uint32_t)(267 - e) << 23) | a.q_sign);
             uint32_t h[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -895,7 +896,8 @@ extern "C" int sphkv_blocks_attend(const sphkv_blocks* c, const void* q, int32_t
   a.out_dtype = out_dtype;
   a.Hq = Hq;
   a.group = group;
-  a.scale_log2 = sm_scale * kLog2e;
+  a.q_sign = sm_scale < 0.f ? 0x80000000u : 0u;
+  a.scale_log2 = fabsf(sm_scale) * kLog2e;
   a.workers = sms;
   const int64_t slots = block_slots(a.r, c->B, 8, 1);
   // key tiles of all blocks of queries are counted in 32 bits

@@ -188,3 +188,35 @@ def test_large_sm_scales(pkg, store, N, dh, Hq, H, dtype, sm_scale):
         least = _least(q[b:b + 1], k, sm_scale, [n - 1], _scales(sides[1], table[b], 0, n), orc.TOP[store])
         _check(out[b:b + 1], want, off + least, torch.float32)
     pkg.check_status(cache)
+
+
+@pytest.mark.parametrize("sm_scale", [-0.3, -1.0, 0.0])
+@pytest.mark.parametrize("store,N,dh,Hq,H,dtype", [(I8, 16, 128, 8, 2, torch.bfloat16), (E4M3, 64, 64, 6, 2, torch.float16)])
+def test_any_finite_sm_scale(pkg, store, N, dh, Hq, H, dtype, sm_scale):
+    """Negative scales and zero, in both of attend's kernels and in decode."""
+    lens = [5, 333, 200, 0]
+    cache = _filled(pkg, lens, H, N, dh, store, 51)
+    sides, table = _sides(cache), cache.block_table.cpu()
+    sign = -1 if sm_scale < 0 else 1
+    for news, first in (([1, 2, 1, 0], None), ([5, 150, 129, 0], None), ([5, 150, 129, 0], [3, 190, 130, 0])):
+        q = _random((sum(news), Hq, dh), 3, dtype)
+        f = None if first is None else torch.tensor(first, dtype=torch.int32, device=DEV)
+        out = pkg.attend_blocks(q.to(DEV), cache, cu_new=_cu(news), first=f, sm_scale=sm_scale, out_dtype=torch.float32)
+        at = 0
+        for b, n in enumerate(news):
+            lo = min(lens[b], 0 if first is None else first[b])
+            k, v = (s.rows(table[b], lo, lens[b]).reshape(-1, H, dh) for s in sides)
+            pos = list(range(lens[b] - n, lens[b]))
+            want, _, _, off, size, _ = orc.attend(sign * q[at:at + n], k, v, lo, pos, abs(sm_scale))
+            if n:
+                least = _least(q[at:at + n], k, sm_scale, pos, _scales(sides[1], table[b], lo, lens[b]), orc.TOP[store], lo)
+                _check(out[at:at + n], want, off + HALF16 * size + least, torch.float32)
+            at += n
+    q = _random((4, Hq, dh), 3, dtype)
+    out = pkg.decode_blocks(q.to(DEV), cache, sm_scale=sm_scale, out_dtype=torch.float32)
+    for b, n in enumerate(lens):
+        k, v = (s.rows(table[b], 0, n).reshape(-1, H, dh) for s in sides)
+        want, _, _, off, _, _ = orc.attend(sign * q[b:b + 1], k, v, 0, [n - 1], abs(sm_scale))
+        least = _least(q[b:b + 1], k, sm_scale, [n - 1], _scales(sides[1], table[b], 0, n), orc.TOP[store])
+        _check(out[b:b + 1], want, off + least, torch.float32)
+    pkg.check_status(cache)
