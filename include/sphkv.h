@@ -461,7 +461,8 @@ int sphkv_blocks_decode(const sphkv_blocks* c, const void* q, int32_t q_dtype, i
 
 /* Causal attention of the last n_b tokens of every sequence: the query at position p sees keys
  * first[b] .. p.  q [rows][Hq][dh] (16-bit types), out [rows][Hq][dh] contiguous; a query without keys gets zeros.
- * Rows past cu[B] are not written.  Values below 2^-80 of the largest value scale that the sequence has count as zeros. */
+ * Rows past cu[B] are not written.  sm_scale here and in sphkv_blocks_decode: any finite number.  Values below 2^-80 of the
+ * largest value scale that the sequence has count as zeros. */
 int64_t sphkv_blocks_attend_scratch_bytes(int32_t B, int64_t rows, int32_t Hq, int32_t Hkv, int32_t dh);
 int sphkv_blocks_attend(const sphkv_blocks* c, const void* q, int32_t q_dtype, int64_t q_row_stride,
                         int64_t q_head_stride, const int32_t* cu, int64_t rows, const int32_t* first, void* out,

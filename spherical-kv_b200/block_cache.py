@@ -17,7 +17,6 @@ allocator per call, so calls on several streams do not meet in them.
 from __future__ import annotations
 
 import ctypes as C
-import math
 from dataclasses import dataclass
 from typing import Optional, Tuple
 
@@ -165,7 +164,7 @@ def decode_blocks(q: torch.Tensor, cache: BlockCache, first: Optional[torch.Tens
     """Attention of one query a sequence, q [B, Hq, dh] (f32, bf16, f16), over its tokens first[b] .. seq_lens[b] - 1 (first:
     int32 [B], None = 0).  Returns [B, Hq, dh]; zeros where a sequence has no such token.  `out_partial` (f32 [B, Hq, dh + 2])
     receives (max, sum, acc), un-normalised, as decode_paged writes them."""
-    return _call("decode", cache, cache.seq_lens, (_calls or _bind())["scratch"][0], q, first, math.nan if sm_scale is None else sm_scale,
+    return _call("decode", cache, cache.seq_lens, (_calls or _bind())["scratch"][0], q, first, sm_scale,
                  _type(out_dtype), out, out_partial, want_out)
 
 
@@ -176,4 +175,4 @@ def attend_blocks(q: torch.Tensor, cache: BlockCache, cu_new: Optional[torch.Ten
     first[b] .. p.  q [B, n, Hq, dh], or [rows, Hq, dh] with cu_new; bf16 or f16.  Returns q's shape; zeros where a query sees
     nothing, and padding rows are not written."""
     return _call("attend", cache, cache.seq_lens, (_calls or _bind())["scratch"][1], q, cu_new, first,
-                 math.nan if sm_scale is None else sm_scale, _type(out_dtype), out)
+                 sm_scale, _type(out_dtype), out)

@@ -220,7 +220,7 @@ int block_rows(BlockRows& r, const sphkv_blocks* c, const int32_t* cu, int64_t r
 // a row's bytes
 int make_codes_map(CUtensorMap* map, const sphkv_blocks& c, void* codes, int box_rows, const char* what);
 int check_queries(const sphkv_blocks& c, const void* q, int q_dtype, const void* out, const float* out_partial, int out_dtype, int Hq,
-                  const char* what);
+                  float sm_scale, const char* what);
 // attention of up to eight query rows a unit: 1 << tshift tokens of a sequence, at most 1 << tokens_shift(group)
 int tokens_shift(int group);
 int few_queries(const sphkv_blocks& c, const BlockRows& r, const void* q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride,

@@ -876,7 +876,7 @@ extern "C" int sphkv_blocks_attend(const sphkv_blocks* c, const void* q, int32_t
   SPHKV_REQUIRE(rows <= 0x7ffffff, SPHKV_E_LIMIT, "blocks_attend: rows=%lld (max 2^27 - 1)", (long long)rows);
   if (rows == 0) return 0;  // tensors without elements have no address
   SPHKV_REQUIRE(q != nullptr, SPHKV_E_ARG, "blocks_attend: q is NULL");
-  if (int rc = check_queries(*c, q, q_dtype, out, nullptr, out_dtype, Hq, "blocks_attend")) return rc;
+  if (int rc = check_queries(*c, q, q_dtype, out, nullptr, out_dtype, Hq, sm_scale, "blocks_attend")) return rc;
   SPHKV_REQUIRE(q_dtype != SPHKV_F32, SPHKV_E_DTYPE, "blocks_attend: q_dtype=%d (16-bit types)", q_dtype);
   SPHKV_REQUIRE(((uintptr_t)out & 15) == 0, SPHKV_E_ALIGN, "blocks_attend: out needs 16 B");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

@@ -21,6 +21,8 @@
 // a segment's beginning and end take 3 us each); 1 x 2048 of 64 dims 13, all of it latency: work dealt 1.2 us, addresses and
 // first tiles 1, tiles 0.8, warps joined 0.8, then the second launch.  DRAM 56 % at 8 x 16384 under cold caches, issue slots 56 %
 // (268 instructions a tile), tensor pipe 24 %: with 16 warps neither bandwidth nor issue is full, the warps' own chains are long.
+#include <cmath>
+
 #include "blocks.cuh"
 
 namespace sphkv {
@@ -598,7 +600,8 @@ static int run_bd(BdArgs& a, void* scratch, int64_t scratch_bytes, const char* w
 }
 
 int check_queries(const sphkv_blocks& c, const void* q, int q_dtype, const void* out, const float* out_partial, int out_dtype, int Hq,
-                  const char* what) {
+                  float sm_scale, const char* what) {
+  SPHKV_REQUIRE(std::isfinite(sm_scale), SPHKV_E_ARG, "%s: sm_scale=%g", what, (double)sm_scale);
   SPHKV_REQUIRE(out || out_partial, SPHKV_E_ARG, "%s: no output", what);
   SPHKV_REQUIRE(q_dtype >= 0 && q_dtype <= 2 && out_dtype >= 0 && out_dtype <= 2, SPHKV_E_DTYPE, "%s: q_dtype=%d out_dtype=%d", what,
                 q_dtype, out_dtype);
@@ -650,7 +653,7 @@ extern "C" int sphkv_blocks_decode(const sphkv_blocks* c, const void* q, int32_t
                                    int64_t scratch_bytes, int32_t Hq, float sm_scale, void* stream) {
   if (int rc = check_blocks(c, "blocks_decode")) return rc;
   SPHKV_REQUIRE(q != nullptr, SPHKV_E_ARG, "blocks_decode: q is NULL");
-  if (int rc = check_queries(*c, q, q_dtype, out, out_partial, out_dtype, Hq, "blocks_decode")) return rc;
+  if (int rc = check_queries(*c, q, q_dtype, out, out_partial, out_dtype, Hq, sm_scale, "blocks_decode")) return rc;
   // one row a sequence, whatever ends[] says: one without tokens has a query all the same
   const BlockRows r = {nullptr, c->B, 1, 1, true};
   return few_queries(*c, r, q, q_dtype, q_row_stride, q_head_stride, first, out, out_dtype, out_partial, scratch, scratch_bytes, Hq,

@@ -112,7 +112,10 @@ struct Args {  // in the order of the Python side
   int i = 0;
   PyObject* next() { return a[i++]; }
   long long integer() { return PyLong_AsLongLong(next()); }
-  double real() { return PyFloat_AsDouble(next()); }
+  double scale(int dh) {  // of logits; None: 1 / sqrt(dh)
+    PyObject* o = next();
+    return o == Py_None ? 1.0 / std::sqrt((double)dh) : PyFloat_AsDouble(o);
+  }
   template <typename F>
   F function() { return reinterpret_cast<F>(static_cast<intptr_t>(integer())); }
   bool wrong = false;          // something that is neither a tensor nor None stood for a tensor
@@ -279,7 +282,7 @@ PyObject* blocks_read(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// fn, last error, stream, cache (7), scratch fn, q, first, scale (NaN: 1 / sqrt(dh)), type (-1: q's), out, out_partial, want out
+// fn, last error, stream, cache (7), scratch fn, q, first, scale (or None), type (-1: q's), out, out_partial, want out
 PyObject* blocks_decode(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   if (n != 18) return PyErr_Format(PyExc_TypeError, "blocks_decode: 18 arguments");
   HANDLE_TH_ERRORS
@@ -291,7 +294,7 @@ PyObject* blocks_decode(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   if (!v.read(args)) return refused(v.why);
   const auto scratch_of = args.function<decltype(&sphkv_blocks_decode_scratch_bytes)>();
   const at::Tensor *q = args.tensor(), *first = args.tensor();
-  double scale = args.real();
+  const double scale = args.scale(v.c.dh);
   int type = (int)args.integer();
   const at::Tensor *given = args.tensor(), *partial = args.tensor();
   const bool want = args.integer() != 0;
@@ -303,7 +306,6 @@ PyObject* blocks_decode(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   const int32_t* at;
   if (!v.i32(first, v.c.B, "first", at)) return refused(v.why);
   if (type < 0) type = type_of(q->scalar_type());
-  if (std::isnan(scale)) scale = 1.0 / std::sqrt((double)v.c.dh);
   const int64_t Hq = q->size(1);
   const std::array<int64_t, 3> rows = {v.c.B, Hq, (int64_t)v.c.dh + 2};
   if (partial != nullptr && (partial->scalar_type() != at::kFloat || partial->device() != v.dev || !partial->is_contiguous() || partial->sizes() != at::IntArrayRef(rows)))
@@ -329,7 +331,7 @@ PyObject* blocks_decode(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// fn, last error, stream, cache (7), scratch fn, q, cu, first, scale (NaN: 1 / sqrt(dh)), type (-1: q's), out
+// fn, last error, stream, cache (7), scratch fn, q, cu, first, scale (or None), type (-1: q's), out
 PyObject* blocks_attend(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   if (n != 17) return PyErr_Format(PyExc_TypeError, "blocks_attend: 17 arguments");
   HANDLE_TH_ERRORS
@@ -341,7 +343,7 @@ PyObject* blocks_attend(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   if (!v.read(args)) return refused(v.why);
   const auto scratch_of = args.function<decltype(&sphkv_blocks_attend_scratch_bytes)>();
   const at::Tensor *q = args.tensor(), *cu = args.tensor(), *first = args.tensor();
-  double scale = args.real();
+  const double scale = args.scale(v.c.dh);
   int type = (int)args.integer();
   const at::Tensor* given = args.tensor();
   if (PyErr_Occurred()) return nullptr;
@@ -352,7 +354,6 @@ PyObject* blocks_attend(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   const int32_t *at, *cu_at;
   if (!v.i32(first, v.c.B, "first", at) || !v.i32(cu, (int64_t)v.c.B + 1, "cu_new", cu_at)) return refused(v.why);
   if (type < 0) type = type_of(q->scalar_type());
-  if (std::isnan(scale)) scale = 1.0 / std::sqrt((double)v.c.dh);
   const int64_t Hq = q->size(q->dim() - 2);
   const at::AutoDispatchBelowADInplaceOrView plain;
   at::Tensor out;

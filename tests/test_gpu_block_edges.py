@@ -220,3 +220,13 @@ def test_any_finite_sm_scale(pkg, store, N, dh, Hq, H, dtype, sm_scale):
         least = _least(q[b:b + 1], k, sm_scale, [n - 1], _scales(sides[1], table[b], 0, n), orc.TOP[store])
         _check(out[b:b + 1], want, off + least, torch.float32)
     pkg.check_status(cache)
+
+
+def test_scales_that_are_no_number_are_refused(pkg):
+    cache = _filled(pkg, [40, 20], 2, 16, 64, I8, 29)
+    q = _random((2, 4, 64), 3, torch.bfloat16).to(DEV)
+    for bad in (math.nan, math.inf, -math.inf, 1e300):
+        for call in (lambda: pkg.decode_blocks(q, cache, sm_scale=bad), lambda: pkg.attend_blocks(q[:, None], cache, sm_scale=bad)):
+            with pytest.raises(pkg.SphKVError, match="sm_scale"):
+                call()
+    assert torch.equal(pkg.decode_blocks(q, cache), pkg.decode_blocks(q, cache, sm_scale=0.125))
