@@ -10,7 +10,9 @@
 // The logits' layout (row 2j, 2j + 1 of keys g, g + 8) becomes the weights' operand by four transposes of 8 x 8.
 // Precision: a query row is scaled by a power of two so that its largest element lies in [2^13, 2^14): bf16 and f16 rows are
 // exact in f16 then, fp32 rows go in as hi + lo (22 bits); weights are hi + lo as well; sums are fp32.  A page's key scale
-// multiplies its logits, its value scale its weights, relative to the largest value scale seen (a power of two, S).
+// multiplies its logits, its value scale its weights.  A row has two references, whole powers of two: one of its logits, for the sum of
+// p, and one of logit and value scale together, for the weights p v, so that f16 has the bits of what weighs most in the row, whatever
+// scales stand beside it.
 //
 // Work: 16-token tiles of all (unit, tile) pairs in one line, cut evenly over the CTAs; a CTA's share of a unit is a segment.
 // A segment's tiles go round the CTA's warps; each warp keeps maxima, sums and outputs of its own, with its own ring of
@@ -28,8 +30,8 @@
 namespace sphkv {
 
 constexpr int kBdWarps = 16, kBdThreads = 32 * kBdWarps;
-constexpr float kLazy = 8.f;     // a reference maximum moves when a logit passes it by 2^8
-constexpr float kWeight = 64.f;  // weights are 2^6 p v / S <= 2^14: f16 keeps 22 bits (hi + lo) of those above 2^-3
+constexpr float kLazy = 8.f;   // a reference moves when a logit passes it by 2^8
+constexpr int kWeightLog = 6;  // a weight at its reference is 2^6 and none is above 2^14: f16 keeps 22 bits (hi + lo) of those above 2^-3
 
 struct BdArgs {
   alignas(64) CUtensorMap k_map, v_map;
@@ -58,8 +60,8 @@ struct Bd {
   static constexpr int kPrefixOff = kBdWarps * kRing;
   static constexpr int kItemsOff = kPrefixOff + (kDealt + 4) * 4;
   static constexpr int kStatOff = kItemsOff + kDealt * 32;
-  static constexpr int kStat = 5 * 8;                              // floats of a warp: maxima, sums, true maxima, S (8 times), factors
-  static constexpr int kQOff = kStatOff + (kBdWarps * kStat + 8 * 3) * 4;
+  static constexpr int kStat = 5 * 8;                              // floats of a warp: references, sums, true maxima, the weights' references, factors
+  static constexpr int kQOff = kStatOff + (kBdWarps * kStat + 8 * 4) * 4;
   static constexpr int kQRow = 2 * (DH + 8);                       // bytes of a row of queries in f16
   static constexpr int kQ = 2 * 8 * kQRow + 32;                    // hi, lo, factors
   static constexpr int kBarOff = kQOff + kQ;
@@ -100,6 +102,23 @@ __device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ float lg2(float x) {
+  float r;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float power_of_2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+// A difference of two references, which are whole, as far as it matters: a row's logits are at most 2^129 times as heavy with
+// their value scales, and where they are 2^240 times as heavy without them, p of all that is not 0 is below 2^-126.
+__device__ __forceinline__ int exponent(float d) { return (int)fminf(fmaxf(d, -240.f), 240.f); }
+// p * vs * 2^(kWeightLog + e), which is at most 2^14 where p and vs are not 0, though vs * 2^e may be beyond fp32.  Not in line:
+// a rare one.  (Scales below fp32's normal numbers are no part of the references, and count as 0.)
+static __device__ __noinline__ float far_weight(float p, float vs, int e) {
+  if (vs < 0x1p-126f) return p * 0.f;
+  if (p == 0.f && vs < INFINITY) return 0.f;
+  const int half = e / 2;
+  return p * power_of_2(half) * power_of_2(kWeightLog) * vs * power_of_2(e - half);
+}
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -139,7 +158,7 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
   const uint32_t ring = smem_u32(smem) + warp * L::kRing;
   const uint32_t bars = smem_u32(smem) + L::kBarOff + warp * S * 8;
   float* const stats = reinterpret_cast<float*>(smem + L::kStatOff);
-  float* const cols_of = stats + WARPS * L::kStat;  // of a query row: maximum, sum, true maximum
+  float4* const cols_of = reinterpret_cast<float4*>(stats + WARPS * L::kStat);  // of a query row: reference, sum, true maximum, the weights' reference
   float* const joined = reinterpret_cast<float*>(smem);  // a warp's outputs: in its ring's place
   constexpr int JOIN = L::kRing / 4;
   const uint32_t q_at = smem_u32(smem) + L::kQOff;  // the segment's queries
@@ -276,7 +295,9 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
     for (int i = 0; i < KS; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
     const float kNone = -3.402823466e38f;
     float m0 = kNone, m1 = kNone, l0 = 0.f, l1 = 0.f, t0 = -INFINITY, t1 = -INFINITY;
-    float big = 0.f, per_big = 0.f;  // S and 1 / S
+    float v0 = kNone, v1 = kNone;  // the weights' references
+    float up0 = 1.f, up1 = 1.f;    // 2^kWeightLog * 2^(m - v), where
+    bool far = false;              // no row has its references more than 2^60 apart
 
     for (int k = 0, base = 0; k < mine; ++k) {
       if (k - base == 32) {
@@ -352,38 +373,39 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
       const float x0 = fmaxf(x[0], x[2]), x1 = fmaxf(x[1], x[3]);
       t0 = fmaxf(t0, x0);
       t1 = fmaxf(t1, x1);
-      const bool larger = vs > big && vs < INFINITY && row >= 0;
-      if (__any_sync(0xffffffffu, x0 > m0 + kLazy || x1 > m1 + kLazy) || larger) {
+      const float lv = lg2(vs);  // approximate: between 2^14 and the largest f16 is room
+      if (__any_sync(0xffffffffu, x0 > fminf(m0, v0 - lv) + kLazy || x1 > fminf(m1, v1 - lv) + kLazy)) {
         float n0 = x0, n1 = x1;
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
           n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
           n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
         }
-        n0 = fmaxf(n0, m0);
-        n1 = fmaxf(n1, m1);
-        float down = 1.f;
-        if (larger) {
-          const float b = __uint_as_float(min((__float_as_uint(vs) + 0x7fffffu) & 0x7f800000u, 0x7e800000u));
-          per_big = __uint_as_float(0x7f000000u - __float_as_uint(b));
-          down = big * per_big;
-          big = b;
-        }
-        const float d0 = ex2(m0 - n0), d1 = ex2(m1 - n1);
-        l0 *= d0;
-        l1 *= d1;
-        const float r0 = d0 * down, r1 = d1 * down;
+        far = false;
+        auto move = [&](float n, float& m, float& l, float& v, float& up) {  // what the weights so far are multiplied by
+          const float to = fmaxf(ceilf(n), m), v_to = fmaxf(ceilf(n + lv), v), r = ex2(v - v_to);
+          const int e = exponent(to - v_to);
+          l *= ex2(m - to);
+          m = to;
+          v = v_to;
+          up = power_of_2(min(max(e, -60), 60) + kWeightLog);
+          far |= abs(e) > 60;
+          return r;
+        };
+        const float r0 = move(n0, m0, l0, v0, up0), r1 = move(n1, m1, l1, v1, up1);
 #pragma unroll
         for (int i = 0; i < KS; ++i) acc[i][0] *= r0, acc[i][1] *= r1, acc[i][2] *= r0, acc[i][3] *= r1;
-        m0 = n0;
-        m1 = n1;
       }
       float w[4] = {ex2(x[0] - m0), ex2(x[1] - m1), ex2(x[2] - m0), ex2(x[3] - m1)};
       l0 += w[0] + w[2];
       l1 += w[1] + w[3];
-      const float ve = vs * per_big * kWeight;
+      if (far || vs > 0x1p60f) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] *= ve;
+        for (int i = 0; i < 4; ++i) w[i] = far_weight(w[i], vs, exponent(i & 1 ? m1 - v1 : m0 - v0));
+      } else {
+        const float ve0 = vs * up0, ve1 = vs * up1;
+        w[0] *= ve0, w[1] *= ve1, w[2] *= ve0, w[3] *= ve1;
+      }
       if (edge) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -420,7 +442,7 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
         st[2 * j] = m0, st[2 * j + 1] = m1;
         st[8 + 2 * j] = l0, st[9 + 2 * j] = l1;
         st[16 + 2 * j] = t0, st[17 + 2 * j] = t1;
-        st[24 + 2 * j] = st[25 + 2 * j] = big;
+        st[24 + 2 * j] = v0, st[25 + 2 * j] = v1;
       }
       float* const mine_at = joined + warp * JOIN + g * (GD + 2);  // this warp has taken every tile of its own
 #pragma unroll
@@ -433,18 +455,19 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
       for (int col = warp; col < cols; col += WARPS) {  // a warp to a query row: lane w looks after warp w
         const float* const of = stats + (lane % WARPS) * L::kStat + col;
         const bool have = lane < n_warps;
-        float top = have ? of[0] : kNone, true_top = have ? of[16] : -INFINITY;
+        float top = have ? of[0] : kNone, true_top = have ? of[16] : -INFINITY, v_top = have ? of[24] : kNone;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
           true_top = fmaxf(true_top, __shfl_xor_sync(0xffffffffu, true_top, o));
+          v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, o));
         }
         const float f = have ? ex2(of[0] - top) : 0.f;
         float sum = have ? of[8] * f : 0.f;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (have) stats[lane * L::kStat + 32 + col] = f * (of[24] * (1.f / kWeight));
-        if (lane == 0) cols_of[3 * col] = top, cols_of[3 * col + 1] = sum, cols_of[3 * col + 2] = true_top;
+        if (have) stats[lane * L::kStat + 32 + col] = ex2(of[24] - v_top);
+        if (lane == 0) cols_of[col] = make_float4(top, sum, true_top, v_top);
       }
       __syncthreads();
       const bool whole = count == u.tiles;
@@ -456,8 +479,11 @@ __global__ void __launch_bounds__(kBdThreads, 1) blocks_decode_kernel(const __gr
 #pragma unroll
         for (int w = 0; w < WARPS; ++w)
           if (w < n_warps) v += from[w * JOIN] * stats[w * L::kStat + 32 + col];
-        const float top = cols_of[3 * col], sum = cols_of[3 * col + 1], true_top = cols_of[3 * col + 2];
+        const float4 of = cols_of[col];
+        const float top = of.x, sum = of.y, true_top = of.z;
         const float to_true = true_top == -INFINITY ? 0.f : ex2(top - true_top);
+        const int e = exponent(of.w - top) - kWeightLog;
+        v = v * power_of_2(e >> 1) * power_of_2(e - (e >> 1));
         if (whole) {
           const int tok = col / a.group, h = head * a.group + col - tok * a.group;
           const int64_t at = (int64_t)(u.row0 + tok) * a.Hq + h;

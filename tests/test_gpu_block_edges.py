@@ -230,3 +230,94 @@ def test_scales_that_are_no_number_are_refused(pkg):
             with pytest.raises(pkg.SphKVError, match="sm_scale"):
                 call()
     assert torch.equal(pkg.decode_blocks(q, cache), pkg.decode_blocks(q, cache, sm_scale=0.125))
+
+
+@pytest.mark.parametrize("power", [10, 20, 30, 70, 110])
+@pytest.mark.parametrize("store,N,dh,q_dtype", [(I8, 128, 128, torch.float32), (E4M3, 16, 64, torch.float16)])
+def test_decode_value_scales_far_apart(pkg, store, N, dh, q_dtype, power):
+    """A page of large values that the softmax gives next to nothing takes no bits from the others, wherever it lies.  Every warp has several
+    tiles: of the page, before and behind it."""
+    H, Hq, ctx, B = 8, 16, 4000, 8
+    direction = torch.sign(_random((1, 1, dh), 9, torch.float32))
+    q = (direction + 0.05 * _random((B, Hq, dh), 3, torch.float32)).to(q_dtype)
+    for at in (0, 2000):
+        cache = _cache(pkg, [ctx] * B, H, N, dh, store, 61)
+        k, v = 0.05 * _random((B, ctx, H, dh), 5, torch.float32), _random((B, ctx, H, dh), 6, torch.float32)
+        page = torch.arange(ctx) // 128 == at // 128
+        # logits of the page: lower by about `power` + 8 in units of log2 e
+        k[:, page] -= direction * ((power + 8) * math.log(2) / dh ** 0.5)
+        v[:, page] *= 2.0 ** power
+        pkg.append_blocks(cache, k.to(DEV), v.to(DEV))
+        sides, table = _sides(cache), cache.block_table.cpu()
+        part = torch.empty(B, Hq, dh + 2, device=DEV)
+        got = pkg.decode_blocks(q.to(DEV), cache, out_dtype=torch.float32, out_partial=part)
+        for b in (0, 3, 7):
+            kk, vv = (s.rows(table[b], 0, ctx) for s in sides)
+            want, _, _, off, _, _ = orc.attend(q[b:b + 1], kk, vv, 0, [ctx - 1], 1 / math.sqrt(dh))
+            least = _least(q[b:b + 1], kk, 1 / math.sqrt(dh), [ctx - 1], _scales(sides[1], table[b], 0, ctx), orc.TOP[store])
+            _check(got[b:b + 1], want, off + least, torch.float32)
+            _check((part[b:b + 1, :, 2:] / part[b:b + 1, :, 1:2]), want, off + least + want.abs() * 2.0 ** -22, torch.float32)
+        pkg.check_status(cache)
+
+
+@pytest.mark.parametrize("power", [20, 60, 110])
+def test_few_tokens_and_values_that_they_do_not_see(pkg, power):
+    """The last token's value is large: the token before it, in the same unit, does not see it."""
+    H, Hq, N, dh, ctx, B = 8, 32, 16, 128, 4000, 8
+    cache = _cache(pkg, [ctx - 1] * B, H, N, dh, I8, 65, max_len=[ctx] * B)
+    k, v = _random((B, ctx, H, dh), 5, torch.float32), _random((B, ctx, H, dh), 6, torch.float32)
+    v[:, -N:] *= 0  # the last page's scale will be the large value's
+    pkg.append_blocks(cache, k[:, :-1].contiguous().to(DEV), v[:, :-1].contiguous().to(DEV))
+    cache.seq_lens += 1
+    v[:, -1] = 2.0 ** power
+    pkg.append_blocks(cache, k[:, -1:].to(DEV), v[:, -1:].to(DEV))
+    # tiles go round a unit's warps in order, and a warp has several: behind the first it starts with what it has
+    first = torch.arange(B, dtype=torch.int32, device=DEV)
+    sides, table = _sides(cache), cache.block_table.cpu()
+    q = _random((B, 2, Hq, dh), 3, torch.float16)
+    got = pkg.attend_blocks(q.to(DEV), cache, first=first, out_dtype=torch.float32)
+    for b in (0, 1, 7):
+        kk, vv = (s.rows(table[b], b, ctx) for s in sides)
+        for i in (0, 1):
+            n = ctx - 1 + i
+            want, _, _, off, _, _ = orc.attend(q[b, i:i + 1], kk[:n - b], vv[:n - b], b, [n - 1], 1 / math.sqrt(dh))
+            scales = _scales(sides[1], table[b], b, n).clone()
+            if i == 0:
+                scales[-(N - 1):] = 0  # its page's scale is large, its values there are zeros
+            _check(got[b, i:i + 1], want, off + _least(q[b, i:i + 1], kk[:n - b], 1 / math.sqrt(dh), [n - 1], scales, 127.0, b), torch.float32)
+    pkg.check_status(cache)
+
+
+def test_decode_scales_at_both_ends(pkg):
+    """Value scales from 2^-126 to 2^120, pages of zeros that outweigh all others by far, and a page of large values 2^100 lighter."""
+    H, Hq, N, dh, ctx, B = 8, 16, 16, 64, 4000, 8
+    direction = torch.sign(_random((1, 1, dh), 9, torch.float32))
+    q = direction + 0.05 * _random((B, Hq, dh), 3, torch.float32)
+    tile = torch.arange(ctx) // 128
+    for small, large, light, zero in ((-119, 119, 250, 0), (-20, 100, 100, 60), (-118, -118, 0, 100), (0, 0, 0, 230), (-110, 0, 105, 20), (0, 112, 108, 0)):
+        k, v = 0.05 * _random((B, ctx, H, dh), 5, torch.float32), _random((B, ctx, H, dh), 6, torch.float32).clamp(-4, 4)
+        v = v.double() * 2.0 ** small
+        lift = torch.zeros(ctx)
+        big, none = tile % 4 == 1, tile % 4 == 2
+        v[:, big] *= 2.0 ** (large - small)
+        v[:, none] = 0
+        lift[big], lift[none] = -light, zero  # log2 of how much heavier a page's tokens are
+        k += direction * (lift * math.log(2) / dh ** 0.5)[:, None, None]
+        v = v.float()
+        assert v.isfinite().all()
+        cache = _cache(pkg, [ctx] * B, H, N, dh, I8, 67)
+        pkg.append_blocks(cache, k.to(DEV), v.to(DEV))
+        sides, table = _sides(cache), cache.block_table.cpu()
+        got = pkg.decode_blocks(q.to(DEV), cache)
+        for b in (0, 7):
+            kk, vv = (s.rows(table[b], 0, ctx) for s in sides)
+            want, _, _, off, _, _ = orc.attend(q[b:b + 1], kk, vv, 0, [ctx - 1], 1 / math.sqrt(dh))
+            least = _least(q[b:b + 1], kk, 1 / math.sqrt(dh), [ctx - 1], _scales(sides[1], table[b], 0, ctx), 127.0)
+            # p and the factors between parts are fp32 numbers: below 2^-126 of the row's largest p (its reference may be one power of two above
+            # that) they are 0, whatever they are multiplied by
+            x = torch.einsum("hgd,thd->hgt", q[b].double().view(H, Hq // H, dh), kk).reshape(Hq, ctx) / math.sqrt(dh)
+            w = torch.exp(x - x.amax(1, keepdim=True))
+            lost = torch.einsum("ht,thd->hd", w.masked_fill(w > 2.0 ** -125, 0.0), vv.abs().repeat_interleave(2, 1)) / w.sum(1, keepdim=True)
+            least = least + lost + 2.0 ** -149
+            _check(got[b:b + 1], want, off + least, torch.float32)
+        pkg.check_status(cache)
