@@ -5,6 +5,8 @@
 // same registers, so tokens are read once.  Measured (32768 bf16 tokens, 16-token pages, int8, cold caches): append 47 us where
 // the bytes take 31 at the copy rate, bound by instructions (16.8 an element, 70 % of issue slots at 43 % of the warps; 64 registers a thread give
 // four blocks an SM, 5 % faster than three); read 34 us, as long as the bytes take.  Steps of one token are latency: 3 us each.
+#include <type_traits>
+
 #include "blocks.cuh"
 
 namespace sphkv {
@@ -20,14 +22,16 @@ struct BlocksIo {
 };
 
 constexpr int kIoThreads = 256;  // eight warps, each with 16 tokens of one (page, side, head)
+constexpr float kLeastScale = 0x1p-110f, kLift = 0x1p64f;  // scale times border has a last bit of 2^-33 of the scale, and fp32 ends at 2^-149
 constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds |q| < 2^22 to a whole number, ties to even
 
 // ---- nearest 8-bit codes -----------------------------------------------------------------------------------
 // q approximates the quotient to 1.5 ulp (a rounded reciprocal or ratio, one product).  Where that leaves the nearest code
 // open, within 2^-15 of a whole number's border or 4 ulp of an e4m3 border, the sign of x - border * s decides, which one fma gives
-// exactly: a border has 8 bits at most, the product 32, and a rounding keeps the sign.  bf16 tokens lie exactly on borders
-// often, since scale and token are quotients of 8-bit numbers: some word of most rows is open, and 64-bit division there was half of
-// the kernel's instructions.
+// exactly: a border has 8 bits at most, the product 32, and a rounding keeps the sign of what is not below fp32's least number (so
+// the smallest scales and their tokens are multiplied by a power of two first).  bf16 tokens lie exactly on borders often, since scale
+// and token are quotients of 8-bit numbers: some word of most rows is open, and 64-bit division there was half of the kernel's
+// instructions.
 template <bool I8>
 __device__ uint32_t code_of_double(double q) {
   if constexpr (I8) return (uint32_t)(int)rint(q) & 0xffu;
@@ -288,25 +292,33 @@ __global__ void __launch_bounds__(kIoThreads, sizeof(T) * DH == 512 ? 2 : 4) blo
   }
   if (t.part == 0 && lane == 0 && grown) *scale_at = s;  // parts > 1: all have read s_old before the barrier
   const bool finite = (__float_as_uint(s) & 0x7f800000u) != 0x7f800000u && s != 0.f;
-  const float inv = finite ? __frcp_rn(s) : 0.f;
+  auto round_new = [&](auto lifted, float by, float inv) {
 #pragma unroll
-  for (int i = 0; i < L; ++i) {
-    const int row = i * RPL + lane / LPR;
-    if (row < first_new || row >= end) continue;
-    uint32_t w[E / 4];
-    float f[E];
-    Chunk<T>::floats(raw[i], f);
+    for (int i = 0; i < L; ++i) {
+      const int row = i * RPL + lane / LPR;
+      if (row < first_new || row >= end) continue;
+      uint32_t w[E / 4];
+      float f[E];
+      Chunk<T>::floats(raw[i], f);
+      if constexpr (decltype(lifted)::value)
 #pragma unroll
-    for (int k = 0; k < E / 4; ++k) {
-      w[k] = 0;
-      if (finite) w[k] = nearest4<I8, true>(f + 4 * k, inv, 1.f, s);
+        for (int k = 0; k < E; ++k) f[k] *= kLift;
+#pragma unroll
+      for (int k = 0; k < E / 4; ++k) {
+        w[k] = 0;
+        if (finite) w[k] = nearest4<I8, true>(f + 4 * k, inv, 1.f, by);
+      }
+      uint8_t* to = codes + row * DH + (lane % LPR) * E;
+      if constexpr (E == 8)
+        *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+      else
+        *reinterpret_cast<uint32_t*>(to) = w[0];
     }
-    uint8_t* to = codes + row * DH + (lane % LPR) * E;
-    if constexpr (E == 8)
-      *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-    else
-      *reinterpret_cast<uint32_t*>(to) = w[0];
-  }
+  };
+  if (s < kLeastScale)  // the whole warp: a branch of its own, since a product more per element is 2 % of the kernel
+    round_new(std::true_type(), s * kLift, finite ? __frcp_rn(s * kLift) : 0.f);
+  else
+    round_new(std::false_type(), s, finite ? __frcp_rn(s) : 0.f);
   if (holds && grown) {
     const float ratio = finite ? __fdiv_rn(s_old, s) : 0.f;
 #pragma unroll

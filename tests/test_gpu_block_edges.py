@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_blocks import DEV, E4M3, I8, _cache, _check, _cu, _filled, _random, _sides
+from test_gpu_blocks import DEV, E4M3, I8, _cache, _check, _cu, _filled, _random, _same, _sides
 import blocks_oracle as orc
 
 pytestmark = pytest.mark.gpu
@@ -321,3 +321,32 @@ def test_decode_scales_at_both_ends(pkg):
             least = least + lost + 2.0 ** -149
             _check(got[b:b + 1], want, off + least, torch.float32)
         pkg.check_status(cache)
+
+
+@pytest.mark.parametrize("store", [I8, E4M3])
+def test_nearest_codes_of_the_smallest_scales(pkg, store):
+    """Scales a few powers of two above 2^-126, tokens a unit of 2^-149 beside the borders between codes: differences that fp32 has no
+    number for."""
+    top, dh, n = orc.TOP[store], 64, 48
+    unit = 2.0 ** -149
+    rows = []
+    for i in range(n):
+        scale = (2 ** 23 + 2 * (3 * i * i * 7919 % (2 ** 22)) + 1) * 2 ** (i // 16)
+        largest = torch.tensor(scale * top, dtype=torch.float64).mul(unit).float()
+        s = orc.f32_quotient(largest, top).double() / unit
+        codes = torch.arange(0, 127, dtype=torch.uint8).view(E4M3).double() if store is E4M3 else torch.arange(0, 127).double()
+        border = (codes[1:] + codes[:-1]) / 2 * s
+        border = border[border < 2 ** 24][:31 * (2 if store is E4M3 else 1)]
+        pick = border[torch.randperm(border.numel(), generator=torch.Generator().manual_seed(i))[:31]]
+        x = torch.cat([torch.floor(pick), torch.ceil(pick)])
+        x = torch.cat([torch.tensor([float(largest) / unit], dtype=torch.float64), x, torch.zeros(dh - 1 - x.numel(), dtype=torch.float64)])
+        rows.append((x * unit).float())
+    rows = torch.stack(rows)[:, None]
+    cache = _cache(pkg, [1] * n, 1, 16, dh, store, 3, max_len=[1] * n)
+    table, sides = cache.block_table.cpu(), _sides(cache)
+    pkg.append_blocks(cache, rows[:, None].to(DEV), -rows[:, None].to(DEV))
+    for b in range(n):
+        sides[0].append(table[b], 1, rows[b:b + 1])
+        sides[1].append(table[b], 1, -rows[b:b + 1])
+    _same(cache, sides, table, [1] * n)
+    pkg.check_status(cache)
