@@ -412,14 +412,14 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
           };
           if (down != 1.f) {
             // S has grown.  The row's reference goes the other way, so that O stays as it is; where the sum would grow past
-            // 32 bits (or all scales were 0) O shrinks instead.
+            // 32 bits (or all scales were 0) O shrinks instead, row by row.
             const int e = (int)(__float_as_uint(down) >> 23) - 127;  // a power of two
             const float grown = l * __uint_as_float((uint32_t)(127 - max(e, -80)) << 23);
-            if (e >= -80 && !__any_sync(0xffffffffu, grown > 0x1p110f)) {
+            const bool stays = e >= -80 && !(grown > 0x1p110f);
+            if (__any_sync(0xffffffffu, !stays)) move(m, stays ? 1.f : down, 0);
+            if (stays) {
               m += (float)e;
               l = grown;
-            } else {
-              move(m, down, 0);
             }
           }
           if (edge) {

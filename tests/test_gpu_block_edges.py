@@ -350,3 +350,26 @@ def test_nearest_codes_of_the_smallest_scales(pkg, store):
         sides[1].append(table[b], 1, -rows[b:b + 1])
     _same(cache, sides, table, [1] * n)
     pkg.check_status(cache)
+
+
+def test_value_scale_reference_moves_row_by_row(pkg):
+    """Thirty-two rows of a warp: the first see only values of 2^-75, so that their sums cannot follow the value scales' reference when it grows
+    by 2^40 for a page that none of them sees; the last, which see that tile's first keys, keep their bits all the same."""
+    B, H, N, dh, n = 20, 16, 16, 64, 64
+    ctx = 100 + n
+    cache = _cache(pkg, [ctx] * B, H, N, dh, I8, 97)
+    k, v = _random((B, ctx, H, dh), 5, torch.float32), _random((B, ctx, H, dh), 6, torch.float32)
+    v[:, :112] *= 2.0 ** -75
+    v[:, 144:] *= 2.0 ** 40
+    pkg.append_blocks(cache, k.to(DEV), v.to(DEV))
+    sides, table = _sides(cache), cache.block_table.cpu()
+    q = _random((B, n, H, dh), 3, torch.float16)
+    got = pkg.attend_blocks(q.to(DEV), cache, out_dtype=torch.float32)
+    for b in range(0, B, 5):
+        kk, vv = (s.rows(table[b], 0, ctx) for s in sides)
+        for lo, hi in ((0, 12), (12, 44), (44, 64)):
+            last = 100 + hi
+            want, _, _, off, size, _ = orc.attend(q[b, lo:hi], kk[:last], vv[:last], 0, list(range(100 + lo, last)), 0.125)
+            least = _least(q[b, lo:hi], kk[:last], 0.125, list(range(100 + lo, last)), _scales(sides[1], table[b], 0, last), 127.0)
+            _check(got[b, lo:hi], want, off + HALF16 * size + least, torch.float32)
+    pkg.check_status(cache)
