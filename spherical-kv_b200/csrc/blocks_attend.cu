@@ -745,10 +745,10 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
           }
           const float ref = big > 0.f ? big : 1.f;
           // The sum of weights takes v out again, which 32 bits allow down to 2^-80: values that are smaller still count as zeros,
-          // like those of scale 0, and v is what serves.
+          // like those of scale 0.  Theirs is the smallest v, so that they do not raise a row's reference above what it sees of others.
           float v = vs_now * (1.f / ref);
           const bool zeros = v < 0x1p-80f;
-          if (zeros) v = 1.f;
+          if (zeros) v = 0x1p-80f;
           bad |= (__ballot_sync(0xffffffffu, there && zeros) & 0xffu) << 8;
           // as far ahead as keys may be: the softmax has left tile n - 3 behind, and this place held n - 4
           if (n >= 2 && !warp_wait(kKFree + (n & 1), (n >> 1) - 1)) break;

@@ -373,3 +373,26 @@ def test_value_scale_reference_moves_row_by_row(pkg):
             least = _least(q[b, lo:hi], kk[:last], 0.125, list(range(100 + lo, last)), _scales(sides[1], table[b], 0, last), 127.0)
             _check(got[b, lo:hi], want, off + HALF16 * size + least, torch.float32)
     pkg.check_status(cache)
+
+
+@pytest.mark.parametrize("power", [20, 40, 70])
+def test_attend_zeros_beside_small_values(pkg, power):
+    """Values far below the sequence's largest, which only later rows see, between pages of zeros: the zeros take no bits from them."""
+    H, N, dh, Hq, ctx, n = 1, 16, 64, 8, 384, 150
+    cache = _cache(pkg, [ctx], H, N, dh, I8, 97)
+    k, v = _random((ctx, H, dh), 5, torch.float32), _random((ctx, H, dh), 6, torch.float32)
+    page = torch.arange(ctx) // N
+    v[page % 3 == 1] = 0
+    v[ctx - N:] *= 2.0 ** power  # seen by the last 16 rows
+    pkg.append_blocks(cache, k.to(DEV), v.to(DEV), cu_new=_cu([ctx]))
+    sides, table = _sides(cache), cache.block_table.cpu()
+    kk, vv = (s.rows(table[0], 0, ctx) for s in sides)
+    q = _random((n, Hq, dh), 3, torch.float16)
+    got = pkg.attend_blocks(q.to(DEV), cache, cu_new=_cu([n]), out_dtype=torch.float32)
+    for lo, hi in ((0, n - N), (n - N, n)):
+        want, _, _, off, size, _ = orc.attend(q[lo:hi], kk, vv, 0, list(range(ctx - n + lo, ctx - n + hi)), 0.125)
+        last = ctx - n + hi
+        # weights below 2^-14 are off by 2^-25 where the row's largest weight times scale is 2^6 at least: 2^-31 of the largest, for each key
+        tiny = last * 2.0 ** -31 * float(vv[:last].abs().max())
+        _check(got[lo:hi], want, off + HALF16 * size + tiny, torch.float32)
+    pkg.check_status(cache)
