@@ -394,6 +394,10 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
                 tmem_st_x16(o_at + 16 * i, o);
               }
             }
+            // Two factors: f16 has no bits for d below 2^-14, where weights (2^14 at most) lose 2^-25 by the first (in fp32: 104.6 us for the
+            // five pieces instead of 102.8).
+            const float most = fmaxf(d, 0x1p-14f), rest = fminf(d * 0x1p14f, 1.f);
+            const uint32_t d1 = pack_f16x2(most, most), d2 = pack_f16x2(rest, rest);
             tmem_wait_st();
 #pragma unroll 1
             for (int h = 0; h < done; ++h) {
@@ -403,8 +407,9 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
 #pragma unroll
               for (int c = 0; c < 16; ++c) {
                 const uint32_t v = __float_as_uint(w[c]);
-                const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&v));
-                w[c] = __uint_as_float(pack_f16x2(x.x * d, x.y * d));  // d in f16 would lose its bits below 2^-14
+                const __half2 r = __hmul2(__hmul2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&d1)),
+                                          *reinterpret_cast<const __half2*>(&d2));
+                w[c] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&r));
               }
               tmem_st_x16(s_at + 16 * h, w);
             }
