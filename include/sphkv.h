@@ -291,7 +291,8 @@ int sphkv_xchg_free(void* dev_ptr);
 
 /* Log-sum-exp combine of R partial sets, each f32 [n_rows][dh+2] = (max, sum, acc),
  * natural-log max.  Same math as sphkv_reduce_kernel (decode_kernel.cu:221-246) with a
- * plain division (no +1e-8); rows whose total sum is 0 produce zeros.  Used after the
+ * plain division (no +1e-8); rows whose total sum is 0 produce zeros, rows with a NaN sum in any
+ * set produce NaN.  Used after the
  * all-gather of per-GPU partials in split-KV decode.  parts: [R][n_rows][dh+2]. */
 int sphkv_merge_partials(const float* parts, int32_t R, int32_t n_rows, int32_t dh, void* out,
                          int32_t out_dtype, void* stream);

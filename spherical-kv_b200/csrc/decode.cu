@@ -337,9 +337,11 @@ __global__ void merge_partials_kernel(const float* __restrict__ parts, int R, in
   const int row = blockIdx.x;
   const int64_t stride = (int64_t)n_rows * (dh + 2);
   float M = -INFINITY;
+  bool nan = false;  // in one set: the row of all sets together has no value either
   for (int rr = 0; rr < R; ++rr) {
     const float* pr = parts + rr * stride + (int64_t)row * (dh + 2);
     if (pr[1] > 0.f) M = fmaxf(M, pr[0]);
+    nan |= isnan(pr[1]);
   }
   for (int d = threadIdx.x; d < dh; d += blockDim.x) {
     float l = 0.f, o = 0.f;
@@ -352,7 +354,7 @@ __global__ void merge_partials_kernel(const float* __restrict__ parts, int R, in
         o += pr[2 + d] * w;
       }
     }
-    store_from_float(out, out_dtype, (int64_t)row * dh + d, l > 0.f ? o / l : 0.f);
+    store_from_float(out, out_dtype, (int64_t)row * dh + d, nan ? NAN : l > 0.f ? o / l : 0.f);
   }
 }
 

@@ -284,7 +284,8 @@ def check_status(cache) -> None:
 def merge_partials(parts: torch.Tensor, out_dtype: torch.dtype = torch.float32,
                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """parts f32 [R, n_rows, dh+2] -> [n_rows, dh]; log-sum-exp combine
-    (decode_kernel.cu:221-246 without the +1e-8)."""
+    (decode_kernel.cu:221-246 without the +1e-8).  A row whose sum is 0 in a set is not in it, and one whose sum is NaN in
+    any set is NaN."""
     lib = _lib.load()
     _need_cuda(parts, out)
     R, n_rows, w = parts.shape

@@ -396,3 +396,30 @@ def test_attend_zeros_beside_small_values(pkg, power):
         tiny = last * 2.0 ** -31 * float(vv[:last].abs().max())
         _check(got[lo:hi], want, off + HALF16 * size + tiny, torch.float32)
     pkg.check_status(cache)
+
+
+def test_nan_reaches_the_merge_with_another_cache(pkg):
+    """A page that reads back as NaN makes its decode's rows NaN, with however few keys, and so the rows of both caches together."""
+    H, N, dh, Hq, ctx = 2, 16, 128, 4, 2000
+    cache = _filled(pkg, [ctx, ctx, 16, ctx], H, N, dh, I8, 71)
+    q = _random((4, Hq, dh), 3, torch.float32).to(DEV)
+    other = torch.randn(4, Hq, dh + 2, device=DEV)
+    other[..., 1] = 2.0
+    for scales in (cache.k_scale, cache.v_scale):
+        clean = scales.clone()
+        scales[cache.block_table[1, 77].long(), 0] = math.nan
+        scales[cache.block_table[2, 0].long(), 0] = math.nan
+        parts = torch.empty(2, 4, Hq, dh + 2, device=DEV)
+        parts[0] = other
+        out = pkg.decode_blocks(q, cache, out_partial=parts[1])
+        merged = pkg.merge_partials(parts.view(2, 4 * Hq, dh + 2)).view(4, Hq, dh)
+        for x in (out, merged):
+            for b in range(4):
+                assert x[b, 2:].isfinite().all(), b
+                assert x[b, :2].isnan().all() if b in (1, 2) else x[b].isfinite().all(), b
+        # nothing in the other one
+        parts[0, ..., 0], parts[0, ..., 1:] = -math.inf, 0.0
+        merged = pkg.merge_partials(parts.view(2, 4 * Hq, dh + 2)).view(4, Hq, dh)
+        assert torch.equal(merged.isnan(), out.isnan())
+        scales.copy_(clean)
+    pkg.check_status(cache)
