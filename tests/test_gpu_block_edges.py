@@ -423,3 +423,50 @@ def test_nan_reaches_the_merge_with_another_cache(pkg):
         assert torch.equal(merged.isnan(), out.isnan())
         scales.copy_(clean)
     pkg.check_status(cache)
+
+
+def test_negative_first_is_none(pkg):
+    cache = _filled(pkg, [40, 700], 2, 16, 64, I8, 29)
+    first = torch.tensor([-5, -2 ** 31], dtype=torch.int32, device=DEV)
+    q = _random((2, 100, 4, 64), 3, torch.bfloat16).to(DEV)
+    for n in (1, 30):
+        assert torch.equal(pkg.attend_blocks(q[:, :n].contiguous(), cache, first=first), pkg.attend_blocks(q[:, :n].contiguous(), cache))
+    assert torch.equal(pkg.decode_blocks(q[:, 0], cache, first=first), pkg.decode_blocks(q[:, 0], cache))
+    pkg.check_status(cache)
+
+
+def test_two_threads(pkg):
+    """Calls from two threads at once, each on a stream and a cache of its own."""
+    import threading
+    caches = [_filled(pkg, [40, 700], 2, 16, 64, I8, 29 + i) for i in (0, 1)]
+    q = _random((2, 40, 4, 64), 3, torch.bfloat16).to(DEV)
+    want = [(pkg.attend_blocks(q, c), pkg.decode_blocks(q[:, 0], c), pkg.read_blocks(c, n=40)[1]) for c in caches]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(50):
+                got = (pkg.attend_blocks(q, caches[i]), pkg.decode_blocks(q[:, 0], caches[i]), pkg.read_blocks(caches[i], n=40)[1])
+                bad.extend(i for a, b in zip(got, want[i]) if not torch.equal(a, b))
+        stream.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+    for c in caches:
+        pkg.check_status(c)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_another_device_than_the_current_one(pkg):
+    import copy
+    cache = _filled(pkg, [40, 700], 2, 16, 64, I8, 29)
+    other = pkg.BlockCache(**{k: t.to("cuda:1") for k, t in copy.copy(cache.__dict__).items()})
+    q = _random((2, 30, 4, 64), 3, torch.bfloat16).to(DEV)
+    assert torch.equal(pkg.attend_blocks(q.to("cuda:1"), other).to(DEV), pkg.attend_blocks(q, cache))
+    assert torch.cuda.current_device() == 0
+    pkg.check_status(other)
