@@ -148,16 +148,6 @@ def read_blocks(cache: BlockCache, n: Optional[int] = None, cu_rows: Optional[to
                  _type(torch.float32 if out_dtype is None else out_dtype), k, v)
 
 
-def _output(out: Optional[torch.Tensor], shape, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
-    if out is None:
-        if dtype not in _DT:
-            _err("out_dtype: float32, bfloat16 or float16")
-        return torch.empty(shape, dtype=dtype, device=dev)
-    if out.shape != shape or out.dtype not in _DT or out.device != dev or not out.is_contiguous():
-        _err(f"out: expected a contiguous tensor {tuple(shape)} on {dev}")
-    return out
-
-
 def decode_blocks(q: torch.Tensor, cache: BlockCache, first: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None,
                   out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
                   out_partial: Optional[torch.Tensor] = None, want_out: bool = True) -> Optional[torch.Tensor]:
