@@ -41,7 +41,9 @@ constexpr int kAtProducts = 16;
 // five warps each (two of softmax, two of codes, one of 16 .. 19), so what goes up has to come down quarter by quarter.
 constexpr int kAtRegs = 96, kAtRegsSoftmax = 136, kAtRegsCodes = 72, kAtRegsRest = 64;
 static_assert(2 * kAtRegsSoftmax + 2 * kAtRegsCodes + kAtRegsRest <= 5 * kAtRegs && 20 * 32 * kAtRegs <= 65536, "registers");
-constexpr float kAtWeight = 6.f, kAtLazy = 14.f;  // log2 of the largest weight where the reference moves, and where it does not yet
+// log2 of the largest weight where the reference moves, to the whole number above (below: it moves more often, 2 % more in all), and where
+// it does not yet
+constexpr float kAtWeight = 6.f, kAtLazy = 14.f;
 
 struct AtArgs {
   sphkv_blocks c;
@@ -394,8 +396,8 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
                 tmem_st_x16(o_at + 16 * i, o);
               }
             }
-            // Two factors: f16 has no bits for d below 2^-14, where weights (2^14 at most) lose 2^-25 by the first (in fp32: 104.6 us for the
-            // five pieces instead of 102.8).
+            // References are whole numbers, so d is a power of two and weights stay rounded once, but for what falls below f16's normal
+            // numbers: 2^-25.  Two factors, as d itself may lie there (one product in fp32: 104.6 us for the five pieces instead of 102.8).
             const float most = fmaxf(d, 0x1p-14f), rest = fminf(d * 0x1p14f, 1.f);
             const uint32_t d1 = pack_f16x2(most, most), d2 = pack_f16x2(rest, rest);
             tmem_wait_st();
@@ -443,7 +445,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
               top = fmaf(top, of.x * f, of.y);
               const bool up = top > m + kAtLazy;
               // 16 keys are half of what move() counts in: an odd group's first half has not been stored yet
-              if (__any_sync(0xffffffffu, up)) move(up ? top - kAtWeight : m, 1.f, (g + 1) >> 1);
+              if (__any_sync(0xffffffffu, up)) move(up ? ceilf(top - kAtWeight) : m, 1.f, (g + 1) >> 1);
               float all = 0.f;
               uint32_t p[8];
 #pragma unroll
@@ -482,7 +484,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) blocks_attend_kernel(const __gr
 #pragma unroll 1
             for (int h = 0; h < 4; ++h) {
               const bool up = mx > m + kAtLazy;
-              if (__any_sync(0xffffffffu, up)) move(up ? mx - kAtWeight : m, 1.f, h);
+              if (__any_sync(0xffffffffu, up)) move(up ? ceilf(mx - kAtWeight) : m, 1.f, h);
               float2 e[16], part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
               uint32_t p[16];
 #pragma unroll

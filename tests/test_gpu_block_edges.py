@@ -1,5 +1,6 @@
 """The 8-bit block cache on the GPU where it can go wrong: what the other tests of it do not reach."""
 import math
+import random
 
 import pytest
 import torch
@@ -470,3 +471,64 @@ def test_another_device_than_the_current_one(pkg):
     assert torch.equal(pkg.attend_blocks(q.to("cuda:1"), other).to(DEV), pkg.attend_blocks(q, cache))
     assert torch.cuda.current_device() == 0
     pkg.check_status(other)
+
+
+@pytest.mark.parametrize("seed", [1998, 5876, 6861, 10839] + list(range(40)))
+def test_drawn_batches(pkg, seed):
+    """Batches of any lengths, groups, pages, rows before and behind, firsts whose older pages are gone, scales of either sign and values over up
+    to forty powers of two: attend and decode within the bounds of fp32 sums and of weights that are rounded once (attend: to f16)."""
+    r = random.Random(seed)
+    H, group = r.choice([1, 2, 3, 4]), r.choice([1, 2, 3, 4, 5, 6, 7, 8])
+    Hq, N, dh, store = H * group, r.choice([16, 32, 64, 128]), r.choice([64, 128]), r.choice([I8, E4M3])
+    B = r.choice([1, 1, 2, 3, 5, 9, 40, 150])
+    top = r.choice([40, 300, 900]) if B < 20 else r.choice([20, 90])
+    lens = [r.choice([0, 1, r.randint(0, top), r.randint(0, top), r.randint(top // 2, top)]) for _ in range(B)]
+    dtype = r.choice([torch.bfloat16, torch.float16])
+    out_dtype = r.choice([dtype, torch.float32])
+    most = r.choice([1, 3, 8, 40, 300])
+    news = [min(x, r.choice([0, 1, r.randint(0, most), most])) for x in lens]
+    first = [r.choice([0, -1, x, x + 5, r.randint(0, max(x, 1))]) for x in lens] if r.random() < 0.5 else None
+    sm_scale = r.choice([None, None, 0.05, -0.2, 0.3])
+    powers = r.choice([0, 0, 6, 20])
+    cache = _cache(pkg, lens, H, N, dh, store, seed + 1)
+    total = sum(lens)
+    k, v = _random((total, H, dh), seed + 6, torch.float32), _random((total, H, dh), seed + 7, torch.float32)
+    if powers and total:
+        spread = torch.rand(total // 16 + 1, 1, 1, generator=torch.Generator().manual_seed(seed + 1)).repeat_interleave(16, 0)[:total]
+        v = v * torch.exp2(powers * (2 * spread - 1))
+    pkg.append_blocks(cache, k.to(DEV), v.to(DEV), cu_new=_cu(lens))
+    sides, table = _sides(cache), cache.block_table.cpu()
+    if first and r.random() < 0.5:
+        for b in range(B):
+            if first[b] < lens[b]:
+                cache.block_table[b, :max(0, first[b]) // N] = -1
+    f = None if first is None else torch.tensor(first, dtype=torch.int32, device=DEV)
+    lead, tail = r.choice([0, 0, 3, 77]), r.choice([0, 2])
+    rows = lead + sum(news) + tail
+    wide = _random((rows, Hq + 1, dh + 8), seed + 8, dtype).to(DEV)
+    off = r.choice([0, 1, 8])
+    head = r.choice([0, 1])
+    q = wide[:, head:head + Hq, off:off + dh]
+    out = torch.full((rows, Hq, dh), 7.0, dtype=out_dtype, device=DEV)
+    pkg.attend_blocks(q, cache, cu_new=_cu(news) + lead, first=f, sm_scale=sm_scale, out=out)
+    q1 = _random((B, Hq, dh), seed + 9, r.choice([torch.float32, dtype]))
+    got1 = pkg.decode_blocks(q1.to(DEV), cache, first=f, sm_scale=sm_scale, out_dtype=torch.float32)
+    pkg.check_status(cache)
+    assert (out[:lead] == 7.0).all() and (out[rows - tail:] == 7.0).all()
+    at, scale, largest = lead, 1 / math.sqrt(dh) if sm_scale is None else sm_scale, torch.finfo(out_dtype).max
+    sign = -1 if scale < 0 else 1
+    for b in range(B):
+        n, end, lo = news[b], lens[b], 0 if first is None else min(max(first[b], 0), lens[b])
+        at += n
+        if B > 9 and b % 29:
+            continue
+        kk, vv = (s.rows(table[b], lo, end).reshape(-1, H, dh) for s in sides)
+        scales = _scales(sides[1], table[b], lo, end).reshape(-1, H)
+        qs = q[at - n:at].cpu()
+        for qq, pos, got, half in ((qs, list(range(end - n, end)), out[at - n:at], HALF16), (q1[b:b + 1], [end - 1], got1[b:b + 1], 0.0)):
+            if not pos:
+                continue
+            want, _, _, bound, size, _ = orc.attend(sign * qq, kk, vv, lo, pos, abs(scale))
+            fits = want.abs() < 0.99 * largest  # beyond, f16 has infinities
+            least = _least(qq, kk, scale, pos, scales, orc.TOP[store], lo)
+            _check(torch.where(fits.to(DEV), got.double(), want.to(DEV)), want, bound + half * size + least, got.dtype)
