@@ -405,7 +405,7 @@ int sphkv_omega_ema(const float* ml, float* omega, int32_t n_units, int32_t kv_g
 /* ---- 8-bit block cache ----------------------------------------------------------------
  * Keys and values in 8 bits with one fp32 scale for each page (block of page_size tokens), head
  * and side, for tokens that are not held in spherical pages.  No counterpart in the reference.
- * A value is code * scale; codes are whole numbers -127 .. 127 or e4m3 floats.  Token t of
+ * A value is code * scale; codes are whole numbers -127 .. 127 or finite e4m3 floats.  Token t of
  * sequence b lies in slot t % page_size of page block_table[b][t / page_size]; a page holds all KV
  * heads of its tokens.  Keys are stored as they come (post-RoPE for sphkv_blocks_decode / _attend).
  *
@@ -462,8 +462,10 @@ int sphkv_blocks_decode(const sphkv_blocks* c, const void* q, int32_t q_dtype, i
 
 /* Causal attention of the last n_b tokens of every sequence: the query at position p sees keys
  * first[b] .. p.  q [rows][Hq][dh] (16-bit types), out [rows][Hq][dh] contiguous; a query without keys gets zeros.
- * Rows past cu[B] are not written.  sm_scale here and in sphkv_blocks_decode: any finite number.  Values below 2^-80 of the
- * largest value scale that the sequence has count as zeros. */
+ * Padding rows are not written.  Softmax weights are rounded to f16 once, and values below 2^-80 of the largest value
+ * scale that the sequence has count as zeros; where rows <= B * n, n the largest power of two with n * Hq / Hkv <= SPHKV_MAX_GQA,
+ * the kernel of sphkv_blocks_decode takes the call, whose errors are those of fp32 sums.  sm_scale here and there: any
+ * finite number. */
 int64_t sphkv_blocks_attend_scratch_bytes(int32_t B, int64_t rows, int32_t Hq, int32_t Hkv, int32_t dh);
 int sphkv_blocks_attend(const sphkv_blocks* c, const void* q, int32_t q_dtype, int64_t q_row_stride,
                         int64_t q_head_stride, const int32_t* cu, int64_t rows, const int32_t* first, void* out,

@@ -35,7 +35,8 @@ _STORE = {torch.int8: _lib.BLOCKS_I8, torch.float8_e4m3fn: _lib.BLOCKS_E4M3}
 
 @dataclass
 class BlockCache:
-    """Device-resident 8-bit cache of one attention layer.  A value is code * scale."""
+    """Device-resident 8-bit cache of one attention layer.  A value is code * scale; codes of a sequence's tokens are finite (append_blocks
+    writes no others: a token without a finite value is a scale that is not finite)."""
     k_codes: torch.Tensor      # i8 | float8_e4m3fn [n_pages, Hkv, page_size, dh]
     v_codes: torch.Tensor      # the same
     k_scale: torch.Tensor      # f32 [n_pages, Hkv]
@@ -123,8 +124,8 @@ def _type(dtype: Optional[torch.dtype]) -> int:
 def append_blocks(cache: BlockCache, k: torch.Tensor, v: torch.Tensor, cu_new: Optional[torch.Tensor] = None) -> None:
     """Quantises the last n_b tokens of every sequence into its pages.
 
-    k, v: [B, n, Hkv, dh], or [rows, Hkv, dh] with cu_new; f32, bf16 or f16, elements of a head contiguous, other strides as
-    they come (slices of a fused projection).  seq_lens counts the new tokens already.  A page keeps one scale per head and
+    k, v: [B, n, Hkv, dh], or [rows, Hkv, dh] with cu_new; f32, bf16 or f16, elements of a head contiguous, rows of all sequences
+    one stride apart, other strides as they come (slices of a fused projection).  seq_lens counts the new tokens already.  A page keeps one scale per head and
     side, max |x| / 127 (e4m3: / 448) of all it was given: where new tokens raise it, the page's earlier tokens of the sequence are
     re-quantised.  Codes are the nearest to x / scale, ties to even.  An infinity or NaN makes its page, head and side read
     back as NaN.  A page that is appended to belongs to one sequence, and stands once in its row of the table."""
@@ -136,7 +137,9 @@ def read_blocks(cache: BlockCache, n: Optional[int] = None, cu_rows: Optional[to
                 out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Keys and values of a run of tokens of every sequence as dense rows: the last `n` (-> [B, n, Hkv, dh]), or cu_rows[b + 1]
     - cu_rows[b] of them (-> [rows, Hkv, dh], `rows` the host's bound of cu_rows[B]).  `ends` (int32 [B]) takes the tokens
-    before position ends[b] instead of before seq_lens[b]: encode_pages can take them as they come out."""
+    before position ends[b] instead of before seq_lens[b].  The rows have the layout that encode_pages takes, and the keys are what
+    was appended: post-RoPE ones make pages that are decoded with decode_paged(rope=None); a decode with a RoPE table expects pages
+    of pre-RoPE keys."""
     if (n is None) == (cu_rows is None):
         raise _lib.SphKVError("read_blocks: either n, or cu_rows with rows")
     k, v = out if out is not None else (None, None)
@@ -153,7 +156,8 @@ def decode_blocks(q: torch.Tensor, cache: BlockCache, first: Optional[torch.Tens
                   out_partial: Optional[torch.Tensor] = None, want_out: bool = True) -> Optional[torch.Tensor]:
     """Attention of one query a sequence, q [B, Hq, dh] (f32, bf16, f16), over its tokens first[b] .. seq_lens[b] - 1 (first:
     int32 [B], None = 0).  Returns [B, Hq, dh]; zeros where a sequence has no such token.  `out_partial` (f32 [B, Hq, dh + 2])
-    receives (max, sum, acc), un-normalised, as decode_paged writes them."""
+    receives (max, sum, acc), un-normalised, as decode_paged writes them.  sm_scale: any finite number, None = 1 / sqrt(dh).  Errors are
+    those of fp32 sums, whatever scales stand beside one another."""
     return _call("decode", cache, cache.seq_lens, (_calls or _bind())["scratch"][0], q, first, sm_scale,
                  _type(out_dtype), out, out_partial, want_out)
 
@@ -162,7 +166,9 @@ def attend_blocks(q: torch.Tensor, cache: BlockCache, cu_new: Optional[torch.Ten
                   sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
                   out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """Causal attention of the last n_b tokens of every sequence (appended before): the query at position p sees tokens
-    first[b] .. p.  q [B, n, Hq, dh], or [rows, Hq, dh] with cu_new; bf16 or f16.  Returns q's shape; zeros where a query sees
-    nothing, and padding rows are not written."""
+    first[b] .. p.  q [B, n, Hq, dh], or [rows, Hq, dh] with cu_new (rows one stride apart, as append_blocks takes them); bf16 or f16.
+    Returns q's shape; zeros where a query sees nothing, and padding rows are not written.  sm_scale as for decode_blocks.  Softmax
+    weights are rounded once to f16 (11 bits), with fp32 outputs too, and values below 2^-80 of the sequence's largest value scale count as
+    zeros; calls of up to 8 / (Hq / Hkv) tokens a sequence have decode_blocks' errors."""
     return _call("attend", cache, cache.seq_lens, (_calls or _bind())["scratch"][1], q, cu_new, first,
                  sm_scale, _type(out_dtype), out)

@@ -3,7 +3,7 @@
 // Both move bytes: a bf16 token of 8 heads of 128 dims is 4096 bytes to read and 2048 to write, and the other way round.  A warp has 16
 // slots of one (page, side, head), so a page of 16 tokens needs no barrier; the largest magnitude and the rounding work on the
 // same registers, so tokens are read once.  Measured (32768 bf16 tokens, 16-token pages, int8, cold caches): append 47 us where
-// the bytes take 31 at the copy rate, bound by instructions (16.8 an element, 70 % of issue slots at 43 % of the warps; 64 registers a thread give
+// the bytes take 31 at the copy rate, bound by instructions (16.4 an element, 70 % of issue slots at 43 % of the warps; 64 registers a thread give
 // four blocks an SM, 5 % faster than three); read 34 us, as long as the bytes take.  Steps of one token are latency: 3 us each.
 #include <type_traits>
 

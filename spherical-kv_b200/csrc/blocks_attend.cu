@@ -11,23 +11,24 @@
 //            factor as one multiplier for its 16 keys and up, weights p v / S_v in f16 back over S as the next product's
 //            operand.  The page's value scale is part of the exponent, so it costs nothing per element; the sum of p takes
 //            it out again once for 16 keys.  The row's reference is of logit and value scale together, so that f16 has the bits
-//            of what weighs most in the row, whatever scales it does not see; it puts the largest at 2^6 and moves only
-//            when one passes 2^14.  O and the tile's weights so far are then rescaled in place (every earlier product is complete:
+//            of what weighs most in the row, whatever scales it does not see; it puts the largest at 2^6 at most, is a whole
+//            number, and moves only when one passes 2^14.  O and the tile's weights so far are then rescaled in place (every earlier product is complete:
 //            S_t(k) is issued behind P_t V(k - 1)).
 // Q rows are scaled by a power of two as in the decode kernel: bf16 and f16 queries are exact in f16.  Weights have f16's 11
-// bits, sums are fp32.  A quarter of the exponentials goes through a polynomial on the fma pipe.
+// bits, rounded once, sums are fp32.  An eighth of the exponentials goes through a polynomial on the fma pipe.
 //
 // Work: (block, head, key tile) in one line, cut evenly over the CTAs; a block that two or more CTAs share is joined by a
 // second launch.
 //
-// Measured: 2048 queries x 32 heads on 32768 tokens 1.10 ms in a graph, 0.97 PFLOP/s, 59 % of what cuBLAS reaches in a burst; five
-// pieces of 301 .. 61 queries on up to 6001 tokens 102 us.  A pair of tiles (256 x 128) takes 5000 cycles.  The floor is 2048 for
+// Measured: 2048 queries x 32 heads on 32768 tokens 1.10 ms in a graph, 0.97 PFLOP/s, 59 % of what cuBLAS reaches in a burst (1.26 ms,
+// 52 %, through the public call in turn with other work, at the clocks that this leaves); on 8192 tokens 294 us, on their own 2048
+// 223 us; five pieces of 301 .. 61 queries on up to 6001 tokens 102 us; 16 x 8192 with 4 or 8 tokens a sequence 152 us.  A pair of tiles (256 x 128) takes 5000 cycles.  The floor is 2048 for
 // the products (their operands ask for 96 of shared memory's 128 bytes a cycle, the conversion for another 32) and 2048 for the
 // exponentials; what is missing is in the chain of each row tile: softmax 2950 cycles (a warp alone needs 1100 for the tile, but
 // there are five on each scheduler), weights seen by the products' warp 400, P V 460, S 570, logits seen 340 (1.29 ms while the next
 // logits came in behind all of a step's weights).  Logits of 64 keys at a time ahead of P V, in the columns that the weights leave
 // free: 1.40 ms, since a product of 64 columns takes as long as one of 128.
-// Tensor pipe 41 %, issue slots 51 %, no local memory.  Local memory is what the arrangement of the roles avoids: with all of L1
+// Tensor pipe 38 %, issue slots 49 % (8192 tokens, cold caches), no local memory.  Local memory is what the arrangement of the roles avoids: with all of L1
 // taken by shared memory a spilled word comes from L2 (1.96 ms with 512 threads and the tile's 128 logits in registers).
 #include "blocks.cuh"
 

@@ -18,11 +18,12 @@
 // A segment's tiles go round the CTA's warps; each warp keeps maxima, sums and outputs of its own, with its own ring of
 // tiles that TMA fills (three of 4 KB: 192 KB on their way per SM), so nothing is shared until the segment's end.
 //
-// Measured (graph replay; codes and outputs at the copy rate of 6563 GB/s in brackets): 8 x 32768 tokens x 8 heads of 128 dims 96 us
-// in int8, 101 in e4m3 (82); 1 x 131072 64 (41); 16 x 8192 57 (41: of 128 units on 148 CTAs most CTAs have two segments, and
-// a segment's beginning and end take 3 us each); 1 x 2048 of 64 dims 13, all of it latency: work dealt 1.2 us, addresses and
-// first tiles 1, tiles 0.8, warps joined 0.8, then the second launch.  DRAM 56 % at 8 x 16384 under cold caches, issue slots 56 %
-// (268 instructions a tile), tensor pipe 24 %: with 16 warps neither bandwidth nor issue is full, the warps' own chains are long.
+// Measured (graph replay; codes and outputs at the copy rate of 6563 GB/s in brackets): 8 x 32768 tokens x 8 heads of 128 dims 100 us
+// in int8, 97 .. 100 in e4m3 (82); 1 x 131072 58 (41); 16 x 8192 59 (41: of 128 units on 148 CTAs most CTAs have two segments, and
+// a segment's beginning and end take 3 us each), two tokens each 60; 1 x 2048 of 64 dims 13, latency: 3.8 us inside the kernel
+// are accounted for (work dealt 1.2, addresses and first tiles 1, tiles 0.8, warps joined 0.8), its launch and end and the second
+// launch are not taken apart.  DRAM 55 % at 8 x 16384 under cold caches, issue slots 56 % (464 instructions a tile in int8, 366
+// in e4m3), tensor pipe 23 %: with 16 warps neither bandwidth nor issue is full, the warps' own chains are long.
 #include <cmath>
 
 #include "blocks.cuh"

@@ -2,8 +2,8 @@
 //
 // Host time between the read of the table sizes and the next launch is what bounds a short prompt; ten
 // allocations, or ten views made from Python, cost 1.3-2 us each, and as much the three of an encode.  And the calls of the
-// block cache: their arguments' checks, outputs and workspaces (a decode of one short sequence took 24 us of host time
-// from Python, 13 us of the GPU's).  Everything that computes is in libsphkv_b200.so behind the C ABI.
+// block cache: their arguments' checks, outputs and workspaces (12 to 27 us of host time a call from Python, 7 to
+// 15 here, where one short sequence's decode takes 13 us of the GPU's).  Everything that computes is in libsphkv_b200.so behind the C ABI.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
