@@ -413,7 +413,8 @@ int sphkv_omega_ema(const float* ml, float* omega, int32_t n_units, int32_t kv_g
  * Their rows in the dense tensors are cu[b] .. cu[b + 1] - 1 (cu: device i32 [B + 1], ascending;
  * rows before cu[0] and from cu[B] on are left alone), or b * n .. b * n + n - 1 with n = rows / B where cu is NULL.
  * A sequence whose numbers do not fit (ends outside [0, max_blocks * page_size], cu not ascending
- * within [0, rows], n_b > ends[b]) is left out and raises SPHKV_ST_BAD_LENGTH in *status; a table
+ * within [0, rows], n_b > ends[b]) is left out and raises SPHKV_ST_BAD_LENGTH in *status (where cu descends,
+ * sequences beside it may be left out as well); a table
  * entry outside [0, n_pages) raises SPHKV_ST_BAD_BLOCK and its tokens count as absent. */
 #define SPHKV_BLOCKS_I8 0
 #define SPHKV_BLOCKS_E4M3 1

@@ -31,10 +31,10 @@ struct BlockPiece {
 __device__ __forceinline__ void bad_status(const sphkv_blocks& c, int bit) {
   if (c.status) atomicOr(c.status, bit);
 }
+__device__ __forceinline__ bool bad_rows(const BlockRows& r, int lo, int hi) { return lo < 0 || hi < lo || hi > r.rows; }
 __device__ __forceinline__ BlockPiece checked_piece(const sphkv_blocks& c, const BlockRows& r, int b, int j, int lo, int hi, int end) {
   BlockPiece p = {b, j, lo, hi - lo, end};
-  if (b < 0 || j < 0 || lo < 0 || hi < lo || hi > r.rows) {  // j < 0: a slot of rows before cu[0], which are no sequence's
-    if (b >= 0 && j >= 0) bad_status(c, SPHKV_ST_BAD_LENGTH);
+  if (b < 0 || j < 0 || bad_rows(r, lo, hi)) {  // j < 0: a slot of rows before cu[0], which are no sequence's
     p.b = -1;
     p.n = 0;
     return p;
@@ -54,6 +54,8 @@ __device__ __forceinline__ int slot_base(const BlockRows& r, int cu, int b, int 
 }
 
 // Called by whole warps; every lane gets the answer.  Everything that may be the answer is read before it is known which is.
+// Whoever looks for the last slot reads all of cu, so offsets that do not fit are reported wherever they stand: where they descend,
+// a sequence may have no slots that lead to it.
 __device__ __forceinline__ BlockPiece find_piece(const sphkv_blocks& c, const BlockRows& r, int slot, int shift, int extra) {
   if (r.cu == nullptr) return even_piece(c, r, slot, shift, extra);
   int b = -1, base = 0, lo = 0, hi = 0, end = 0;
@@ -61,6 +63,7 @@ __device__ __forceinline__ BlockPiece find_piece(const sphkv_blocks& c, const Bl
     const int i = min(b0 + (int)(threadIdx.x & 31), c.B - 1);
     const bool there = b0 + (int)(threadIdx.x & 31) < c.B;
     const int from = r.cu[i], to = r.cu[i + 1], e = c.ends[i];
+    if (there && bad_rows(r, from, to)) bad_status(c, SPHKV_ST_BAD_LENGTH);
     const int mine = there ? slot_base(r, from, i, shift, extra) : 0x7fffffff;
     const unsigned below = __ballot_sync(0xffffffffu, mine <= slot);
     if (below == 0) break;
@@ -74,9 +77,10 @@ __device__ __forceinline__ BlockPiece find_piece(const sphkv_blocks& c, const Bl
   }
   return checked_piece(c, r, b, slot - base, lo, hi, end);
 }
-// The same by one thread.
+// The same by one thread.  There is a slot for every sequence, and whoever looks for it reports that sequence's offsets.
 __device__ __forceinline__ BlockPiece find_piece_alone(const sphkv_blocks& c, const BlockRows& r, int slot, int shift, int extra) {
   if (r.cu == nullptr) return even_piece(c, r, slot, shift, extra);
+  if (slot < c.B && bad_rows(r, r.cu[slot], r.cu[slot + 1])) bad_status(c, SPHKV_ST_BAD_LENGTH);
   int lo = 0;  // the last sequence whose slots begin at or before this one
   if (c.B <= 32) {  // loads that do not wait for one another
 #pragma unroll 8

@@ -532,3 +532,24 @@ def test_drawn_batches(pkg, seed):
             fits = want.abs() < 0.99 * largest  # beyond, f16 has infinities
             least = _least(qq, kk, scale, pos, scales, orc.TOP[store], lo)
             _check(torch.where(fits.to(DEV), got.double(), want.to(DEV)), want, bound + half * size + least, got.dtype)
+
+
+@pytest.mark.parametrize("times", [1, 37])
+@pytest.mark.parametrize("cu", [[0, 7, 3, 10], [5, 2, 9], [0, 4, 12, 8], [0, 9, 1, 2, 3, 4, 12], [0, 13], [-1, 4], "long"])
+def test_offsets_that_do_not_ascend_are_reported(pkg, cu, times):
+    """In every operator, wherever the bad pair stands and whichever sequences its neighbours' rows go to."""
+    if cu == "long":
+        cu = list(range(0, 140, 2))
+        cu[50] = 3
+    B, rows, H, N, dh = len(cu) - 1, 12 * times if len(cu) < 9 else 140 * times, 2, 16, 64
+    ctx = 16 * times + 300
+    cache = _filled(pkg, [ctx] * B, H, N, dh, I8, 23)
+    c = torch.tensor([x * times for x in cu], dtype=torch.int32, device=DEV)
+    k = _random((rows, H, dh), 5, torch.bfloat16).to(DEV)
+    q = _random((rows, 4, dh), 6, torch.bfloat16).to(DEV)
+    for call in (lambda: pkg.read_blocks(cache, cu_rows=c, rows=rows), lambda: pkg.attend_blocks(q, cache, cu_new=c),
+                 lambda: pkg.append_blocks(cache, k, k, cu_new=c)):
+        pkg.check_status(cache)
+        call()
+        with pytest.raises(pkg.SphKVError, match="do not fit"):
+            pkg.check_status(cache)
