@@ -553,3 +553,47 @@ def test_offsets_that_do_not_ascend_are_reported(pkg, cu, times):
         call()
         with pytest.raises(pkg.SphKVError, match="do not fit"):
             pkg.check_status(cache)
+
+
+def test_recorded_calls_follow_lengths_and_offsets(pkg):
+    """More sequences than a block deals by itself, recorded once in two graphs that replay in turn while lengths, offsets and firsts change on the
+    device, in front of a bound of rows that is never reached."""
+    B, H, N, dh, Hq, rows = 150, 2, 16, 64, 4, 700
+    steps = [[(7 * b + 3 * i) % 9 for b in range(B)] for i in range(3)]
+    final = [sum(s[b] for s in steps) + 1 for b in range(B)]
+    caches = [_cache(pkg, [0] * B, H, N, dh, I8, 31, max_len=final) for _ in range(2)]
+    k, v, q = (_random((3, rows, h, dh), 40 + h + i, torch.bfloat16).to(DEV) for i, h in enumerate((H, H, Hq)))
+    held = [torch.zeros_like(x[0]) for x in (k, v, q)]
+    cu, first = torch.zeros(B + 1, dtype=torch.int32, device=DEV), torch.zeros(B, dtype=torch.int32, device=DEV)
+
+    def step(cache, kk, vv, qq, c, f):
+        pkg.append_blocks(cache, kk, vv, cu_new=c)
+        out = torch.full((rows, Hq, dh), 7.0, dtype=torch.bfloat16, device=DEV)
+        pkg.attend_blocks(qq, cache, cu_new=c, first=f, out=out)
+        back = tuple(torch.full((rows, H, dh), 7.0, device=DEV) for _ in range(2))
+        pkg.read_blocks(cache, cu_rows=c, out=back)
+        return (out, pkg.decode_blocks(qq[:B], cache, first=f)) + back
+    step(caches[1], *held, cu, first)  # nothing to do, but loads the kernels
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step(caches[1], *held, cu, first))
+        graphs.append(graph)
+    lens = [0] * B
+    for i, news in enumerate(steps):
+        lens = [a + b for a, b in zip(lens, news)]
+        for c in caches:
+            c.seq_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        cu.copy_(_cu(news))
+        first.copy_(torch.tensor([n // 3 for n in lens], dtype=torch.int32))
+        for x, y in zip(held, (k, v, q)):
+            x.copy_(y[i])
+        want = step(caches[0], k[i], v[i], q[i], cu, first)
+        graphs[i % 2].replay()
+        for a, b in zip(outs[i % 2], want):
+            assert torch.equal(a, b)
+        assert (want[0][sum(news):] == 7.0).all() and want[0][:sum(news)].isfinite().all()
+    for c in caches:
+        pkg.check_status(c)
